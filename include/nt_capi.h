@@ -71,7 +71,13 @@ typedef enum NtTrainingKernelType {
     NT_TRAIN_FINALIZE = 2        /* network gradients only, latents frozen */
 } NtTrainingKernelType;
 
-typedef enum NtDtype { NT_DTYPE_F16 = 0, NT_DTYPE_F32 = 1, NT_DTYPE_U8 = 2, NT_DTYPE_I32 = 3 } NtDtype;
+typedef enum NtDtype {
+    NT_DTYPE_F16 = 0,
+    NT_DTYPE_F32 = 1,
+    NT_DTYPE_U8 = 2,
+    NT_DTYPE_I32 = 3,
+    NT_DTYPE_BF16 = 4 /* texel-layer operators only: checkpoints do not store it */
+} NtDtype;
 
 /* Opaque CUDA stream (cudaStream_t); NULL means the legacy default stream. */
 typedef void *nt_stream_t;
@@ -492,6 +498,113 @@ NT_API nt_status nt_nccl_train_step(NtNcclComm *comm, const NtShard *shard, void
  * and NT_ERR_TIMEOUT when the time ran out; in both error cases the communicator is aborted (its
  * ranks' pending operations end with an error) and must be destroyed. */
 NT_API nt_status nt_nccl_comm_wait(NtNcclComm *comm, int32_t timeout_ms);
+
+/* ---- texel layers: channels-last group normalisation, 4-bit microscaled matrices ----------
+ * (no reference counterpart: the reference's network is one fixed per-texel MLP)
+ *
+ * The operators of a layer that maps a channels-last feature map [image][row][texel][channel]
+ * to another one texel by texel: normalisation with an activation, then a product with a weight
+ * matrix, both of its operands in 4 bits.  They take fp16, bf16 and fp32 (NtDtype), queue their
+ * work on `stream`, allocate nothing and may be captured into a graph. */
+typedef enum NtActivation {
+    NT_ACT_NONE = 0,
+    NT_ACT_RELU = 1,
+    NT_ACT_SILU = 2, /* z / (1 + exp(-z)) */
+    NT_ACT_GELU = 3  /* z (1 + erf(z / sqrt 2)) / 2 */
+} NtActivation;
+
+/* A feature map: element (n, y, x, c) is data[n * image_stride + y * row_stride +
+ * x * texel_stride + c], strides in elements.  Maps that are read may have any strides (0 repeats
+ * a texel, a row or an image); maps that are written must not overlap themselves. */
+typedef struct NtFeatureMap {
+    void *data;
+    int64_t image_stride;
+    int64_t row_stride;
+    int64_t texel_stride;
+} NtFeatureMap;
+
+/* Group normalisation.  Per image n and group g of channels / groups consecutive channels, over
+ * the group's values on all texels: mean, rstd = 1 / sqrt(variance + epsilon) (biased variance);
+ *   h = (x - mean) rstd,  z = gamma[c] h + beta[c],  y = activation(z).
+ * Statistics and sums are fp32 (centred, so a large common offset costs no digits); y is rounded
+ * once.  A NaN or an infinity makes its own group NaN and no other.  Results do not depend on
+ * the order in which thread blocks run. */
+#define NT_GROUP_NORM_MAX_CHANNELS 8192
+typedef struct NtGroupNorm {
+    int32_t images;   /* may be 0: nothing to do (backward: dgamma = dbeta = 0) */
+    int32_t height;
+    int32_t width;    /* height * width < 2^31 */
+    int32_t channels; /* 1 .. NT_GROUP_NORM_MAX_CHANNELS, a multiple of groups */
+    int32_t groups;
+    int32_t dtype;    /* of x, y, dy and dx */
+    int32_t activation;
+    float epsilon;    /* > 0 */
+    NtFeatureMap x;
+    const float *gamma; /* [channels], or NULL for 1 */
+    const float *beta;  /* [channels], or NULL for 0 */
+    float *mean;        /* [images][groups]: written by the forward call (NULL: not wanted), read by */
+    float *rstd;        /* the backward call                                                        */
+    NtFeatureMap y;     /* forward; may be x itself (same data and strides) */
+    NtFeatureMap dy;    /* backward */
+    NtFeatureMap dx;    /* backward; may be x or dy itself */
+    float *dgamma;      /* backward: [channels], overwritten; NULL: not wanted */
+    float *dbeta;
+    void *workspace;    /* device, 16-byte aligned, any contents */
+    int64_t workspace_bytes;
+} NtGroupNorm;
+
+/* Device bytes of the workspace that the call needs (backward != 0: nt_group_norm_backward); 0 if
+ * it needs none or the sizes are invalid. */
+NT_API size_t nt_group_norm_workspace_bytes(const NtGroupNorm *p, int32_t backward);
+NT_API nt_status nt_group_norm_forward(const NtGroupNorm *p, nt_stream_t stream);
+/* With e = dy activation'(z): dbeta[c] = sum e, dgamma[c] = sum e h over images and texels, and
+ * dx = rstd (gamma e - (s1 + h s2) / M), s1 = sum gamma e, s2 = sum gamma e h over the M values of
+ * the group: the gradient through mean and rstd, which are read from the forward call. */
+NT_API nt_status nt_group_norm_backward(const NtGroupNorm *p, nt_stream_t stream);
+
+/* A rows x cols matrix in 4-bit microscaled form.  Values are E2M1 codes (sign, 2 exponent bits,
+ * 1 mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6) times the scale of their block of consecutive
+ * columns: `block` 32 with power-of-two scales (E8M0: 2^(byte - 127)) or `block` 16 with E4M3
+ * scales.
+ *   data    code of column c in byte c / 2 of its row, low nibble first; rows `pitch` bytes apart
+ *           (a multiple of 16, at least nt_mx4_pitch(cols)); codes past cols are 0
+ *   scales  tiles of 128 rows x 4 blocks, 512 bytes each, tile (i, j) at 512 (i T + j) with
+ *           T = ceil(cols / (4 block)); row r, block k of a tile at byte
+ *           16 (r % 32) + 4 (r / 32) + k: the order in which the tensor cores take them;
+ *           scales past the matrix are 0
+ * Both 16-byte aligned device memory. */
+typedef struct NtMx4Matrix {
+    void *data;
+    void *scales;
+    int64_t pitch;
+    int32_t rows; /* may be 0 */
+    int32_t cols; /* >= 1 */
+    int32_t block; /* 16 or 32 */
+} NtMx4Matrix;
+
+/* Bytes of one row of codes: ceil(cols / 32) * 16 (0 if cols < 1). */
+NT_API size_t nt_mx4_pitch(int32_t cols);
+/* Bytes of the scale array (0 if the sizes are invalid or rows is 0). */
+NT_API size_t nt_mx4_scales_bytes(int32_t rows, int32_t cols, int32_t block);
+/* Quantises x (element (r, c) at src[r * row_stride + c * col_stride], strides in elements, any
+ * non-negative values: a transposed matrix is read in place) into dst, padding included.  With a the
+ * largest magnitude of a block:
+ *   block 32: scale = 2^max(floor(log2 a) - 2, -127)
+ *   block 16: scale = a / 6 in fp32, rounded to E4M3 (nearest, ties to even; at most 448)
+ * and code = x / scale rounded to the nearest E2M1 value (ties to the even code), at most 6 in
+ * magnitude; 0 where the scale is 0.  The sign is kept, of zeros too.  A block that holds a NaN or
+ * an infinity gets the NaN scale (0xff / 0x7f), so that everything made from it is NaN. */
+NT_API nt_status nt_mx4_quantize(const void *src, int32_t dtype, int64_t row_stride, int64_t col_stride,
+                                 const NtMx4Matrix *dst, nt_stream_t stream);
+/* code * scale, rounded to dtype, to dst[r * row_stride + c] (row_stride >= cols). */
+NT_API nt_status nt_mx4_dequantize(const NtMx4Matrix *src, void *dst, int32_t dtype, int64_t row_stride,
+                                   nt_stream_t stream);
+/* d[m * row_stride + n] = activation(alpha sum_k a[m][k] b[n][k] + bias[n]), rounded to dtype once; a is
+ * M x K, b is N x K with the same block size, bias [N] fp32 or NULL, sums in fp32.  Runs on the
+ * tensor cores' block-scaled product.  The result does not depend on the order in which thread
+ * blocks run. */
+NT_API nt_status nt_mx4_product(const NtMx4Matrix *a, const NtMx4Matrix *b, const float *bias, int32_t activation,
+                                float alpha, void *d, int32_t dtype, int64_t row_stride, nt_stream_t stream);
 
 /* ---- tensor-core self-test (no reference counterpart) ---------------------------------- */
 

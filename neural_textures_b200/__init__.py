@@ -33,3 +33,11 @@ from .api import (  # noqa: F401
     run_forward_pass_test,
     train_step,
 )
+from .layers import (  # noqa: F401
+    Mx4Tensor,
+    group_norm,
+    group_norm_backward,
+    mx4_dequantize,
+    mx4_product,
+    mx4_quantize,
+)

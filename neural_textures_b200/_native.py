@@ -30,6 +30,11 @@ NT_DTYPE_F16 = 0
 NT_DTYPE_F32 = 1
 NT_DTYPE_U8 = 2
 NT_DTYPE_I32 = 3
+NT_DTYPE_BF16 = 4
+NT_ACT_NONE = 0
+NT_ACT_RELU = 1
+NT_ACT_SILU = 2
+NT_ACT_GELU = 3
 NT_CKPT_NAME_LEN = 32
 NT_MAX_REFERENCE_TEXTURES = 16
 
@@ -118,6 +123,25 @@ class NtBc6hSurface(C.Structure):
                 ("channel_stride", C.c_int64), ("row_stride", C.c_int64), ("texel_stride", C.c_int64)]
 
 
+class NtFeatureMap(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("image_stride", C.c_int64), ("row_stride", C.c_int64),
+                ("texel_stride", C.c_int64)]
+
+
+class NtGroupNorm(C.Structure):
+    _fields_ = [("images", C.c_int32), ("height", C.c_int32), ("width", C.c_int32), ("channels", C.c_int32),
+                ("groups", C.c_int32), ("dtype", C.c_int32), ("activation", C.c_int32), ("epsilon", C.c_float),
+                ("x", NtFeatureMap), ("gamma", C.c_void_p), ("beta", C.c_void_p), ("mean", C.c_void_p),
+                ("rstd", C.c_void_p), ("y", NtFeatureMap), ("dy", NtFeatureMap), ("dx", NtFeatureMap),
+                ("dgamma", C.c_void_p), ("dbeta", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_int64)]
+
+
+class NtMx4Matrix(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("scales", C.c_void_p), ("pitch", C.c_int64), ("rows", C.c_int32),
+                ("cols", C.c_int32), ("block", C.c_int32)]
+
+
 # Every symbol include/nt_capi.h declares: name -> (restype, argtypes)
 _P = C.POINTER(NtKernelParams)
 _S = C.POINTER(NtBc6hSurface)
@@ -165,6 +189,16 @@ SIGNATURES = {
                                       C.POINTER(C.c_int32)]),
     "nt_checkpoint_read": (C.c_int, [C.c_char_p, C.c_char_p, C.c_void_p, C.c_int64]),
     "nt_build_mips": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p]),
+    # parameter blocks as c_void_p: layers.py passes them packed as bytes, C.byref works too
+    "nt_group_norm_workspace_bytes": (C.c_size_t, [C.c_void_p, C.c_int32]),
+    "nt_group_norm_forward": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "nt_group_norm_backward": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "nt_mx4_pitch": (C.c_size_t, [C.c_int32]),
+    "nt_mx4_scales_bytes": (C.c_size_t, [C.c_int32] * 3),
+    "nt_mx4_quantize": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p]),
+    "nt_mx4_dequantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_void_p]),
+    "nt_mx4_product": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_float, C.c_void_p, C.c_int32,
+                                 C.c_int64, C.c_void_p]),
     "nt_nccl_unique_id": (C.c_int, [C.c_void_p]),
     "nt_nccl_comm_create": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_void_p)]),
     "nt_nccl_comm_destroy": (C.c_int, [C.c_void_p]),

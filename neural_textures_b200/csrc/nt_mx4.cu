@@ -1,0 +1,332 @@
+// nt_mx4.cu -- 4-bit microscaled matrices: quantisation from fp16 / bf16 / fp32 and back
+// (nt_mx4_quantize, nt_mx4_dequantize).
+#include "nt_mx4.cuh"
+
+namespace nt {
+namespace mx4 {
+
+constexpr int kThreads = 256;
+constexpr int kGroupCols = 128;  // columns of one thread block of the quantise kernels
+
+struct QuantizeLaunch {
+    const void *src;
+    int64_t row_stride, col_stride;
+    uint8_t *data, *scales;
+    int64_t pitch;
+    int32_t rows, cols, tiles, groups;  // scale tiles a row of tiles; column groups
+};
+
+// 16 values of a row from column c (0 past the matrix).
+template <class T, bool VEC>
+__device__ __forceinline__ void load16(const QuantizeLaunch &p, int64_t row, int64_t c, T (&v)[16])
+{
+    const T *src = static_cast<const T *>(p.src) + row * p.row_stride;
+    if (VEC && row < p.rows && c + 16 <= p.cols) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T); ++i)
+            reinterpret_cast<uint4 *>(v)[i] = __ldg(reinterpret_cast<const uint4 *>(src + c) + i);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const bool in = row < p.rows && c + i < p.cols;
+        v[i] = in ? src[(c + i) * p.col_stride] : from_f32<T>(0.f);
+    }
+}
+
+// The bits of max |v| as fp32; NaN and infinity compare above every number as integers.
+template <class T, int N>
+__device__ __forceinline__ uint32_t amax_bits(const T (&v)[N])
+{
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = max(m, __float_as_uint(to_f32(v[i])) & 0x7fffffffu);
+    return m;
+}
+
+template <class T, int BLOCK, int N>
+__device__ __forceinline__ void quantize_codes(const T (&v)[N], uint32_t byte, uint32_t (&codes)[N / 8])
+{
+    const float inv = inverse_scale<BLOCK>(byte), s = BLOCK == 16 ? scale_value<16>(byte) : 0.f;
+#pragma unroll
+    for (int q = 0; q < N / 8; ++q) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = scaled<BLOCK, sizeof(T) == 4>(to_f32(v[8 * q + i]), inv, s);
+        codes[q] = codes8(f);
+    }
+}
+
+// Rows along the memory.  A thread block takes 128 rows x 128 columns.  BLOCK / 4 lanes share a row
+// (16 values each), so that they hold the four scales of one word; a lane takes rows r, r + 32,
+// r + 64 and r + 96, whose words are the 16 bytes of row r in the scale tile: one store.
+template <class T, int BLOCK, bool VEC>
+__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeLaunch p)
+{
+    constexpr int LPR = BLOCK / 4, RPW = 32 / LPR;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t tile = blockIdx.x / p.groups;
+    const int group = blockIdx.x % p.groups;
+    const int half = BLOCK == 16 ? warp >> 2 : 0;
+    const int residue = (BLOCK == 16 ? warp & 3 : warp) * RPW + lane / LPR;
+    const int64_t c = (int64_t)group * kGroupCols + half * 64 + (lane % LPR) * 16;
+    uint32_t words[4];
+    constexpr int U = sizeof(T) == 2 ? 4 : 2;  // rows in flight
+#pragma unroll
+    for (int j0 = 0; j0 < 4; j0 += U) {
+        alignas(16) T v[U][16];
+#pragma unroll
+        for (int u = 0; u < U; ++u) load16<T, VEC>(p, tile * kTileRows + (j0 + u) * 32 + residue, c, v[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t row = tile * kTileRows + (j0 + u) * 32 + residue;
+            uint32_t m = amax_bits(v[u]);
+            if (BLOCK == 32) m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            const uint32_t byte = scale_byte<BLOCK>(m);
+            uint32_t codes[2];
+            quantize_codes<T, BLOCK>(v[u], byte, codes);
+            if (row < p.rows && c < row_pitch(p.cols) * 2)
+                *reinterpret_cast<uint2 *>(p.data + row * p.pitch + (c >> 1)) = make_uint2(codes[0], codes[1]);
+            uint32_t w = byte << (8 * ((lane % LPR) * 16 / BLOCK));
+            w |= __shfl_xor_sync(0xffffffffu, w, LPR / 2);
+            w |= __shfl_xor_sync(0xffffffffu, w, LPR / 4);
+            words[j0 + u] = w;
+        }
+    }
+    const int tcol = BLOCK == 16 ? group * 2 + half : group;
+    if (lane % LPR == 0 && tcol < p.tiles)
+        *reinterpret_cast<uint4 *>(p.scales + (tile * p.tiles + tcol) * kTileBytes + residue * 16) =
+            make_uint4(words[0], words[1], words[2], words[3]);
+}
+
+// Columns along the memory (a transposed matrix): lane = row, so that a warp's load of one column is
+// contiguous; a thread quantises 64 columns of its row, 32 bytes of codes, without any exchange.
+template <class T, int BLOCK>
+__global__ void __launch_bounds__(kThreads) quantize_columns_kernel(const QuantizeLaunch p)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t tile = blockIdx.x / p.groups;
+    const int group = blockIdx.x % p.groups;
+    const int j = warp & 3, half = warp >> 2;
+    const int64_t row = tile * kTileRows + j * 32 + lane;
+    const int64_t c0 = (int64_t)group * kGroupCols + half * 64;
+    const T *src = static_cast<const T *>(p.src) + row;
+    uint32_t word = 0;
+#pragma unroll
+    for (int b = 0; b < 64 / 32; ++b) {
+        T v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const int64_t c = c0 + 32 * b + i;
+            v[i] = row < p.rows && c < p.cols ? src[c * p.col_stride] : from_f32<T>(0.f);
+        }
+        uint32_t codes[4];
+        if (BLOCK == 32) {
+            const uint32_t byte = scale_byte<32>(amax_bits(v));
+            quantize_codes<T, 32>(v, byte, codes);
+            word |= byte << (8 * b);
+        } else {
+            T(&lo)[16] = *reinterpret_cast<T(*)[16]>(&v[0]);
+            T(&hi)[16] = *reinterpret_cast<T(*)[16]>(&v[16]);
+            const uint32_t b0 = scale_byte<16>(amax_bits(lo)), b1 = scale_byte<16>(amax_bits(hi));
+            quantize_codes<T, 16>(lo, b0, *reinterpret_cast<uint32_t(*)[2]>(&codes[0]));
+            quantize_codes<T, 16>(hi, b1, *reinterpret_cast<uint32_t(*)[2]>(&codes[2]));
+            word |= (b0 | b1 << 8) << (16 * b);
+        }
+        const int64_t c = c0 + 32 * b;
+        if (row < p.rows && c < row_pitch(p.cols) * 2)
+            *reinterpret_cast<uint4 *>(p.data + row * p.pitch + (c >> 1)) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+    }
+    const int tcol = BLOCK == 16 ? group * 2 + half : group;
+    if (tcol < p.tiles) {
+        uint8_t *at = p.scales + (tile * p.tiles + tcol) * kTileBytes + lane * 16 + j * 4;
+        if (BLOCK == 16) *reinterpret_cast<uint32_t *>(at) = word;
+        else *reinterpret_cast<uint16_t *>(at + 2 * half) = (uint16_t)word;
+    }
+}
+
+template <class T, int BLOCK>
+cudaError_t launch_quantize(QuantizeLaunch p, cudaStream_t st)
+{
+    p.tiles = tiles_per_row(p.cols, BLOCK);
+    p.groups = (int32_t)(((int64_t)p.cols + kGroupCols - 1) / kGroupCols);
+    const int64_t blocks = ((int64_t)p.rows + kTileRows - 1) / kTileRows * p.groups;
+    if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    const bool vec = p.col_stride == 1 && is_aligned(p.src, 16) && p.row_stride * sizeof(T) % 16 == 0;
+    if (vec) quantize_rows_kernel<T, BLOCK, true><<<(unsigned)blocks, kThreads, 0, st>>>(p);
+    else if (p.row_stride == 1 && p.col_stride != 1) quantize_columns_kernel<T, BLOCK><<<(unsigned)blocks, kThreads, 0, st>>>(p);
+    else quantize_rows_kernel<T, BLOCK, false><<<(unsigned)blocks, kThreads, 0, st>>>(p);
+    count_launch();
+    return cudaGetLastError();
+}
+
+// ---- back --------------------------------------------------------------------------------
+
+struct DequantizeLaunch {
+    const uint8_t *data, *scales;
+    void *dst;
+    int64_t pitch, row_stride;
+    int32_t rows, cols, tiles;
+    int32_t lanes_log2;  // lanes that share a row
+    int32_t col_blocks;  // thread blocks that share a row
+    int32_t vec;         // 16-byte stores
+};
+
+constexpr int kDequantRows = 4;  // rows of one lane
+
+// A lane takes 8 codes (one word) of a row and writes 16 or 32 bytes.
+template <class T, int BLOCK>
+__global__ void __launch_bounds__(kThreads) dequantize_kernel(const DequantizeLaunch p)
+{
+    const int lanes = 1 << p.lanes_log2;
+    const int sub = threadIdx.x & (lanes - 1);
+    const int rows_per_pass = kThreads >> p.lanes_log2;
+    const int64_t row0 =
+        (int64_t)(blockIdx.x / p.col_blocks) * rows_per_pass * kDequantRows + (threadIdx.x >> p.lanes_log2);
+    const int64_t c = ((int64_t)(blockIdx.x % p.col_blocks) * lanes + sub) * 8;
+    if (c >= p.cols) return;
+    uint32_t codes[kDequantRows], bytes[kDequantRows];
+#pragma unroll
+    for (int j = 0; j < kDequantRows; ++j) {
+        const int64_t row = row0 + (int64_t)j * rows_per_pass;
+        if (row >= p.rows) break;
+        codes[j] = __ldg(reinterpret_cast<const uint32_t *>(p.data + row * p.pitch + (c >> 1)));
+        bytes[j] = __ldg(p.scales + scale_at(row, (int)(c / BLOCK), p.tiles));
+    }
+#pragma unroll
+    for (int j = 0; j < kDequantRows; ++j) {
+        const int64_t row = row0 + (int64_t)j * rows_per_pass;
+        if (row >= p.rows) break;
+        const float s = scale_value<BLOCK>(bytes[j]);
+        uint32_t h2[4];
+        values8(codes[j], h2);
+        alignas(16) T out[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h2[i]));
+            out[2 * i] = from_f32<T>(f.x * s);
+            out[2 * i + 1] = from_f32<T>(f.y * s);
+        }
+        T *dst = static_cast<T *>(p.dst) + row * p.row_stride + c;
+        if (p.vec && c + 8 <= p.cols) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+                reinterpret_cast<uint4 *>(dst)[i] = reinterpret_cast<const uint4 *>(out)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < p.cols) dst[i] = out[i];
+        }
+    }
+}
+
+template <class T, int BLOCK>
+cudaError_t launch_dequantize(DequantizeLaunch p, cudaStream_t st)
+{
+    p.tiles = tiles_per_row(p.cols, BLOCK);
+    const int64_t words = ((int64_t)p.cols + 7) / 8;
+    p.lanes_log2 = 0;
+    while (p.lanes_log2 < 5 && (1 << p.lanes_log2) < words) ++p.lanes_log2;
+    p.vec = is_aligned(p.dst, 16) && p.row_stride * sizeof(T) % 16 == 0;
+    p.col_blocks = (int32_t)((words + (1 << p.lanes_log2) - 1) >> p.lanes_log2);
+    const int64_t rows_per_block = (int64_t)(kThreads >> p.lanes_log2) * kDequantRows;
+    const int64_t grid = ((int64_t)p.rows + rows_per_block - 1) / rows_per_block * p.col_blocks;
+    if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    dequantize_kernel<T, BLOCK><<<(unsigned)grid, kThreads, 0, st>>>(p);
+    count_launch();
+    return cudaGetLastError();
+}
+
+// Shared checks of a matrix argument.
+nt_status check_matrix(const NtMx4Matrix *m, const char *name)
+{
+    NT_LAYER_REQUIRE(m, "%s is null", name);
+    NT_LAYER_REQUIRE(m->block == 16 || m->block == 32, "%s: block must be 16 or 32 (got %d)", name, m->block);
+    NT_LAYER_REQUIRE(m->rows >= 0 && m->cols >= 1, "%s: %d x %d is not a matrix size", name, m->rows, m->cols);
+    NT_LAYER_REQUIRE(m->pitch >= row_pitch(m->cols) && m->pitch % 16 == 0,
+                     "%s: pitch must be a multiple of 16 and at least %lld (got %lld)", name,
+                     (long long)row_pitch(m->cols), (long long)m->pitch);
+    NT_LAYER_REQUIRE(m->rows == 0 || (m->data && m->scales && is_aligned(m->data, 16) && is_aligned(m->scales, 16)),
+                     "%s: data and scales must be non-null 16-byte aligned device pointers", name);
+    return NT_OK;
+}
+
+}  // namespace mx4
+}  // namespace nt
+
+using namespace nt;
+
+extern "C" {
+
+size_t nt_mx4_pitch(int32_t cols) { return cols < 1 ? 0 : (size_t)mx4::row_pitch(cols); }
+
+size_t nt_mx4_scales_bytes(int32_t rows, int32_t cols, int32_t block)
+{
+    if (rows < 1 || cols < 1 || (block != 16 && block != 32)) return 0;
+    return (size_t)(((int64_t)rows + mx4::kTileRows - 1) / mx4::kTileRows) * mx4::tiles_per_row(cols, block) * mx4::kTileBytes;
+}
+
+nt_status nt_mx4_quantize(const void *src, int32_t dtype, int64_t row_stride, int64_t col_stride,
+                          const NtMx4Matrix *dst, nt_stream_t stream)
+{
+    nt_status st = mx4::check_matrix(dst, "dst");
+    if (st != NT_OK) return st;
+    const int size = layer_dtype_size(dtype);
+    NT_LAYER_REQUIRE(size, "dtype must be NT_DTYPE_F16, NT_DTYPE_BF16 or NT_DTYPE_F32 (got %d)", dtype);
+    NT_LAYER_REQUIRE(row_stride >= 0 && col_stride >= 0, "strides must be non-negative");
+    if (dst->rows == 0) return NT_OK;
+    NT_LAYER_REQUIRE(src && is_aligned(src, size), "src must be a non-null device pointer aligned to its element");
+    mx4::QuantizeLaunch p = {};
+    p.src = src;
+    p.row_stride = row_stride;
+    p.col_stride = col_stride;
+    p.data = static_cast<uint8_t *>(dst->data);
+    p.scales = static_cast<uint8_t *>(dst->scales);
+    p.pitch = dst->pitch;
+    p.rows = dst->rows;
+    p.cols = dst->cols;
+    const cudaStream_t s = (cudaStream_t)stream;
+    cudaError_t e;
+    if (dst->block == 16)
+        e = dtype == NT_DTYPE_F16    ? mx4::launch_quantize<__half, 16>(p, s)
+            : dtype == NT_DTYPE_BF16 ? mx4::launch_quantize<__nv_bfloat16, 16>(p, s)
+                                     : mx4::launch_quantize<float, 16>(p, s);
+    else
+        e = dtype == NT_DTYPE_F16    ? mx4::launch_quantize<__half, 32>(p, s)
+            : dtype == NT_DTYPE_BF16 ? mx4::launch_quantize<__nv_bfloat16, 32>(p, s)
+                                     : mx4::launch_quantize<float, 32>(p, s);
+    return e == cudaSuccess ? NT_OK : set_error(NT_ERR_CUDA, "4-bit quantise: %s", cudaGetErrorString(e));
+}
+
+nt_status nt_mx4_dequantize(const NtMx4Matrix *src, void *dst, int32_t dtype, int64_t row_stride, nt_stream_t stream)
+{
+    nt_status st = mx4::check_matrix(src, "src");
+    if (st != NT_OK) return st;
+    const int size = layer_dtype_size(dtype);
+    NT_LAYER_REQUIRE(size, "dtype must be NT_DTYPE_F16, NT_DTYPE_BF16 or NT_DTYPE_F32 (got %d)", dtype);
+    NT_LAYER_REQUIRE(src->rows <= 1 || row_stride >= src->cols, "row_stride (%lld) must be at least cols (%d)",
+                     (long long)row_stride, src->cols);
+    if (src->rows == 0) return NT_OK;
+    NT_LAYER_REQUIRE(dst && is_aligned(dst, size), "dst must be a non-null device pointer aligned to its element");
+    mx4::DequantizeLaunch p = {};
+    p.data = static_cast<const uint8_t *>(src->data);
+    p.scales = static_cast<const uint8_t *>(src->scales);
+    p.dst = dst;
+    p.pitch = src->pitch;
+    p.row_stride = row_stride;
+    p.rows = src->rows;
+    p.cols = src->cols;
+    const cudaStream_t s = (cudaStream_t)stream;
+    cudaError_t e;
+    if (src->block == 16)
+        e = dtype == NT_DTYPE_F16    ? mx4::launch_dequantize<__half, 16>(p, s)
+            : dtype == NT_DTYPE_BF16 ? mx4::launch_dequantize<__nv_bfloat16, 16>(p, s)
+                                     : mx4::launch_dequantize<float, 16>(p, s);
+    else
+        e = dtype == NT_DTYPE_F16    ? mx4::launch_dequantize<__half, 32>(p, s)
+            : dtype == NT_DTYPE_BF16 ? mx4::launch_dequantize<__nv_bfloat16, 32>(p, s)
+                                     : mx4::launch_dequantize<float, 32>(p, s);
+    return e == cudaSuccess ? NT_OK : set_error(NT_ERR_CUDA, "4-bit read-back: %s", cudaGetErrorString(e));
+}
+
+}  // extern "C"
