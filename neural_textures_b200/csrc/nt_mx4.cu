@@ -242,7 +242,7 @@ nt_status check_matrix(const NtMx4Matrix *m, const char *name)
 {
     NT_LAYER_REQUIRE(m, "%s is null", name);
     NT_LAYER_REQUIRE(m->block == 16 || m->block == 32, "%s: block must be 16 or 32 (got %d)", name, m->block);
-    NT_LAYER_REQUIRE(m->rows >= 0 && m->cols >= 1, "%s: %d x %d is not a matrix size", name, m->rows, m->cols);
+    NT_LAYER_REQUIRE(m->rows >= 0 && m->cols >= 1 && m->rows <= 0x7fffff00 && m->cols <= 0x7fffff00, "%s: %d x %d is not a matrix size", name, m->rows, m->cols);
     NT_LAYER_REQUIRE(m->pitch >= row_pitch(m->cols) && m->pitch % 16 == 0,
                      "%s: pitch must be a multiple of 16 and at least %lld (got %lld)", name,
                      (long long)row_pitch(m->cols), (long long)m->pitch);

@@ -1,14 +1,41 @@
-// nt_mx4_product.cu -- d = activation(alpha a b^T + bias) of two 4-bit microscaled matrices
-// (nt_mx4_product).
+// nt_mx4_product.cu -- d = activation(alpha a b^T + bias) of two 4-bit microscaled matrices on the
+// tensor cores' block-scaled product (nt_mx4_product).
+//
+// One operand's rows are the accumulator's 128 lanes (the lane operand), the other's its bn columns
+// (the column operand).  A thread block computes 128 x bn tiles, 256 values of K a stage:
+//   warp 0      copies: TMA tiles of codes (128-byte rows, 128-byte swizzle; zeros past the matrix)
+//               and the scale tiles, which lie in memory as tensor memory wants them
+//   warp 1      per stage: scale tiles shared -> tensor memory, four products of K = 64, commit
+//   warps 4-7   epilogue: accumulator -> scale, bias, activation, rounding -> shared -> rows of d
+// Accumulators are doubled in tensor memory, so that the epilogue of a tile runs under the products
+// of the next; blocks take tiles gridDim apart.
+//
+// Few rows (m <= 64): the weights' rows go to the lanes, and bn is m rounded up, so that a token costs no
+// empty columns.  Few tiles: a cluster of up to 8 blocks splits K, leaves its partial sums in shared
+// memory, and each block joins its share of the columns in rank order.
+//
+// Every wait is bounded; a timeout sets bit 0 of the status word that nt_read_device_status returns.
+#include <cuda.h>
+
+#include <algorithm>
+
 #include "nt_mx4.cuh"
+#include "nt_umma.cuh"
 
 namespace nt {
 namespace mx4 {
 
+__device__ unsigned int g_product_status;  // bit 0: a bounded wait gave up
+
 struct ProductLaunch {
-    const uint8_t *a, *b, *a_scales, *b_scales;
-    int64_t a_pitch, b_pitch;
-    int32_t m, n, k, tiles;
+    const uint8_t *l_scales, *c_scales;  // of the lane and the column operand
+    int32_t l_rows, c_rows, k;
+    int32_t bn, l_tiles, c_tiles;
+    int32_t scale_tiles;       // scale tiles of 128 rows of either operand
+    int32_t stages, stage_bytes;
+    int32_t split;             // thread blocks of a cluster, each with a share of K
+    int32_t swapped;           // 1: lanes are b's rows (d's columns)
+    int32_t dtype, vec;        // vec: rows of d take 16-byte stores
     const float *bias;
     int32_t activation;
     float alpha;
@@ -16,72 +43,457 @@ struct ProductLaunch {
     int64_t row_stride;
 };
 
-constexpr int kSide = 64, kStep = 32;
+constexpr int kThreads = 256;
+constexpr int kStageK = 256, kStageRow = 128;  // values and bytes of a row of a stage
+constexpr int kLaneBytes = 128 * kStageRow;
+constexpr int kMaxStages = 8;
+constexpr int kMaxBn = 128;
+constexpr int kStagePitch = 144;  // epilogue staging row: 128 bytes and a 16-byte shift of the banks
+constexpr uint32_t kTmemCols = 512, kScaleCol = 256, kScaleCols = 32;
 
-// Codes of kSide rows x kStep columns -> fp32 values [column][row].
+struct Control {
+    alignas(8) uint64_t full[kMaxStages];
+    uint64_t empty[kMaxStages];
+    uint64_t acc_full[2], acc_empty[2];
+    uint32_t tmem;
+};
+
+struct Shared {
+    alignas(128) uint8_t staging[4 * 32 * kStagePitch];
+    Control ctl;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
+__device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+// Codes: rows of 128 bytes, 8-row groups 1024 bytes apart, 128-byte swizzle.
+__device__ __forceinline__ uint64_t codes_desc(uint32_t addr)
+{
+    return umma::desc(addr, 16, 1024) | (uint64_t)2 << 61;
+}
+
+// A scale tile: 32 rows of 16 bytes -> 4 columns of all four lane quarters.
+__device__ __forceinline__ void copy_scale_tile(uint32_t tmem, uint32_t addr)
+{
+    const uint64_t d = umma::desc(addr, 0, 128);
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d) : "memory");
+}
+
+// Instruction descriptor: E2M1 operands, 128 x n, scale format (0: E4M3, 1: E8M0), the byte of each
+// scale word at which the step's scales start.
 template <int BLOCK>
-__device__ __forceinline__ void stage(const uint8_t *data, const uint8_t *scales, int64_t pitch, int rows, int cols,
-                                      int tiles, int64_t row0, int k0, float (*out)[kSide + 1])
+__device__ __forceinline__ uint32_t idesc(int n, uint32_t scale_byte)
 {
-    const int r = threadIdx.x >> 2, q = threadIdx.x & 3;  // 4 threads a row, 8 columns each
-    const int64_t row = row0 + r;
-    const int k = k0 + 8 * q;
-    uint32_t h2[4] = {0, 0, 0, 0};
-    float s = 0.f;
-    if (row < rows && k < cols) {
-        values8(*reinterpret_cast<const uint32_t *>(data + row * pitch + (k >> 1)), h2);
-        s = scale_value<BLOCK>(scales[scale_at(row, k / BLOCK, tiles)]);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h2[i]));
-        out[8 * q + 2 * i][r] = f.x * s;
-        out[8 * q + 2 * i + 1][r] = f.y * s;
-    }
+    return (scale_byte << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((BLOCK == 32 ? 1u : 0u) << 23) |
+           (8u << 24) | (scale_byte << 29);
 }
 
-template <class T, int BLOCK>
-__global__ void __launch_bounds__(256) product_kernel(const ProductLaunch p)
+template <int BLOCK>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, uint32_t sa, uint32_t sb, uint32_t acc)
 {
-    __shared__ float sa[kStep][kSide + 1], sb[kStep][kSide + 1];
-    const int64_t tiles_n = (p.n + kSide - 1) / kSide;
-    const int64_t m0 = blockIdx.x / tiles_n * kSide, n0 = blockIdx.x % tiles_n * kSide;
-    const int tm = threadIdx.x / 16, tn = threadIdx.x % 16;
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < p.k; k0 += kStep) {
-        stage<BLOCK>(p.a, p.a_scales, p.a_pitch, p.m, p.k, p.tiles, m0, k0, sa);
-        stage<BLOCK>(p.b, p.b_scales, p.b_pitch, p.n, p.k, p.tiles, n0, k0, sb);
-        __syncthreads();
-#pragma unroll 8
-        for (int k = 0; k < kStep; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[k][tm + 16 * i], sb[k][tn + 16 * j], acc[i][j]);
-        __syncthreads();
+    if (BLOCK == 16)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+            "l"(a), "l"(b), "r"(desc), "r"(sa), "r"(sb), "r"(acc)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+            "l"(a), "l"(b), "r"(desc), "r"(sa), "r"(sb), "r"(acc)
+            : "memory");
+}
+
+__device__ __forceinline__ void ld32(uint32_t taddr, uint32_t (&r)[32])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+        "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity)
+{
+    if (umma::mbar_wait(bar, parity)) return true;
+    atomicOr(&g_product_status, 1u);
+    return false;
+}
+
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ float peer_f32(uint32_t addr, uint32_t rank)
+{
+    uint32_t remote;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ void store_one(const ProductLaunch &p, int64_t at, float v)
+{
+    if (p.dtype == NT_DTYPE_F32) static_cast<float *>(p.d)[at] = v;
+    else if (p.dtype == NT_DTYPE_F16) static_cast<__half *>(p.d)[at] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16 *>(p.d)[at] = __float2bfloat16_rn(v);
+}
+
+__device__ __forceinline__ uint32_t pack2(int dtype, float lo, float hi)
+{
+    if (dtype == NT_DTYPE_F16) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
     }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int64_t m = m0 + tm + 16 * i, n = n0 + tn + 16 * j;
-            if (m >= p.m || n >= p.n) continue;
-            const float z = p.alpha * acc[i][j] + (p.bias ? p.bias[n] : 0.f);
-            static_cast<T *>(p.d)[m * p.row_stride + n] = from_f32<T>(activate(z, p.activation));
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Lanes are b's rows: lane = column of d, accumulator columns = rows of d; a warp's store is contiguous.
+__device__ __forceinline__ void epilogue_swapped(const ProductLaunch &p, uint32_t tmem, int lane0, int col0)
+{
+    const int64_t n = lane0 + (threadIdx.x & 127);
+    const float bias = p.bias && n < p.l_rows ? __ldg(p.bias + n) : 0.f;
+    for (int c0 = 0; c0 < p.bn; c0 += 32) {
+        uint32_t v[32];
+        ld32(tmem + c0, v);
+        umma::wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const int64_t m = col0 + c0 + i;
+            if (c0 + i < p.bn && m < p.c_rows && n < p.l_rows)
+                store_one(p, m * p.row_stride + n, activate(fmaf(p.alpha, __uint_as_float(v[i]), bias), p.activation));
         }
+    }
 }
 
-template <class T, int BLOCK>
-cudaError_t launch_product(const ProductLaunch &p, cudaStream_t st)
+// Lanes are a's rows: a warp turns 32 rows x 32 or 64 columns in shared memory and writes them row by row.
+__device__ __forceinline__ void epilogue_rows(const ProductLaunch &p, uint32_t tmem, int lane0, int col0, uint8_t *staging)
 {
-    const int64_t blocks = ((int64_t)p.m + kSide - 1) / kSide * (((int64_t)p.n + kSide - 1) / kSide);
-    if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    product_kernel<T, BLOCK><<<(unsigned)blocks, 256, 0, st>>>(p);
+    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) & 3;
+    const int size = p.dtype == NT_DTYPE_F32 ? 4 : 2;
+    const int width = size == 2 && p.bn % 64 == 0 ? 64 : 32;  // columns of a pass
+    uint8_t *mine = staging + warp * 32 * kStagePitch;
+    for (int c0 = 0; c0 < p.bn; c0 += width) {
+        if (col0 + c0 >= p.c_rows) break;
+        for (int s = 0; s < width; s += 32) {
+            uint32_t v[32];
+            ld32(tmem + c0 + s, v);
+            const int64_t nb = col0 + c0 + s + lane;
+            const float bias = p.bias && nb < p.c_rows ? __ldg(p.bias + nb) : 0.f;
+            umma::wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                v[i] = __float_as_uint(
+                    activate(fmaf(p.alpha, __uint_as_float(v[i]), __shfl_sync(0xffffffffu, bias, i)), p.activation));
+            uint8_t *row = mine + lane * kStagePitch + s * size;
+            if (size == 4) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    *reinterpret_cast<uint4 *>(row + 16 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t h[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        h[e] = pack2(p.dtype, __uint_as_float(v[8 * i + 2 * e]), __uint_as_float(v[8 * i + 2 * e + 1]));
+                    *reinterpret_cast<uint4 *>(row + 16 * i) = make_uint4(h[0], h[1], h[2], h[3]);
+                }
+            }
+        }
+        __syncwarp();
+        const int64_t m0 = lane0 + warp * 32, n0 = col0 + c0;
+        const int rows = (int)min((int64_t)32, p.l_rows - m0);
+        uint8_t *dst = static_cast<uint8_t *>(p.d) + (m0 * p.row_stride + n0) * size;
+        if (p.vec && n0 + width <= p.c_rows) {
+            const int per_row = width * size / 16, step = 32 / per_row;  // 4 or 8 lanes a row
+            for (int r = lane / per_row; r < rows; r += step)
+                *reinterpret_cast<uint4 *>(dst + r * p.row_stride * size + (lane % per_row) * 16) =
+                    *reinterpret_cast<const uint4 *>(mine + r * kStagePitch + (lane % per_row) * 16);
+        } else {
+            const int cols = (int)min((int64_t)width, p.c_rows - n0);
+            for (int r = 0; r < rows; ++r)
+                for (int c = lane; c < cols; c += 32) {
+                    if (size == 4)
+                        *reinterpret_cast<uint32_t *>(dst + (r * p.row_stride + c) * 4) =
+                            *reinterpret_cast<const uint32_t *>(mine + r * kStagePitch + c * 4);
+                    else
+                        *reinterpret_cast<uint16_t *>(dst + (r * p.row_stride + c) * 2) =
+                            *reinterpret_cast<const uint16_t *>(mine + r * kStagePitch + c * 2);
+                }
+        }
+        __syncwarp();
+    }
+}
+
+template <int BLOCK>
+__global__ void __launch_bounds__(kThreads, 1)
+    product_kernel(const __grid_constant__ CUtensorMap l_map, const __grid_constant__ CUtensorMap c_map, const ProductLaunch p)
+{
+    constexpr int kTiles = BLOCK == 16 ? 4 : 2;  // scale tiles of a stage
+    extern __shared__ uint8_t raw[];
+    __shared__ Shared sh;
+    Control &ctl = sh.ctl;
+    uint8_t *stages = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t base = smem_u32(stages), full = smem_u32(ctl.full), empty = smem_u32(ctl.empty),
+                   acc_full = smem_u32(ctl.acc_full), acc_empty = smem_u32(ctl.acc_empty);
+    const int c_off = kLaneBytes, ls_off = c_off + p.bn * kStageRow, cs_off = ls_off + kTiles * kTileBytes;
+    const int k_stages = (p.k + kStageK - 1) / kStageK, k_steps = (p.k + 63) / 64;
+    const int rank = p.split > 1 ? blockIdx.x % p.split : 0;
+    const int k_lo = (int)((int64_t)k_stages * rank / p.split), k_hi = (int)((int64_t)k_stages * (rank + 1) / p.split);
+    const int64_t tiles = (int64_t)p.l_tiles * p.c_tiles;
+    const int64_t tile0 = blockIdx.x / p.split, tile_step = gridDim.x / p.split;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < p.stages; ++i) {
+            umma::mbar_init(full + 8 * i, 1);
+            umma::mbar_init(empty + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            umma::mbar_init(acc_full + 8 * i, 1);
+            umma::mbar_init(acc_empty + 8 * i, 4);
+        }
+        umma::mbar_fence_init();
+    }
+    if (warp == 2) umma::alloc(smem_u32(&ctl.tmem), kTmemCols);
+    umma::fence_before();
+    __syncthreads();
+    umma::fence_after();
+    const uint32_t tmem = ctl.tmem;
+
+    if (warp == 0 && lane == 0) {
+        int s = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int64_t t = tile0; ok && t < tiles; t += tile_step) {
+            const int lt = (int)(t % p.l_tiles), ct = (int)(t / p.l_tiles);
+            const int c0 = ct * p.bn;
+            for (int ks = k_lo; ks < k_hi; ++ks) {
+                if (!(ok = wait(empty + 8 * s, phase ^ 1))) break;
+                const uint32_t at = base + s * p.stage_bytes, bar = full + 8 * s;
+                const int st = min(kTiles, p.scale_tiles - ks * kTiles);
+                expect_tx(bar, kLaneBytes + p.bn * kStageRow + 2 * st * kTileBytes);
+                tma_2d(at, &l_map, ks * kStageRow, lt * 128, bar);
+                tma_2d(at + c_off, &c_map, ks * kStageRow, c0, bar);
+                bulk_copy(at + ls_off, p.l_scales + ((int64_t)lt * p.scale_tiles + ks * kTiles) * kTileBytes, st * kTileBytes, bar);
+                bulk_copy(at + cs_off, p.c_scales + ((int64_t)(c0 >> 7) * p.scale_tiles + ks * kTiles) * kTileBytes, st * kTileBytes, bar);
+                if (++s == p.stages) s = 0, phase ^= 1;
+            }
+        }
+        if (!ok)  // the products have stopped: wait for the copies that nobody will wait for
+            for (int i = 0; i < p.stages; ++i) umma::mbar_wait(full + 8 * i, i < s ? phase : phase ^ 1, 1u << 16);
+    } else if (warp == 1 && lane == 0) {
+        int s = 0, buf = 0, sbuf = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        bool ok = true;
+        for (int64_t t = tile0; ok && t < tiles; t += tile_step) {
+            if (!(ok = wait(acc_empty + 8 * buf, acc_phase ^ 1))) break;
+            umma::fence_after();
+            const uint32_t acc = tmem + buf * kMaxBn;
+            uint32_t more = 0;
+            for (int ks = k_lo; ks < k_hi; ++ks) {
+                if (!(ok = wait(full + 8 * s, phase))) break;
+                umma::fence_after();
+                const uint32_t at = base + s * p.stage_bytes, sl = tmem + kScaleCol + sbuf * kScaleCols, sc = sl + 16;
+                const int steps = min(4, k_steps - ks * 4), st = BLOCK == 16 ? steps : (steps + 1) >> 1;
+                for (int i = 0; i < st; ++i) {
+                    copy_scale_tile(sl + 4 * i, at + ls_off + i * kTileBytes);
+                    copy_scale_tile(sc + 4 * i, at + cs_off + i * kTileBytes);
+                }
+                const uint64_t da = codes_desc(at), db = codes_desc(at + c_off);
+                for (int i = 0; i < steps; ++i) {
+                    const int tile = BLOCK == 16 ? i : i >> 1;
+                    mma<BLOCK>(acc, da + 2 * i, db + 2 * i, idesc<BLOCK>(p.bn, BLOCK == 16 ? 0 : (i & 1) * 2), sl + 4 * tile,
+                               sc + 4 * tile, more);
+                    more = 1;
+                }
+                umma::commit(empty + 8 * s);
+                if (++s == p.stages) s = 0, phase ^= 1;
+                sbuf ^= 1;
+            }
+            if (ok) umma::commit(acc_full + 8 * buf);
+            buf ^= 1;
+            if (buf == 0) acc_phase ^= 1;
+        }
+    } else if (warp >= 4) {
+        int buf = 0;
+        uint32_t acc_phase = 0;
+        for (int64_t t = tile0; t < tiles; t += tile_step) {
+            if (!__all_sync(0xffffffffu, wait(acc_full + 8 * buf, acc_phase))) break;
+            umma::fence_after();
+            const uint32_t acc = tmem + buf * kMaxBn + ((uint32_t)(warp & 3) << 21);
+            const int lane0 = (int)(t % p.l_tiles) * 128, col0 = (int)(t / p.l_tiles) * p.bn;
+            if (p.split > 1) {  // partial sums [column][lane], a lane a bank
+                float *dump = reinterpret_cast<float *>(stages) + (threadIdx.x & 127);
+                for (int c0 = 0; c0 < p.bn; c0 += 32) {
+                    uint32_t v[32];
+                    ld32(acc + c0, v);
+                    umma::wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (c0 + i < p.bn) dump[(c0 + i) * 129] = __uint_as_float(v[i]);
+                }
+            } else if (p.swapped) {
+                epilogue_swapped(p, acc, lane0, col0);
+            } else {
+                epilogue_rows(p, acc, lane0, col0, sh.staging);
+            }
+            umma::fence_before();
+            __syncwarp();
+            if (lane == 0) umma::mbar_arrive(acc_empty + 8 * buf);
+            buf ^= 1;
+            if (buf == 0) acc_phase ^= 1;
+        }
+    }
+    __syncwarp();  // the single lanes of warps 0 and 1 rejoin the others
+    if (p.split > 1) {
+        __syncthreads();
+        cluster_sync();
+        const int lane0 = (int)(tile0 % p.l_tiles) * 128, col0 = (int)(tile0 / p.l_tiles) * p.bn;
+        const int lo = p.bn * rank / p.split, cols = p.bn * (rank + 1) / p.split - lo;
+        for (int i = threadIdx.x; i < cols * 128; i += kThreads) {
+            // consecutive threads along d's rows
+            const int l = p.swapped ? i & 127 : i / cols, c = lo + (p.swapped ? i >> 7 : i % cols);
+            float sum = 0.f;
+            for (int r = 0; r < p.split; ++r) sum += peer_f32(base + (c * 129 + l) * 4, r);
+            const int64_t row = p.swapped ? col0 + c : lane0 + l, col = p.swapped ? lane0 + l : col0 + c;
+            if (lane0 + l < p.l_rows && col0 + c < p.c_rows)
+                store_one(p, row * p.row_stride + col,
+                          activate(fmaf(p.alpha, sum, p.bias ? __ldg(p.bias + col) : 0.f), p.activation));
+        }
+        cluster_sync();  // a block's sums stay until its peers have read them
+    }
+    umma::fence_before();
+    __syncthreads();
+    umma::fence_after();
+    if (warp == 2) umma::dealloc(tmem, kTmemCols);
+}
+
+// ---- host ------------------------------------------------------------------------------------
+
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                 const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled()
+{
+    static const EncodeTiled fn = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<EncodeTiled>(f);
+    }();
+    return fn;
+}
+
+// Codes as a byte matrix, read in boxes of `box_rows` rows x 128 bytes.
+bool encode_codes(CUtensorMap *map, const NtMx4Matrix *m, int box_rows)
+{
+    const EncodeTiled encode = encode_tiled();
+    if (!encode) return false;
+    const cuuint64_t size[2] = {(cuuint64_t)row_pitch(m->cols), (cuuint64_t)m->rows}, stride[1] = {(cuuint64_t)m->pitch};
+    const cuuint32_t box[2] = {kStageRow, (cuuint32_t)box_rows}, step[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, m->data, size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Columns of a tile when the lanes are a's rows.  Tiles of several start at a multiple of 128 columns, where
+// their scale tile starts; a narrower one is the only one.
+int choose_bn(int64_t n) { return n <= 32 ? 32 : n <= 64 ? 64 : 128; }
+
+template <int BLOCK>
+nt_status launch_product(const NtMx4Matrix *a, const NtMx4Matrix *b, ProductLaunch p, cudaStream_t st)
+{
+    constexpr int kTiles = BLOCK == 16 ? 4 : 2;
+    const int sms = sm_count();
+    p.swapped = a->rows <= 64;
+    const NtMx4Matrix *l = p.swapped ? b : a, *c = p.swapped ? a : b;
+    p.bn = !p.swapped ? choose_bn(b->rows)
+           : a->rows <= 8 ? 8 : a->rows <= 16 ? 16 : a->rows <= 32 ? 32 : 64;
+    p.l_rows = l->rows;
+    p.c_rows = c->rows;
+    p.k = a->cols;
+    p.l_tiles = (int32_t)ceil_div(l->rows, 128);
+    p.c_tiles = (int32_t)ceil_div(c->rows, p.bn);
+    p.scale_tiles = tiles_per_row(p.k, BLOCK);
+    p.l_scales = static_cast<const uint8_t *>(l->scales);
+    p.c_scales = static_cast<const uint8_t *>(c->scales);
+    const int64_t tiles = (int64_t)p.l_tiles * p.c_tiles, k_stages = ceil_div(p.k, kStageK);
+    // split K while blocks stand idle and every share keeps two stages
+    p.split = 1;
+    while (p.split < 8 && p.bn <= 128 && tiles * p.split * 2 <= sms && k_stages >= p.split * 4) p.split *= 2;
+    p.stage_bytes = (int32_t)ceil_div(kLaneBytes + p.bn * kStageRow + 2 * kTiles * kTileBytes, 1024) * 1024;
+    const int room = 227 * 1024 - 1024 - (int)sizeof(Shared);
+    p.stages = std::min(kMaxStages, room / p.stage_bytes);
+    const size_t smem = 1024 + std::max((size_t)p.stages * p.stage_bytes, p.split > 1 ? (size_t)p.bn * 129 * 4 : 0);
+    const int64_t grid = p.split > 1 ? tiles * p.split : std::min<int64_t>(tiles, sms);
+    CUtensorMap l_map, c_map;
+    if (!encode_codes(&l_map, l, 128) || !encode_codes(&c_map, c, p.bn))
+        return set_error(NT_ERR_CUDA, "4-bit product: the tensor maps could not be encoded");
+    const void *kernel = reinterpret_cast<const void *>(&product_kernel<BLOCK>);
+    cudaError_t e = set_smem_limit(kernel, 227 * 1024 - sizeof(Shared));
+    if (e == cudaSuccess) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)grid);
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)p.split;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        e = cudaLaunchKernelEx(&cfg, product_kernel<BLOCK>, l_map, c_map, p);
+    }
+    if (e != cudaSuccess) return set_error(NT_ERR_CUDA, "4-bit product: %s", cudaGetErrorString(e));
     count_launch();
-    return cudaGetLastError();
+    return NT_OK;
 }
 
 nt_status check_matrix(const NtMx4Matrix *m, const char *name);
 
 }  // namespace mx4
+
+cudaError_t read_product_status(uint32_t *status, bool clear)
+{
+    cudaError_t e = cudaMemcpyFromSymbol(status, mx4::g_product_status, sizeof(uint32_t));
+    if (e != cudaSuccess || !clear) return e;
+    const uint32_t zero = 0;
+    return cudaMemcpyToSymbol(mx4::g_product_status, &zero, sizeof(uint32_t));
+}
+
 }  // namespace nt
 
 using namespace nt;
@@ -104,30 +516,13 @@ extern "C" nt_status nt_mx4_product(const NtMx4Matrix *a, const NtMx4Matrix *b, 
     NT_LAYER_REQUIRE(d && is_aligned(d, size), "d must be a non-null device pointer aligned to its element");
     NT_LAYER_REQUIRE(is_aligned(bias, 4), "bias must be a 4-byte aligned device pointer");
     mx4::ProductLaunch p = {};
-    p.a = static_cast<const uint8_t *>(a->data);
-    p.b = static_cast<const uint8_t *>(b->data);
-    p.a_scales = static_cast<const uint8_t *>(a->scales);
-    p.b_scales = static_cast<const uint8_t *>(b->scales);
-    p.a_pitch = a->pitch;
-    p.b_pitch = b->pitch;
-    p.m = a->rows;
-    p.n = b->rows;
-    p.k = a->cols;
-    p.tiles = mx4::tiles_per_row(a->cols, a->block);
     p.bias = bias;
     p.activation = activation;
     p.alpha = alpha;
     p.d = d;
+    p.dtype = dtype;
     p.row_stride = row_stride;
-    const cudaStream_t s = (cudaStream_t)stream;
-    cudaError_t e;
-    if (a->block == 16)
-        e = dtype == NT_DTYPE_F16    ? mx4::launch_product<__half, 16>(p, s)
-            : dtype == NT_DTYPE_BF16 ? mx4::launch_product<__nv_bfloat16, 16>(p, s)
-                                     : mx4::launch_product<float, 16>(p, s);
-    else
-        e = dtype == NT_DTYPE_F16    ? mx4::launch_product<__half, 32>(p, s)
-            : dtype == NT_DTYPE_BF16 ? mx4::launch_product<__nv_bfloat16, 32>(p, s)
-                                     : mx4::launch_product<float, 32>(p, s);
-    return e == cudaSuccess ? NT_OK : set_error(NT_ERR_CUDA, "4-bit product: %s", cudaGetErrorString(e));
+    p.vec = is_aligned(d, 16) && row_stride * size % 16 == 0;
+    return a->block == 16 ? mx4::launch_product<16>(a, b, p, (cudaStream_t)stream)
+                          : mx4::launch_product<32>(a, b, p, (cudaStream_t)stream);
 }
