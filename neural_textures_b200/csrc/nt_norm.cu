@@ -1,244 +1,139 @@
-// nt_norm.cu -- channels-last group normalisation with an activation, forward and backward
-// (nt_group_norm_forward, nt_group_norm_backward).
-//
-// Sums over an image are split over kSplit thread blocks and joined in a fixed order:
-//   forward   per (split, channel) count, mean and centred sum of squares, joined per group
-//   backward  per (split, channel) sums of e and e h (e = dy act'(z)), joined per group for dx
-//             and over images for dgamma and dbeta
+// nt_norm.cu -- channels-last group normalisation with an activation: argument checks and launch
+// plan of nt_group_norm_forward and nt_group_norm_backward (the kernel is in nt_norm.cuh).
 #include <algorithm>
 
-#include "nt_layer_common.cuh"
+#include "nt_norm.cuh"
 
 namespace nt {
 namespace norm {
 
-constexpr int kThreads = 256;
-constexpr int kSplit = 64;
+__device__ unsigned int g_norm_status;  // bit 0: the wait at the grid's barrier gave up
 
-struct NormLaunch {
-    NtGroupNorm p;
-    int32_t per;  // channels of a group
-    float *partials;  // [image][split][channel][2]
-    float *sums;      // [image][group][2]
+__global__ void __launch_bounds__(kThreads) join_channels_kernel(const NormLaunch L)
+{
+    const int c = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    if (c < L.p.channels) join_channel(L, c);
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Thread blocks of an image, and how they meet.  A function of the sizes alone, so that the caller's
+// workspace does not depend on addresses.
+struct Plan {
+    int splits;
+    bool cluster;
+    int per_sm;  // blocks that an SM holds: two, or one of the kernels whose vectors cross groups
 };
 
-__device__ __forceinline__ int64_t offset(const NtFeatureMap &f, int64_t n, int64_t texel, int width)
+Plan plan(const NtGroupNorm *p)
 {
-    return n * f.image_stride + texel / width * f.row_stride + texel % width * f.texel_stride;
+    const int64_t values = (int64_t)p->height * p->width * p->channels;
+    const int per_sm = p->channels / p->groups % (16 / layer_dtype_size(p->dtype)) == 0 ? 2 : 1;
+    const int64_t resident = (int64_t)per_sm * sm_count();
+    // at least 4 vectors of 8 channels for each thread of a block
+    const int64_t wanted = std::max<int64_t>(1, values / (kThreads * 32));
+    const int64_t most = std::max<int64_t>(1, resident / p->images);
+    const int64_t splits = std::min({wanted, most, (int64_t)p->height * p->width});
+    if (splits <= 2 * kMaxCluster) return {(int)std::min<int64_t>(splits, kMaxCluster), true, per_sm};
+    return {(int)splits, false, per_sm};
 }
 
-struct Stats {
-    float count, mean, m2;
+size_t align16(size_t n) { return (n + 15) / 16 * 16; }
+
+// Workspace: the barrier, group partials, channel partials.
+struct Layout {
+    size_t groups_at, channels_at, total;
 };
 
-__device__ __forceinline__ Stats join(const Stats &a, const Stats &b)
+Layout layout(const NtGroupNorm *p, const Plan &pl, bool backward)
 {
-    if (b.count == 0.f) return a;
-    if (a.count == 0.f) return b;
-    const float n = a.count + b.count, d = b.mean - a.mean, w = b.count / n;
-    return {n, a.mean + d * w, a.m2 + b.m2 + d * d * a.count * w};
+    Layout l;
+    l.groups_at = pl.cluster ? 0 : 16;
+    l.channels_at = l.groups_at + (pl.cluster ? 0 : align16((size_t)p->images * p->groups * pl.splits * sizeof(float2)));
+    l.total = l.channels_at + (backward ? (size_t)p->images * pl.splits * p->channels * sizeof(float2) : 0);
+    return l;
 }
 
-// grid (split, image): a thread takes a channel and every (256 / channels)-th texel of the split
-template <class T>
-__global__ void __launch_bounds__(kThreads) forward_stats_kernel(const NormLaunch L)
+bool flat(const NtFeatureMap &f, const NtGroupNorm *p) { return p->height == 1 || p->width == 1 || f.row_stride == p->width * f.texel_stride; }
+
+// Widest vector that every map's addresses allow.
+int vector_width(const NtGroupNorm *p, int size, bool backward)
 {
-    const NtGroupNorm &p = L.p;
-    __shared__ Stats part[kThreads];
-    const int64_t texels = (int64_t)p.height * p.width, n = blockIdx.y;
-    const int64_t lo = texels * blockIdx.x / kSplit, hi = texels * (blockIdx.x + 1) / kSplit;
-    const int rows = p.channels < kThreads ? kThreads / p.channels : 1;
-    for (int c0 = 0; c0 < p.channels; c0 += kThreads) {
-        const int width = min(kThreads, p.channels - c0), c = c0 + threadIdx.x % width, row = threadIdx.x / width;
-        Stats s = {0.f, 0.f, 0.f};
-        if (row < rows)
-            for (int64_t t = lo + row; t < hi; t += rows) {
-                const float v = to_f32(static_cast<const T *>(p.x.data)[offset(p.x, n, t, p.width) + c]);
-                s.count += 1.f;
-                const float d = v - s.mean;
-                s.mean += d / s.count;
-                s.m2 += d * (v - s.mean);
-            }
-        part[threadIdx.x] = s;
-        __syncthreads();
-        if (row == 0) {
-            for (int r = 1; r < rows; ++r) s = join(s, part[r * width + threadIdx.x]);
-            float *out = L.partials + ((n * kSplit + blockIdx.x) * p.channels + c) * 2;
-            out[0] = s.mean;
-            out[1] = s.m2;
-        }
-        __syncthreads();
+    for (int v = 16 / size; v > 1; v /= 2) {
+        bool ok = p->channels % v == 0;
+        for (const NtFeatureMap *f : {&p->x, backward ? &p->dy : &p->y, backward ? &p->dx : &p->y})
+            ok = ok && is_aligned(f->data, v * size) && f->image_stride % v == 0 && f->row_stride % v == 0 && f->texel_stride % v == 0;
+        if (ok) return v;
     }
+    return 1;
 }
 
-// grid (group, image)
-__global__ void forward_join_kernel(const NormLaunch L)
+cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
 {
-    const NtGroupNorm &p = L.p;
-    __shared__ Stats part[kThreads];
-    const int64_t texels = (int64_t)p.height * p.width, n = blockIdx.y;
-    Stats s = {0.f, 0.f, 0.f};
-    for (int i = threadIdx.x; i < kSplit * L.per; i += kThreads) {
-        const int split = i / L.per, c = blockIdx.x * L.per + i % L.per;
-        const float *in = L.partials + ((n * kSplit + split) * p.channels + c) * 2;
-        const float count = (float)(texels * (split + 1) / kSplit - texels * split / kSplit);
-        s = join(s, {count, in[0], in[1]});
+    const int size = layer_dtype_size(p->dtype);
+    const Plan pl = plan(p);
+    const Layout at = layout(p, pl, backward);
+    char *ws = static_cast<char *>(p->workspace);
+    NormLaunch L = {};
+    L.p = *p;
+    if (p->width == 1) {  // one texel a row: rows are the texels
+        L.p.x.texel_stride = p->x.row_stride;
+        L.p.y.texel_stride = p->y.row_stride;
+        L.p.dy.texel_stride = p->dy.row_stride;
+        L.p.dx.texel_stride = p->dx.row_stride;
     }
-    part[threadIdx.x] = s;
-    for (int w = kThreads / 2; w > 0; w >>= 1) {
-        __syncthreads();
-        if ((int)threadIdx.x < w) part[threadIdx.x] = join(part[threadIdx.x], part[threadIdx.x + w]);
-    }
-    if (threadIdx.x == 0) {
-        const float rstd = 1.f / sqrtf(part[0].m2 / part[0].count + p.epsilon);
-        const int64_t at = n * p.groups + blockIdx.x;
-        L.sums[2 * at] = part[0].mean;
-        L.sums[2 * at + 1] = rstd;
-        if (p.mean) p.mean[at] = part[0].mean;
-        if (p.rstd) p.rstd[at] = rstd;
-    }
-}
+    const int v = vector_width(p, size, backward);
+    L.per = p->channels / p->groups;
+    L.splits = pl.splits;
+    L.cluster = pl.cluster;
+    L.flat = flat(p->x, p) && flat(backward ? p->dy : p->y, p) && flat(backward ? p->dx : p->y, p);
+    L.texels = p->height * p->width;
+    L.vectors = p->channels / v;
+    L.tx = std::min(L.vectors, kThreads);
+    L.ty = kThreads / L.tx;
+    L.inv_count = 1.f / ((float)L.texels * (float)L.per);
+    L.barrier = reinterpret_cast<unsigned int *>(ws);
+    L.groups_part = reinterpret_cast<float2 *>(ws + at.groups_at);
+    L.channels_part = reinterpret_cast<float2 *>(ws + at.channels_at);
+    const bool whole = L.per % v == 0;
+    const size_t entries = (size_t)L.ty * (backward || !whole ? p->channels : L.vectors);
+    L.scratch = (int32_t)align16((2 * (size_t)p->groups + entries) * sizeof(float2));
+    const size_t slot = (size_t)kThreads * v * size * (backward ? 2 : 1);
+    const size_t most = 227 * 1024 / pl.per_sm - 1024;
+    const size_t room = (size_t)L.scratch < most ? most - L.scratch : 0;
+    const int64_t slots = ceil_div(ceil_div(L.texels, L.splits), L.ty) * ceil_div(L.vectors, L.tx);
+    L.keep = (int32_t)std::min<int64_t>(slots, room / slot);
+    const size_t smem = L.scratch + L.keep * slot;
 
-template <class T>
-__global__ void __launch_bounds__(kThreads) forward_apply_kernel(const NormLaunch L)
-{
-    const NtGroupNorm &p = L.p;
-    const int64_t texels = (int64_t)p.height * p.width, count = texels * p.channels, n = blockIdx.y;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < count; i += (int64_t)gridDim.x * kThreads) {
-        const int64_t t = i / p.channels;
-        const int c = (int)(i % p.channels);
-        const float *stat = L.sums + 2 * (n * p.groups + c / L.per);
-        const float h = (to_f32(static_cast<const T *>(p.x.data)[offset(p.x, n, t, p.width) + c]) - stat[0]) * stat[1];
-        const float z = (p.gamma ? p.gamma[c] : 1.f) * h + (p.beta ? p.beta[c] : 0.f);
-        static_cast<T *>(p.y.data)[offset(p.y, n, t, p.width) + c] = from_f32<T>(activate(z, p.activation));
-    }
-}
-
-template <class T>
-__device__ __forceinline__ void backward_terms(const NormLaunch &L, int64_t n, int64_t t, int c, float &e, float &h)
-{
-    const NtGroupNorm &p = L.p;
-    const int64_t at = n * p.groups + c / L.per;
-    h = (to_f32(static_cast<const T *>(p.x.data)[offset(p.x, n, t, p.width) + c]) - p.mean[at]) * p.rstd[at];
-    const float z = (p.gamma ? p.gamma[c] : 1.f) * h + (p.beta ? p.beta[c] : 0.f);
-    e = to_f32(static_cast<const T *>(p.dy.data)[offset(p.dy, n, t, p.width) + c]) * activation_slope(z, p.activation);
-}
-
-template <class T>
-__global__ void __launch_bounds__(kThreads) backward_sums_kernel(const NormLaunch L)
-{
-    const NtGroupNorm &p = L.p;
-    __shared__ float2 part[kThreads];
-    const int64_t texels = (int64_t)p.height * p.width, n = blockIdx.y;
-    const int64_t lo = texels * blockIdx.x / kSplit, hi = texels * (blockIdx.x + 1) / kSplit;
-    const int rows = p.channels < kThreads ? kThreads / p.channels : 1;
-    for (int c0 = 0; c0 < p.channels; c0 += kThreads) {
-        const int width = min(kThreads, p.channels - c0), c = c0 + threadIdx.x % width, row = threadIdx.x / width;
-        float2 s = make_float2(0.f, 0.f);
-        if (row < rows)
-            for (int64_t t = lo + row; t < hi; t += rows) {
-                float e, h;
-                backward_terms<T>(L, n, t, c, e, h);
-                s.x += e;
-                s.y += e * h;
-            }
-        part[threadIdx.x] = s;
-        __syncthreads();
-        if (row == 0) {
-            for (int r = 1; r < rows; ++r) s.x += part[r * width + threadIdx.x].x, s.y += part[r * width + threadIdx.x].y;
-            reinterpret_cast<float2 *>(L.partials)[(n * kSplit + blockIdx.x) * p.channels + c] = s;
-        }
-        __syncthreads();
-    }
-}
-
-// grid (group, image): s1, s2 of a group
-__global__ void backward_join_kernel(const NormLaunch L)
-{
-    const NtGroupNorm &p = L.p;
-    __shared__ float2 part[kThreads];
-    const int64_t n = blockIdx.y;
-    float2 s = make_float2(0.f, 0.f);
-    for (int i = threadIdx.x; i < kSplit * L.per; i += kThreads) {
-        const int c = blockIdx.x * L.per + i % L.per;
-        const float g = p.gamma ? p.gamma[c] : 1.f;
-        const float2 v = reinterpret_cast<const float2 *>(L.partials)[(n * kSplit + i / L.per) * p.channels + c];
-        s.x += g * v.x;
-        s.y += g * v.y;
-    }
-    part[threadIdx.x] = s;
-    for (int w = kThreads / 2; w > 0; w >>= 1) {
-        __syncthreads();
-        if ((int)threadIdx.x < w)
-            part[threadIdx.x].x += part[threadIdx.x + w].x, part[threadIdx.x].y += part[threadIdx.x + w].y;
-    }
-    if (threadIdx.x == 0) reinterpret_cast<float2 *>(L.sums)[n * p.groups + blockIdx.x] = part[0];
-}
-
-// grid (channel): dgamma, dbeta
-__global__ void backward_params_kernel(const NormLaunch L)
-{
-    const NtGroupNorm &p = L.p;
-    __shared__ float2 part[kThreads];
-    float2 s = make_float2(0.f, 0.f);
-    for (int64_t i = threadIdx.x; i < (int64_t)p.images * kSplit; i += kThreads) {
-        const float2 v = reinterpret_cast<const float2 *>(L.partials)[i * p.channels + blockIdx.x];
-        s.x += v.x;
-        s.y += v.y;
-    }
-    part[threadIdx.x] = s;
-    for (int w = kThreads / 2; w > 0; w >>= 1) {
-        __syncthreads();
-        if ((int)threadIdx.x < w)
-            part[threadIdx.x].x += part[threadIdx.x + w].x, part[threadIdx.x].y += part[threadIdx.x + w].y;
-    }
-    if (threadIdx.x == 0) {
-        if (p.dbeta) p.dbeta[blockIdx.x] = part[0].x;
-        if (p.dgamma) p.dgamma[blockIdx.x] = part[0].y;
-    }
-}
-
-template <class T>
-__global__ void __launch_bounds__(kThreads) backward_apply_kernel(const NormLaunch L)
-{
-    const NtGroupNorm &p = L.p;
-    const int64_t texels = (int64_t)p.height * p.width, count = texels * p.channels, n = blockIdx.y;
-    const float inv = 1.f / ((float)texels * (float)L.per);
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < count; i += (int64_t)gridDim.x * kThreads) {
-        const int64_t t = i / p.channels;
-        const int c = (int)(i % p.channels);
-        float e, h;
-        backward_terms<T>(L, n, t, c, e, h);
-        const int64_t at = n * p.groups + c / L.per;
-        const float2 s = reinterpret_cast<const float2 *>(L.sums)[at];
-        const float dx = p.rstd[at] * ((p.gamma ? p.gamma[c] : 1.f) * e - (s.x + h * s.y) * inv);
-        static_cast<T *>(p.dx.data)[offset(p.dx, n, t, p.width) + c] = from_f32<T>(dx);
-    }
-}
-
-size_t partial_floats(const NtGroupNorm *p) { return (size_t)p->images * kSplit * p->channels * 2; }
-
-template <class T>
-cudaError_t launch(const NormLaunch &L, bool backward, cudaStream_t st)
-{
-    const NtGroupNorm &p = L.p;
-    const dim3 split(kSplit, p.images), group(p.groups, p.images);
-    const int64_t count = (int64_t)p.height * p.width * p.channels;
-    const dim3 apply((unsigned)std::min<int64_t>((count + kThreads - 1) / kThreads, 8 * sm_count()), p.images);
-    if (!backward) {
-        forward_stats_kernel<T><<<split, kThreads, 0, st>>>(L);
-        forward_join_kernel<<<group, kThreads, 0, st>>>(L);
-        forward_apply_kernel<T><<<apply, kThreads, 0, st>>>(L);
+    const NormKernel kernel = backward ? backward_kernel(p->dtype, v, whole) : forward_kernel(p->dtype, v, whole);
+    unsigned int *status = nullptr;
+    cudaError_t e = cudaGetSymbolAddress(reinterpret_cast<void **>(&status), g_norm_status);
+    if (e == cudaSuccess) e = set_smem_limit(reinterpret_cast<const void *>(kernel), 227 * 1024 - 1024);
+    if (e != cudaSuccess) return e;
+    if (!pl.cluster && (e = cudaMemsetAsync(ws, 0, 16, st)) != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((int64_t)p->images * pl.splits));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    if (pl.cluster) {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)pl.splits;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     } else {
-        backward_sums_kernel<T><<<split, kThreads, 0, st>>>(L);
-        backward_join_kernel<<<group, kThreads, 0, st>>>(L);
-        backward_apply_kernel<T><<<apply, kThreads, 0, st>>>(L);
-        if (p.dgamma || p.dbeta) {
-            backward_params_kernel<<<p.channels, kThreads, 0, st>>>(L);
-            count_launch();
-        }
+        attr[0].id = cudaLaunchAttributeCooperative;
+        attr[0].val.cooperative = 1;
     }
-    for (int i = 0; i < 3; ++i) count_launch();
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, L, status);
+    if (e != cudaSuccess) return e;
+    count_launch();
+    if (backward && pl.cluster && (p->dgamma || p->dbeta)) {
+        join_channels_kernel<<<(unsigned)ceil_div(p->channels, kWarps), kThreads, 0, st>>>(L);
+        count_launch();
+    }
     return cudaGetLastError();
 }
 
@@ -275,9 +170,9 @@ nt_status check_shape(const NtGroupNorm *p)
     return NT_OK;
 }
 
-size_t workspace_bytes(const NtGroupNorm *p, bool)
+size_t workspace_bytes(const NtGroupNorm *p, bool backward)
 {
-    return p->images ? (partial_floats(p) + (size_t)p->images * p->groups * 2) * sizeof(float) : 0;
+    return p->images ? layout(p, plan(p), backward).total : 0;
 }
 
 nt_status run(const NtGroupNorm *p, bool backward, nt_stream_t stream)
@@ -307,20 +202,22 @@ nt_status run(const NtGroupNorm *p, bool backward, nt_stream_t stream)
         return st;
     }
     const size_t need = workspace_bytes(p, backward);
-    NT_LAYER_REQUIRE(need == 0 || (p->workspace && is_aligned(p->workspace, 16) && p->workspace_bytes >= (int64_t)need),
+    NT_LAYER_REQUIRE(is_aligned(p->workspace, 16) && (need == 0 || (p->workspace && p->workspace_bytes >= (int64_t)need)),
                      "workspace must be 16-byte aligned and hold %zu bytes (got %lld)", need, (long long)p->workspace_bytes);
-    NormLaunch L;
-    L.p = *p;
-    L.per = p->channels / p->groups;
-    L.partials = static_cast<float *>(p->workspace);
-    L.sums = L.partials + partial_floats(p);
-    const cudaError_t e = p->dtype == NT_DTYPE_F16    ? launch<__half>(L, backward, s)
-                          : p->dtype == NT_DTYPE_BF16 ? launch<__nv_bfloat16>(L, backward, s)
-                                                      : launch<float>(L, backward, s);
+    const cudaError_t e = launch(p, backward, s);
     return e == cudaSuccess ? NT_OK : set_error(NT_ERR_CUDA, "group norm: %s", cudaGetErrorString(e));
 }
 
 }  // namespace norm
+
+cudaError_t read_norm_status(uint32_t *status, bool clear)
+{
+    cudaError_t e = cudaMemcpyFromSymbol(status, norm::g_norm_status, sizeof(uint32_t));
+    if (e != cudaSuccess || !clear) return e;
+    const uint32_t zero = 0;
+    return cudaMemcpyToSymbol(norm::g_norm_status, &zero, sizeof(uint32_t));
+}
+
 }  // namespace nt
 
 using namespace nt;
