@@ -40,33 +40,92 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// 1 / (1 + exp(-z)); exp(-z) = inf gives 0.
-__device__ __forceinline__ float sigmoid_f32(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp(float x)
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
+
+// 1 / a of both lanes with one reciprocal: 1 / (a.x a.y), times the other lane.  The special-function unit
+// is the narrowest one that an activation uses.  |a| stays within 2^+-63.
+__device__ __forceinline__ float2 rcp2(float2 a)
+{
+    const float r = rcp(a.x * a.y);
+    return make_float2(a.y * r, a.x * r);
+}
+
+// 1 / (1 + exp(-z)).  Below -43 the true value is under 3e-19, where it is held.
+__device__ __forceinline__ float2 sigmoid2(float2 z)
+{
+    const float2 m = make_float2(fmaxf(z.x, -43.f), fmaxf(z.y, -43.f));
+    const float2 t = __fmul2_rn(m, f2(-1.44269504f));
+    return rcp2(__fadd2_rn(make_float2(ex2(t.x), ex2(t.y)), f2(1.f)));
+}
+
+// The normal distribution's integral Phi(z), and exp(-z^2 / 2).  With x = |z| / sqrt 2, t = 1 / (1 + p x):
+// erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2) within 1.5e-7 (Abramowitz and Stegun, 7.1.26).
+__device__ __forceinline__ float2 normal_cdf2(float2 z, float2 &bell)
+{
+    const float2 x = make_float2(fminf(fabsf(z.x), 64.f), fminf(fabsf(z.y), 64.f));
+    const float2 t = rcp2(__ffma2_rn(x, f2(0.3275911f * 0.70710678f), f2(1.f)));
+    const float2 q = __fmul2_rn(__fmul2_rn(x, x), f2(-0.5f * 1.44269504f));
+    bell = make_float2(ex2(q.x), ex2(q.y));
+    float2 s = __ffma2_rn(t, f2(0.5f * 1.061405429f), f2(0.5f * -1.453152027f));
+    s = __ffma2_rn(s, t, f2(0.5f * 1.421413741f));
+    s = __ffma2_rn(s, t, f2(0.5f * -0.284496736f));
+    s = __ffma2_rn(s, t, f2(0.5f * 0.254829592f));
+    const float2 tail = __fmul2_rn(__fmul2_rn(s, t), bell);  // Phi(-|z|)
+    return make_float2(z.x < 0.f ? tail.x : 1.f - tail.x, z.y < 0.f ? tail.y : 1.f - tail.y);
+}
 
 // A NaN stays a NaN under every activation.
-__device__ __forceinline__ float activate(float z, int act)
+template <int ACT>
+__device__ __forceinline__ float2 activate2(float2 z)
+{
+    if (ACT == NT_ACT_RELU) return make_float2(z.x < 0.f ? 0.f : z.x, z.y < 0.f ? 0.f : z.y);
+    if (ACT == NT_ACT_SILU) return __fmul2_rn(z, sigmoid2(z));
+    if (ACT == NT_ACT_GELU) {
+        float2 bell;
+        return __fmul2_rn(z, normal_cdf2(z, bell));
+    }
+    return z;
+}
+
+__device__ __forceinline__ float2 activate2(float2 z, int act)
 {
     switch (act) {
-    case NT_ACT_RELU: return z < 0.f ? 0.f : z;
-    case NT_ACT_SILU: return z * sigmoid_f32(z);
-    case NT_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    case NT_ACT_RELU: return activate2<NT_ACT_RELU>(z);
+    case NT_ACT_SILU: return activate2<NT_ACT_SILU>(z);
+    case NT_ACT_GELU: return activate2<NT_ACT_GELU>(z);
     default: return z;
     }
 }
 
-// d activation / dz
-__device__ __forceinline__ float activation_slope(float z, int act)
+__device__ __forceinline__ float activate1(float z, int act) { return activate2(make_float2(z, 0.f), act).x; }
+
+// e d activation / dz
+template <int ACT>
+__device__ __forceinline__ float2 times_slope2(float2 e, float2 z)
 {
-    switch (act) {
-    case NT_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-    case NT_ACT_SILU: {
-        const float s = sigmoid_f32(z);
-        return s * (1.f + z * (1.f - s));
+    if (ACT == NT_ACT_RELU) return make_float2(z.x > 0.f ? e.x : e.x * 0.f, z.y > 0.f ? e.y : e.y * 0.f);
+    if (ACT == NT_ACT_SILU) {  // s (1 + z (1 - s)) = s + y (1 - s), y = z s
+        const float2 s = sigmoid2(z);
+        return __fmul2_rn(e, __ffma2_rn(__fmul2_rn(z, s), __ffma2_rn(s, f2(-1.f), f2(1.f)), s));
     }
-    case NT_ACT_GELU:
-        return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __expf(-0.5f * z * z);
-    default: return 1.f;
+    if (ACT == NT_ACT_GELU) {
+        float2 bell;
+        const float2 cdf = normal_cdf2(z, bell);
+        return __fmul2_rn(e, __ffma2_rn(__fmul2_rn(z, f2(0.39894228f)), bell, cdf));
     }
+    return e;
 }
 
 }  // namespace nt

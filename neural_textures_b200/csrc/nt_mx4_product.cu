@@ -187,7 +187,7 @@ __device__ __forceinline__ void epilogue_swapped(const ProductLaunch &p, uint32_
         for (int i = 0; i < 32; ++i) {
             const int64_t m = col0 + c0 + i;
             if (c0 + i < p.bn && m < p.c_rows && n < p.l_rows)
-                store_one(p, m * p.row_stride + n, activate(fmaf(p.alpha, __uint_as_float(v[i]), bias), p.activation));
+                store_one(p, m * p.row_stride + n, activate1(fmaf(p.alpha, __uint_as_float(v[i]), bias), p.activation));
         }
     }
 }
@@ -208,9 +208,13 @@ __device__ __forceinline__ void epilogue_rows(const ProductLaunch &p, uint32_t t
             const float bias = p.bias && nb < p.c_rows ? __ldg(p.bias + nb) : 0.f;
             umma::wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-                v[i] = __float_as_uint(
-                    activate(fmaf(p.alpha, __uint_as_float(v[i]), __shfl_sync(0xffffffffu, bias, i)), p.activation));
+            for (int i = 0; i < 32; i += 2) {
+                const float2 b = make_float2(__shfl_sync(0xffffffffu, bias, i), __shfl_sync(0xffffffffu, bias, i + 1));
+                const float2 z = __ffma2_rn(f2(p.alpha), make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), b);
+                const float2 y = activate2(z, p.activation);
+                v[i] = __float_as_uint(y.x);
+                v[i + 1] = __float_as_uint(y.y);
+            }
             uint8_t *row = mine + lane * kStagePitch + s * size;
             if (size == 4) {
 #pragma unroll
@@ -386,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int64_t row = p.swapped ? col0 + c : lane0 + l, col = p.swapped ? lane0 + l : col0 + c;
             if (lane0 + l < p.l_rows && col0 + c < p.c_rows)
                 store_one(p, row * p.row_stride + col,
-                          activate(fmaf(p.alpha, sum, p.bias ? __ldg(p.bias + col) : 0.f), p.activation));
+                          activate1(fmaf(p.alpha, sum, p.bias ? __ldg(p.bias + col) : 0.f), p.activation));
         }
         cluster_sync();  // a block's sums stay until its peers have read them
     }

@@ -9,9 +9,11 @@ namespace norm {
 
 __device__ unsigned int g_norm_status;  // bit 0: the wait at the grid's barrier gave up
 
-__global__ void __launch_bounds__(kThreads) join_channels_kernel(const NormLaunch L)
+constexpr int kJoinWarps = 8;
+
+__global__ void __launch_bounds__(32 * kJoinWarps) join_channels_kernel(const NormLaunch L)
 {
-    const int c = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int c = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
     if (c < L.p.channels) join_channel(L, c);
 }
 
@@ -30,8 +32,8 @@ Plan plan(const NtGroupNorm *p)
     const int64_t values = (int64_t)p->height * p->width * p->channels;
     const int per_sm = p->channels / p->groups % (16 / layer_dtype_size(p->dtype)) == 0 ? 2 : 1;
     const int64_t resident = (int64_t)per_sm * sm_count();
-    // at least 4 vectors of 8 channels for each thread of a block
-    const int64_t wanted = std::max<int64_t>(1, values / (kThreads * 32));
+    // at least 4 vectors of 8 channels for each of 512 threads
+    const int64_t wanted = std::max<int64_t>(1, values / (512 * 32));
     const int64_t most = std::max<int64_t>(1, resident / p->images);
     const int64_t splits = std::min({wanted, most, (int64_t)p->height * p->width});
     if (splits <= 2 * kMaxCluster) return {(int)std::min<int64_t>(splits, kMaxCluster), true, per_sm};
@@ -54,8 +56,6 @@ Layout layout(const NtGroupNorm *p, const Plan &pl, bool backward)
     return l;
 }
 
-bool flat(const NtFeatureMap &f, const NtGroupNorm *p) { return p->height == 1 || p->width == 1 || f.row_stride == p->width * f.texel_stride; }
-
 // Widest vector that every map's addresses allow.
 int vector_width(const NtGroupNorm *p, int size, bool backward)
 {
@@ -76,21 +76,20 @@ cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
     char *ws = static_cast<char *>(p->workspace);
     NormLaunch L = {};
     L.p = *p;
-    if (p->width == 1) {  // one texel a row: rows are the texels
-        L.p.x.texel_stride = p->x.row_stride;
-        L.p.y.texel_stride = p->y.row_stride;
-        L.p.dy.texel_stride = p->dy.row_stride;
-        L.p.dx.texel_stride = p->dx.row_stride;
-    }
     const int v = vector_width(p, size, backward);
     L.per = p->channels / p->groups;
     L.splits = pl.splits;
     L.cluster = pl.cluster;
-    L.flat = flat(p->x, p) && flat(backward ? p->dy : p->y, p) && flat(backward ? p->dx : p->y, p);
     L.texels = p->height * p->width;
     L.vectors = p->channels / v;
-    L.tx = std::min(L.vectors, kThreads);
-    L.ty = kThreads / L.tx;
+    const int threads = backward ? kBackwardThreads : kForwardThreads;
+    // threads along a texel's vectors: all of them, or the number of turns that leaves the fewest threads idle
+    double used = 0;
+    for (int turns = (int)ceil_div(L.vectors, threads), last = turns + 3; turns <= last; ++turns) {
+        const int tx = (int)ceil_div(L.vectors, turns), ty = threads / tx;
+        const double share = (double)L.vectors * ty / ((double)turns * threads);
+        if (share > used + 0.05) used = share, L.tx = tx, L.ty = ty;
+    }
     L.inv_count = 1.f / ((float)L.texels * (float)L.per);
     L.barrier = reinterpret_cast<unsigned int *>(ws);
     L.groups_part = reinterpret_cast<float2 *>(ws + at.groups_at);
@@ -98,7 +97,7 @@ cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
     const bool whole = L.per % v == 0;
     const size_t entries = (size_t)L.ty * (backward || !whole ? p->channels : L.vectors);
     L.scratch = (int32_t)align16((2 * (size_t)p->groups + entries) * sizeof(float2));
-    const size_t slot = (size_t)kThreads * v * size * (backward ? 2 : 1);
+    const size_t slot = (size_t)threads * v * size * (backward ? 2 : 1);
     const size_t most = 227 * 1024 / pl.per_sm - 1024;
     const size_t room = (size_t)L.scratch < most ? most - L.scratch : 0;
     const int64_t slots = ceil_div(ceil_div(L.texels, L.splits), L.ty) * ceil_div(L.vectors, L.tx);
@@ -113,7 +112,7 @@ cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
     if (!pl.cluster && (e = cudaMemsetAsync(ws, 0, 16, st)) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((int64_t)p->images * pl.splits));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -131,7 +130,7 @@ cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
     if (e != cudaSuccess) return e;
     count_launch();
     if (backward && pl.cluster && (p->dgamma || p->dbeta)) {
-        join_channels_kernel<<<(unsigned)ceil_div(p->channels, kWarps), kThreads, 0, st>>>(L);
+        join_channels_kernel<<<(unsigned)ceil_div(p->channels, kJoinWarps), 32 * kJoinWarps, 0, st>>>(L);
         count_launch();
     }
     return cudaGetLastError();

@@ -20,8 +20,8 @@
 namespace nt {
 namespace norm {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
+constexpr int kForwardThreads = 512;
+constexpr int kBackwardThreads = 384;  // 84 registers a thread with two blocks on an SM: 64 spill
 constexpr int kMaxCluster = 8;
 constexpr uint32_t kSpinLimit = 1u << 24;
 
@@ -30,7 +30,6 @@ struct NormLaunch {
     int32_t per;        // channels of a group
     int32_t splits;     // thread blocks of an image
     int32_t cluster;    // 1: they form a cluster; 0: the grid meets at *barrier
-    int32_t flat;       // texels of every map are evenly spaced
     int32_t texels, vectors;  // vectors of V channels in a texel
     int32_t tx, ty;     // threads along channels and texels
     int32_t keep;       // vectors of a thread (of x, and of dy) that stay in shared memory
@@ -42,6 +41,21 @@ struct NormLaunch {
 };
 
 // V consecutive channels.
+template <class T>
+struct Pair;
+template <>
+struct Pair<__half> { using type = __half2; };
+template <>
+struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
+__device__ __forceinline__ float2 pair_f32(__half2 v) { return __half22float2(v); }
+__device__ __forceinline__ float2 pair_f32(__nv_bfloat162 v) { return __bfloat1622float2(v); }
+template <class T>
+__device__ __forceinline__ typename Pair<T>::type f32_pair(float2 v);
+template <>
+__device__ __forceinline__ __half2 f32_pair<__half>(float2 v) { return __float22half2_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat162 f32_pair<__nv_bfloat16>(float2 v) { return __float22bfloat162_rn(v); }
+
 template <class T, int V>
 struct alignas(V * sizeof(T) > 16 ? 16 : V * sizeof(T)) Vec {
     T v[V];
@@ -70,46 +84,40 @@ __device__ __forceinline__ void store_vec(T *p, const Vec<T, V> &r)
     else __stcs(reinterpret_cast<uint16_t *>(p), *reinterpret_cast<const uint16_t *>(&r));
 }
 
-template <int V>
-__device__ __forceinline__ void activate_all(float (&z)[V], int act)
+// A vector's values in pairs, for packed fp32 arithmetic (of a single value, beside a zero).
+template <class T, int V>
+__device__ __forceinline__ void unpack(const Vec<T, V> &a, float2 (&f)[(V + 1) / 2])
 {
-    switch (act) {
-    case NT_ACT_RELU:
 #pragma unroll
-        for (int i = 0; i < V; ++i) z[i] = activate(z[i], NT_ACT_RELU);
-        break;
-    case NT_ACT_SILU:
-#pragma unroll
-        for (int i = 0; i < V; ++i) z[i] = activate(z[i], NT_ACT_SILU);
-        break;
-    case NT_ACT_GELU:
-#pragma unroll
-        for (int i = 0; i < V; ++i) z[i] = activate(z[i], NT_ACT_GELU);
-        break;
-    default: break;
+    for (int j = 0; j < (V + 1) / 2; ++j) {
+        if constexpr (V == 1) f[j] = make_float2(to_f32(a.v[0]), 0.f);
+        else if constexpr (sizeof(T) == 4) f[j] = make_float2(a.v[2 * j], a.v[2 * j + 1]);
+        else f[j] = pair_f32(reinterpret_cast<const typename Pair<T>::type *>(&a)[j]);
     }
 }
 
-// e = dy act'(z)
-template <int V>
-__device__ __forceinline__ void times_slope(float (&e)[V], const float (&z)[V], int act)
+template <class T, int V>
+__device__ __forceinline__ Vec<T, V> pack(const float2 (&f)[(V + 1) / 2])
 {
-    switch (act) {
-    case NT_ACT_RELU:
+    Vec<T, V> r;
 #pragma unroll
-        for (int i = 0; i < V; ++i) e[i] *= activation_slope(z[i], NT_ACT_RELU);
-        break;
-    case NT_ACT_SILU:
-#pragma unroll
-        for (int i = 0; i < V; ++i) e[i] *= activation_slope(z[i], NT_ACT_SILU);
-        break;
-    case NT_ACT_GELU:
-#pragma unroll
-        for (int i = 0; i < V; ++i) e[i] *= activation_slope(z[i], NT_ACT_GELU);
-        break;
-    default: break;
+    for (int j = 0; j < (V + 1) / 2; ++j) {
+        if constexpr (V == 1) r.v[0] = from_f32<T>(f[0].x);
+        else if constexpr (sizeof(T) == 4) r.v[2 * j] = f[j].x, r.v[2 * j + 1] = f[j].y;
+        else reinterpret_cast<typename Pair<T>::type *>(&r)[j] = f32_pair<T>(f[j]);
     }
+    return r;
 }
+
+// A thread's way through a map: every ty-th texel of its block's range, forwards or backwards.  Texels
+// advance by whole rows and a remainder; a texel past the end of its row wraps into the next.
+struct Walk {
+    int64_t step, wrap;  // bytes
+    __device__ __forceinline__ Walk(const NtFeatureMap &f, int width, int rows, int rest, int size)
+        : step((rows * f.row_stride + rest * f.texel_stride) * size), wrap((f.row_stride - width * f.texel_stride) * size)
+    {
+    }
+};
 
 // Count, mean and sum of squares about the mean.
 struct Stats {
@@ -191,120 +199,349 @@ __device__ __forceinline__ void join_channel(const NormLaunch &L, int c)
     }
 }
 
+// What a thread's passes share.
+template <class T, int V, bool WHOLE, bool BACKWARD>
+struct Threads {
+    static constexpr int P = (V + 1) / 2;
+    static constexpr int NT = BACKWARD ? kBackwardThreads : kForwardThreads;
+    const NormLaunch &L;
+    int64_t n;
+    int lo, row, col, mine;  // first texel of the block; place of the thread; its texels
+    const float2 *stat;
+    float2 *scratch;
+    Vec<T, V> *kept;
+    int rows, rest;  // ty texels: whole rows of the image, and the rest
+
+    // The x coordinate of texel i of this thread, and where it lies in map f.
+    __device__ __forceinline__ int seek(const NtFeatureMap &f, int i, int c, char *&at) const
+    {
+        const int t = lo + row + i * L.ty, y = t / L.p.width, x = t - y * L.p.width;
+        at = static_cast<char *>(f.data) + (n * f.image_stride + y * f.row_stride + x * f.texel_stride + c) * (int64_t)sizeof(T);
+        return x;
+    }
+    __device__ __forceinline__ bool forth(int &x) const
+    {
+        x += rest;
+        const bool over = x >= L.p.width;
+        if (over) x -= L.p.width;
+        return over;
+    }
+    __device__ __forceinline__ bool back(int &x) const
+    {
+        x -= rest;
+        const bool over = x < 0;
+        if (over) x += L.p.width;
+        return over;
+    }
+    // Per-channel values of a parameter, in pairs.
+    __device__ __forceinline__ void channels(const float *param, float other, int c, float2 (&v)[P]) const
+    {
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+            v[j] = make_float2(param ? __ldg(param + c + 2 * j) : other, V > 1 && param ? __ldg(param + c + 2 * j + 1) : other);
+    }
+    // Group of channel c + i (of the whole vector, when it lies in one).
+    __device__ __forceinline__ int group(int c, int i) const { return (c + (WHOLE || i >= V ? 0 : i)) / L.per; }
+
+    // ---- pass 1 ----
+    // `near` texels are kept from slot `slot0` on.
+    __device__ __forceinline__ void forward_sums(int c, int count, int near, int slot0) const
+    {
+        constexpr int U = 4;
+        float2 pivot[P] = {}, s1[P] = {}, s2[P] = {};
+        char *at;
+        int x = seek(L.p.x, 0, c, at);
+        const Walk w(L.p.x, L.p.width, rows, rest, sizeof(T));
+        if (count > 0) unpack<T, V>(load_vec<T, V>(reinterpret_cast<const T *>(at), false), pivot);
+#pragma unroll
+        for (int j = 0; j < P; ++j) pivot[j] = make_float2(-pivot[j].x, -pivot[j].y);
+        auto load = [&](bool stream) {
+            const Vec<T, V> v = load_vec<T, V>(reinterpret_cast<const T *>(at), stream);
+            at += w.step;
+            if (forth(x)) at += w.wrap;
+            return v;
+        };
+        auto add = [&](const Vec<T, V> &v) {
+            float2 f[P];
+            unpack<T, V>(v, f);
+#pragma unroll
+            for (int j = 0; j < P; ++j) {
+                const float2 d = __fadd2_rn(f[j], pivot[j]);
+                s1[j] = __fadd2_rn(s1[j], d);
+                s2[j] = __ffma2_rn(d, d, s2[j]);
+            }
+        };
+        Vec<T, V> *keep = kept + slot0 * NT + threadIdx.x;
+        int i = 0;
+        for (; i + U <= near; i += U) {
+            Vec<T, V> v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = load(true);
+#pragma unroll
+            for (int u = 0; u < U; ++u, keep += NT) *keep = v[u], add(v[u]);
+        }
+        for (; i < near; ++i, keep += NT) {
+            const Vec<T, V> v = load(true);
+            *keep = v;
+            add(v);
+        }
+        for (; i + U <= count; i += U) {
+            Vec<T, V> v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = load(false);
+#pragma unroll
+            for (int u = 0; u < U; ++u) add(v[u]);
+        }
+        for (; i < count; ++i) add(load(false));
+        if (row >= L.ty) return;
+        // (mean, centred squares) of the vector, or of each channel
+        const float inv = count > 0 ? __fdividef(1.f, (float)count) : 0.f;
+        Stats all = {0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float a = j & 1 ? s1[j / 2].y : s1[j / 2].x, b = j & 1 ? s2[j / 2].y : s2[j / 2].x;
+            const float k = -(j & 1 ? pivot[j / 2].y : pivot[j / 2].x);
+            const Stats one = {(float)max(count, 0), fmaf(a, inv, k), fmaxf(b - a * a * inv, 0.f)};
+            if (WHOLE) all = join(all, one);
+            else scratch[row * L.p.channels + c + j] = make_float2(one.mean, one.m2);
+        }
+        if (WHOLE) scratch[row * L.vectors + c / V] = make_float2(all.mean, all.m2);
+    }
+
+    // The terms of the backward pass: h, z and e = dy act'(z).
+    template <int ACT>
+    __device__ __forceinline__ static void terms(const Vec<T, V> &a, const Vec<T, V> &b, const float2 (&shift)[P],
+                                                 const float2 (&rstd)[P], const float2 (&gamma)[P], const float2 (&beta)[P],
+                                                 int j, float2 fa, float2 fb, float2 &h, float2 &e)
+    {
+        h = __fmul2_rn(__fadd2_rn(fa, shift[WHOLE ? 0 : j]), rstd[WHOLE ? 0 : j]);
+        e = ACT == NT_ACT_NONE ? fb : times_slope2<ACT>(fb, __ffma2_rn(gamma[j], h, beta[j]));
+    }
+
+    __device__ __forceinline__ void statistics(int c, float2 (&shift)[P], float2 (&rstd)[P]) const
+    {
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            if (WHOLE && j) break;
+            const int64_t g0 = n * L.p.groups + group(c, 2 * j), g1 = n * L.p.groups + group(c, 2 * j + 1);
+            shift[j] = make_float2(-__ldg(L.p.mean + g0), -__ldg(L.p.mean + g1));
+            rstd[j] = make_float2(__ldg(L.p.rstd + g0), __ldg(L.p.rstd + g1));
+        }
+    }
+
+    template <int ACT>
+    __device__ __forceinline__ void backward_sums(int c, int count, int near, int slot0) const
+    {
+        constexpr int U = 2;
+        float2 s1[P] = {}, s2[P] = {}, shift[P], rstd[P], gamma[P], beta[P];
+        statistics(c, shift, rstd);
+        channels(L.p.gamma, 1.f, c, gamma);
+        channels(L.p.beta, 0.f, c, beta);
+        char *at, *gt;
+        int x = seek(L.p.x, 0, c, at);
+        seek(L.p.dy, 0, c, gt);
+        const Walk w(L.p.x, L.p.width, rows, rest, sizeof(T)), g(L.p.dy, L.p.width, rows, rest, sizeof(T));
+        auto load = [&](Vec<T, V> &a, Vec<T, V> &b, bool stream) {
+            a = load_vec<T, V>(reinterpret_cast<const T *>(at), stream);
+            b = load_vec<T, V>(reinterpret_cast<const T *>(gt), stream);
+            at += w.step;
+            gt += g.step;
+            if (forth(x)) at += w.wrap, gt += g.wrap;
+        };
+        auto add = [&](const Vec<T, V> &a, const Vec<T, V> &b) {
+            float2 fa[P], fb[P];
+            unpack<T, V>(a, fa);
+            unpack<T, V>(b, fb);
+#pragma unroll
+            for (int j = 0; j < P; ++j) {
+                float2 h, e;
+                terms<ACT>(a, b, shift, rstd, gamma, beta, j, fa[j], fb[j], h, e);
+                s1[j] = __fadd2_rn(s1[j], e);
+                s2[j] = __ffma2_rn(e, h, s2[j]);
+            }
+        };
+        Vec<T, V> *keep = kept + 2 * slot0 * NT + threadIdx.x;
+        int i = 0;
+        for (; i < near; ++i, keep += 2 * NT) {
+            Vec<T, V> a, b;
+            load(a, b, true);
+            keep[0] = a;
+            keep[NT] = b;
+            add(a, b);
+        }
+        for (; i + U <= count; i += U) {
+            Vec<T, V> a[U], b[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) load(a[u], b[u], false);
+#pragma unroll
+            for (int u = 0; u < U; ++u) add(a[u], b[u]);
+        }
+        for (; i < count; ++i) {
+            Vec<T, V> a, b;
+            load(a, b, false);
+            add(a, b);
+        }
+        if (row < L.ty)
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                scratch[row * L.p.channels + c + j] =
+                    j & 1 ? make_float2(s1[j / 2].y, s2[j / 2].y) : make_float2(s1[j / 2].x, s2[j / 2].x);
+    }
+
+    // ---- pass 2, the texels read last first ----
+    template <int ACT>
+    __device__ __forceinline__ void forward_apply(int c, int count, int near, int slot0) const
+    {
+        constexpr int U = 4;
+        float2 shift[P], scale[P], beta[P];
+        channels(L.p.gamma, 1.f, c, scale);
+        channels(L.p.beta, 0.f, c, beta);
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const float2 a = stat[group(c, 2 * j)], b = stat[group(c, 2 * j + 1)];
+            shift[j] = make_float2(-a.x, -b.x);
+            scale[j] = __fmul2_rn(scale[j], make_float2(a.y, b.y));
+        }
+        char *at, *out;
+        int x = seek(L.p.x, count - 1, c, at);
+        seek(L.p.y, count - 1, c, out);
+        const Walk w(L.p.x, L.p.width, rows, rest, sizeof(T)), o(L.p.y, L.p.width, rows, rest, sizeof(T));
+        int xo = x;
+        auto load = [&] {
+            const Vec<T, V> v = load_vec<T, V>(reinterpret_cast<const T *>(at), true);
+            at -= w.step;
+            if (back(x)) at -= w.wrap;
+            return v;
+        };
+        auto put = [&](const Vec<T, V> &v) {
+            float2 f[P];
+            unpack<T, V>(v, f);
+#pragma unroll
+            for (int j = 0; j < P; ++j)
+                f[j] = activate2<ACT>(__ffma2_rn(__fadd2_rn(f[j], shift[WHOLE ? 0 : j]), scale[j], beta[j]));
+            store_vec<T, V>(reinterpret_cast<T *>(out), pack<T, V>(f));
+            out -= o.step;
+            if (back(xo)) out -= o.wrap;
+        };
+        int i = count;
+        for (; i - U >= near; i -= U) {
+            Vec<T, V> v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = load();
+#pragma unroll
+            for (int u = 0; u < U; ++u) put(v[u]);
+        }
+        for (; i > near; --i) put(load());
+        const Vec<T, V> *keep = kept + (slot0 + near - 1) * NT + threadIdx.x;
+        for (; i > 0; --i, keep -= NT) put(*keep);
+    }
+
+    template <int ACT>
+    __device__ __forceinline__ void backward_apply(int c, int count, int near, int slot0) const
+    {
+        constexpr int U = 2;
+        float2 shift[P], rstd[P], gamma[P], beta[P], k1[P], k2[P];
+        statistics(c, shift, rstd);
+        channels(L.p.gamma, 1.f, c, gamma);
+        channels(L.p.beta, 0.f, c, beta);
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            if (WHOLE && j) break;
+            const float2 a = stat[group(c, 2 * j)], b = stat[group(c, 2 * j + 1)];
+            k1[j] = make_float2(-a.x * L.inv_count, -b.x * L.inv_count);
+            k2[j] = make_float2(-a.y * L.inv_count, -b.y * L.inv_count);
+        }
+        char *at, *gt, *out;
+        int x = seek(L.p.x, count - 1, c, at);
+        seek(L.p.dy, count - 1, c, gt);
+        seek(L.p.dx, count - 1, c, out);
+        const Walk w(L.p.x, L.p.width, rows, rest, sizeof(T)), g(L.p.dy, L.p.width, rows, rest, sizeof(T)),
+            o(L.p.dx, L.p.width, rows, rest, sizeof(T));
+        int xo = x;
+        auto load = [&](Vec<T, V> &a, Vec<T, V> &b) {
+            a = load_vec<T, V>(reinterpret_cast<const T *>(at), true);
+            b = load_vec<T, V>(reinterpret_cast<const T *>(gt), true);
+            at -= w.step;
+            gt -= g.step;
+            if (back(x)) at -= w.wrap, gt -= g.wrap;
+        };
+        auto put = [&](const Vec<T, V> &a, const Vec<T, V> &b) {
+            float2 fa[P], fb[P];
+            unpack<T, V>(a, fa);
+            unpack<T, V>(b, fb);
+#pragma unroll
+            for (int j = 0; j < P; ++j) {
+                const int s = WHOLE ? 0 : j;
+                float2 h, e;
+                terms<ACT>(a, b, shift, rstd, gamma, beta, j, fa[j], fb[j], h, e);
+                fa[j] = __fmul2_rn(rstd[s], __ffma2_rn(gamma[j], e, __ffma2_rn(h, k2[s], k1[s])));
+            }
+            store_vec<T, V>(reinterpret_cast<T *>(out), pack<T, V>(fa));
+            out -= o.step;
+            if (back(xo)) out -= o.wrap;
+        };
+        int i = count;
+        for (; i - U >= near; i -= U) {
+            Vec<T, V> a[U], b[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) load(a[u], b[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u) put(a[u], b[u]);
+        }
+        for (; i > near; --i) {
+            Vec<T, V> a, b;
+            load(a, b);
+            put(a, b);
+        }
+        const Vec<T, V> *keep = kept + 2 * (slot0 + near - 1) * NT + threadIdx.x;
+        for (; i > 0; --i, keep -= 2 * NT) put(keep[0], keep[NT]);
+    }
+
+    template <int ACT>
+    __device__ __forceinline__ void first(int c, int count, int near, int slot0) const
+    {
+        if constexpr (BACKWARD) backward_sums<ACT>(c, count, near, slot0);
+        else forward_sums(c, count, near, slot0);
+    }
+    template <int ACT>
+    __device__ __forceinline__ void second(int c, int count, int near, int slot0) const
+    {
+        if constexpr (BACKWARD) backward_apply<ACT>(c, count, near, slot0);
+        else forward_apply<ACT>(c, count, near, slot0);
+    }
+};
+
 // WHOLE: a vector lies in one group.
 template <class T, int V, bool WHOLE, bool BACKWARD>
-__global__ void __launch_bounds__(kThreads, WHOLE ? 2 : 1) norm_kernel(const __grid_constant__ NormLaunch L, unsigned int *status)
+__global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads), WHOLE ? 2 : 1)
+    norm_kernel(const __grid_constant__ NormLaunch L, unsigned int *status)
 {
-    constexpr int U = BACKWARD ? 2 : 4;  // texels in flight
-    using Vec = norm::Vec<T, V>;
+    constexpr int NT = BACKWARD ? kBackwardThreads : kForwardThreads, kWarps = NT / 32;
     extern __shared__ __align__(16) uint8_t smem[];
     const NtGroupNorm &p = L.p;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t n = blockIdx.x / L.splits;
     const int split = blockIdx.x % L.splits;
     const int lo = (int)((int64_t)L.texels * split / L.splits), hi = (int)((int64_t)L.texels * (split + 1) / L.splits);
-    const int row = tid / L.tx, col = tid % L.tx;
-    const int mine = row < L.ty && lo + row < hi ? (hi - lo - row + L.ty - 1) / L.ty : 0;  // texels of this thread
     // shared memory: group results [groups], group partials [groups], scratch, kept vectors
     float2 *stat = reinterpret_cast<float2 *>(smem), *part = stat + p.groups, *scratch = part + p.groups;
-    Vec *kept = reinterpret_cast<Vec *>(smem + L.scratch);
-
-    const T *x = static_cast<const T *>(p.x.data) + n * p.x.image_stride;
-    const T *dy = BACKWARD ? static_cast<const T *>(p.dy.data) + n * p.dy.image_stride : nullptr;
-    const NtFeatureMap &out_map = BACKWARD ? p.dx : p.y;
-    T *out = static_cast<T *>(out_map.data) + n * out_map.image_stride;
-    auto texel = [&](const NtFeatureMap &f, int i) -> int64_t {
-        const int t = lo + row + i * L.ty;
-        if (L.flat) return t * f.texel_stride;
-        const int y = t / p.width;
-        return y * f.row_stride + (t - y * p.width) * f.texel_stride;
-    };
-
-    // ---- pass 1 ----
+    const int row = tid / L.tx, col = tid % L.tx;
+    const int mine = row < L.ty && lo + row < hi ? (hi - lo - row + L.ty - 1) / L.ty : 0;  // texels of this thread
+    const int most = (hi - lo + L.ty - 1) / L.ty;                                        // and of any
+    const Threads<T, V, WHOLE, BACKWARD> th = {L,    n,       lo, row, col, mine,
+                                               stat, scratch, reinterpret_cast<Vec<T, V> *>(smem + L.scratch),
+                                               L.ty / p.width, L.ty % p.width};
     int slot0 = 0;
-    for (int v0 = 0; v0 < L.vectors; v0 += L.tx) {
-        const int vec = v0 + col, c = vec * V;
-        const int count = vec < L.vectors ? mine : 0;
-        float s1[V] = {}, s2[V] = {};
-        if constexpr (!BACKWARD) {
-            float pivot[V] = {};
-            for (int i = 0; i < count; i += U) {
-                Vec a[U];
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (i + u < count) a[u] = load_vec<T, V>(x + texel(p.x, i + u) + c, slot0 + i + u < L.keep);
-                if (i == 0)
-#pragma unroll
-                    for (int j = 0; j < V; ++j) pivot[j] = to_f32(a[0].v[j]);
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (i + u >= count) break;
-                    if (slot0 + i + u < L.keep) kept[(slot0 + i + u) * kThreads + tid] = a[u];
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        const float d = to_f32(a[u].v[j]) - pivot[j];
-                        s1[j] += d;
-                        s2[j] = fmaf(d, d, s2[j]);
-                    }
-                }
-            }
-            if (vec < L.vectors && row < L.ty) {
-                const float inv = count ? __fdividef(1.f, (float)count) : 0.f;
-                Stats all = {0.f, 0.f, 0.f};
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const Stats one = {(float)count, fmaf(s1[j], inv, pivot[j]), fmaxf(s2[j] - s1[j] * s1[j] * inv, 0.f)};
-                    if (WHOLE) all = join(all, one);
-                    else scratch[row * p.channels + c + j] = make_float2(one.mean, one.m2);
-                }
-                if (WHOLE) scratch[row * L.vectors + vec] = make_float2(all.mean, all.m2);
-            }
-        } else {
-            float mean[V], rstd[V], gamma[V], beta[V];
-            if (vec < L.vectors)
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const int64_t g = n * p.groups + (c + (WHOLE ? 0 : j)) / L.per;
-                    mean[j] = WHOLE && j ? mean[0] : __ldg(p.mean + g);
-                    rstd[j] = WHOLE && j ? rstd[0] : __ldg(p.rstd + g);
-                    gamma[j] = p.gamma ? __ldg(p.gamma + c + j) : 1.f;
-                    beta[j] = p.beta ? __ldg(p.beta + c + j) : 0.f;
-                }
-            for (int i = 0; i < count; i += U) {
-                Vec a[U], b[U];
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (i + u < count) {
-                        a[u] = load_vec<T, V>(x + texel(p.x, i + u) + c, slot0 + i + u < L.keep);
-                        b[u] = load_vec<T, V>(dy + texel(p.dy, i + u) + c, slot0 + i + u < L.keep);
-                    }
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (i + u >= count) break;
-                    if (slot0 + i + u < L.keep) {
-                        kept[(2 * (slot0 + i + u)) * kThreads + tid] = a[u];
-                        kept[(2 * (slot0 + i + u) + 1) * kThreads + tid] = b[u];
-                    }
-                    float e[V], h[V], z[V];
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        h[j] = (to_f32(a[u].v[j]) - mean[j]) * rstd[j];
-                        z[j] = fmaf(gamma[j], h[j], beta[j]);
-                        e[j] = to_f32(b[u].v[j]);
-                    }
-                    times_slope<V>(e, z, p.activation);
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        s1[j] += e[j];
-                        s2[j] = fmaf(e[j], h[j], s2[j]);
-                    }
-                }
-            }
-            if (vec < L.vectors && row < L.ty)
-#pragma unroll
-                for (int j = 0; j < V; ++j) scratch[row * p.channels + c + j] = make_float2(s1[j], s2[j]);
+    for (int v0 = 0; v0 < L.vectors; v0 += L.tx, slot0 += most) {
+        const int vec = v0 + col;
+        if (vec >= L.vectors || row >= L.ty) continue;
+        const int near = min(max(L.keep - slot0, 0), mine);
+        switch (BACKWARD ? p.activation : NT_ACT_NONE) {
+        case NT_ACT_RELU: th.template first<NT_ACT_RELU>(vec * V, mine, near, slot0); break;
+        case NT_ACT_SILU: th.template first<NT_ACT_SILU>(vec * V, mine, near, slot0); break;
+        case NT_ACT_GELU: th.template first<NT_ACT_GELU>(vec * V, mine, near, slot0); break;
+        default: th.template first<NT_ACT_NONE>(vec * V, mine, near, slot0); break;
         }
-        slot0 += (hi - lo + L.ty - 1) / L.ty;
     }
     __syncthreads();
 
@@ -331,7 +568,7 @@ __global__ void __launch_bounds__(kThreads, WHOLE ? 2 : 1) norm_kernel(const __g
         // the rows of each channel, folded in halves
         for (int rows = L.ty; rows > 1; rows = (rows + 1) >> 1) {
             const int half = (rows + 1) >> 1;
-            for (int i = tid; i < (rows - half) * p.channels; i += kThreads) {
+            for (int i = tid; i < (rows - half) * p.channels; i += NT) {
                 const float2 v = scratch[half * p.channels + i];
                 scratch[i].x += v.x;
                 scratch[i].y += v.y;
@@ -339,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, WHOLE ? 2 : 1) norm_kernel(const __g
             __syncthreads();
         }
         if (p.dgamma || p.dbeta)
-            for (int c = tid; c < p.channels; c += kThreads) L.channels_part[(int64_t)c * parts + blockIdx.x] = scratch[c];
+            for (int c = tid; c < p.channels; c += NT) L.channels_part[(int64_t)c * parts + blockIdx.x] = scratch[c];
         for (int g = warp; g < p.groups; g += kWarps) {
             float2 s = make_float2(0.f, 0.f);
             for (int e = lane; e < L.per; e += 32) {
@@ -394,68 +631,16 @@ __global__ void __launch_bounds__(kThreads, WHOLE ? 2 : 1) norm_kernel(const __g
     if (BACKWARD && !L.cluster && (p.dgamma || p.dbeta))
         for (int64_t c = (int64_t)warp * gridDim.x + blockIdx.x; c < p.channels; c += (int64_t)kWarps * gridDim.x) join_channel(L, (int)c);
 
-    // ---- pass 2, the texels read last first ----
     for (int v0 = (L.vectors - 1) / L.tx * L.tx; v0 >= 0; v0 -= L.tx) {
-        slot0 -= (hi - lo + L.ty - 1) / L.ty;
-        const int vec = v0 + col, c = vec * V;
-        if (vec >= L.vectors) continue;
-        float mean[V], scale[V], gamma[V], beta[V], k1[V], k2[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int g = (c + (WHOLE ? 0 : j)) / L.per;
-            gamma[j] = p.gamma ? __ldg(p.gamma + c + j) : 1.f;
-            beta[j] = p.beta ? __ldg(p.beta + c + j) : 0.f;
-            if constexpr (!BACKWARD) {
-                mean[j] = stat[g].x;
-                scale[j] = stat[g].y * gamma[j];
-            } else {
-                mean[j] = WHOLE && j ? mean[0] : __ldg(p.mean + n * p.groups + g);
-                scale[j] = WHOLE && j ? scale[0] : __ldg(p.rstd + n * p.groups + g);
-                k1[j] = stat[g].x * L.inv_count;
-                k2[j] = stat[g].y * L.inv_count;
-            }
-        }
-        for (int i = mine - 1; i >= 0; i -= U) {
-            Vec a[U], b[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int k = i - u, slot = slot0 + k;
-                if (k < 0) continue;
-                const bool near = slot < L.keep;
-                if constexpr (!BACKWARD) {
-                    a[u] = near ? kept[slot * kThreads + tid] : load_vec<T, V>(x + texel(p.x, k) + c, true);
-                } else {
-                    a[u] = near ? kept[2 * slot * kThreads + tid] : load_vec<T, V>(x + texel(p.x, k) + c, true);
-                    b[u] = near ? kept[(2 * slot + 1) * kThreads + tid] : load_vec<T, V>(dy + texel(p.dy, k) + c, true);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int k = i - u;
-                if (k < 0) continue;
-                Vec r;
-                float z[V];
-                if constexpr (!BACKWARD) {
-#pragma unroll
-                    for (int j = 0; j < V; ++j) z[j] = fmaf(to_f32(a[u].v[j]) - mean[j], scale[j], beta[j]);
-                    activate_all<V>(z, p.activation);
-#pragma unroll
-                    for (int j = 0; j < V; ++j) r.v[j] = from_f32<T>(z[j]);
-                } else {
-                    float e[V], h[V];
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        h[j] = (to_f32(a[u].v[j]) - mean[j]) * scale[j];
-                        z[j] = fmaf(gamma[j], h[j], beta[j]);
-                        e[j] = to_f32(b[u].v[j]);
-                    }
-                    times_slope<V>(e, z, p.activation);
-#pragma unroll
-                    for (int j = 0; j < V; ++j)
-                        r.v[j] = from_f32<T>(scale[j] * (fmaf(gamma[j], e[j], -k1[j]) - h[j] * k2[j]));
-                }
-                store_vec<T, V>(out + texel(out_map, k) + c, r);
-            }
+        slot0 -= most;
+        const int vec = v0 + col;
+        if (vec >= L.vectors || mine == 0) continue;
+        const int near = min(max(L.keep - slot0, 0), mine);
+        switch (p.activation) {
+        case NT_ACT_RELU: th.template second<NT_ACT_RELU>(vec * V, mine, near, slot0); break;
+        case NT_ACT_SILU: th.template second<NT_ACT_SILU>(vec * V, mine, near, slot0); break;
+        case NT_ACT_GELU: th.template second<NT_ACT_GELU>(vec * V, mine, near, slot0); break;
+        default: th.template second<NT_ACT_NONE>(vec * V, mine, near, slot0); break;
         }
     }
 }
