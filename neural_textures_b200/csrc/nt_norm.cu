@@ -24,13 +24,14 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 struct Plan {
     int splits;
     bool cluster;
-    int per_sm;  // blocks that an SM holds: two, or one of the kernels whose vectors cross groups
+    int per_sm;  // blocks that an SM holds: two, or one where vectors cross groups or the sums of a texel need the room
 };
 
 Plan plan(const NtGroupNorm *p)
 {
     const int64_t values = (int64_t)p->height * p->width * p->channels;
-    const int per_sm = p->channels / p->groups % (16 / layer_dtype_size(p->dtype)) == 0 ? 2 : 1;
+    const bool whole = p->channels / p->groups % (16 / layer_dtype_size(p->dtype)) == 0;
+    const int per_sm = whole && p->channels <= 2048 ? 2 : 1;
     const int64_t resident = (int64_t)per_sm * sm_count();
     // at least 4 vectors of 8 channels for each of 512 threads
     const int64_t wanted = std::max<int64_t>(1, values / (512 * 32));
@@ -76,33 +77,38 @@ cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
     char *ws = static_cast<char *>(p->workspace);
     NormLaunch L = {};
     L.p = *p;
-    const int v = vector_width(p, size, backward);
+    const int threads = backward ? kBackwardThreads : kForwardThreads, ring = backward ? kBackwardRing : kForwardRing;
     L.per = p->channels / p->groups;
     L.splits = pl.splits;
     L.cluster = pl.cluster;
     L.texels = p->height * p->width;
-    L.vectors = p->channels / v;
-    const int threads = backward ? kBackwardThreads : kForwardThreads;
-    // threads along a texel's vectors: all of them, or the number of turns that leaves the fewest threads idle
-    double used = 0;
-    for (int turns = (int)ceil_div(L.vectors, threads), last = turns + 3; turns <= last; ++turns) {
-        const int tx = (int)ceil_div(L.vectors, turns), ty = threads / tx;
-        const double share = (double)L.vectors * ty / ((double)turns * threads);
-        if (share > used + 0.05) used = share, L.tx = tx, L.ty = ty;
-    }
     L.inv_count = 1.f / ((float)L.texels * (float)L.per);
     L.barrier = reinterpret_cast<unsigned int *>(ws);
     L.groups_part = reinterpret_cast<float2 *>(ws + at.groups_at);
     L.channels_part = reinterpret_cast<float2 *>(ws + at.channels_at);
-    const bool whole = L.per % v == 0;
-    const size_t entries = (size_t)L.ty * (backward || !whole ? p->channels : L.vectors);
-    L.scratch = (int32_t)align16((2 * (size_t)p->groups + entries) * sizeof(float2));
-    const size_t slot = (size_t)threads * v * size * (backward ? 2 : 1);
     const size_t most = 227 * 1024 / pl.per_sm - 1024;
-    const size_t room = (size_t)L.scratch < most ? most - L.scratch : 0;
-    const int64_t slots = ceil_div(ceil_div(L.texels, L.splits), L.ty) * ceil_div(L.vectors, L.tx);
-    L.keep = (int32_t)std::min<int64_t>(slots, room / slot);
-    const size_t smem = L.scratch + L.keep * slot;
+    size_t smem = 0;
+    int v = vector_width(p, size, backward);
+    bool whole = true;
+    for (;; v /= 2) {  // narrower vectors where the sums of very many groups leave no room for the ring
+        whole = L.per % v == 0;
+        L.vectors = p->channels / v;
+        // threads along a texel's vectors: all of them, or the number of turns that leaves the fewest threads idle
+        double used = 0;
+        for (int turns = (int)ceil_div(L.vectors, threads), last = turns + 3; turns <= last; ++turns) {
+            const int tx = (int)ceil_div(L.vectors, turns), ty = threads / tx;
+            const double share = (double)L.vectors * ty / ((double)turns * threads);
+            if (share > used + 0.05) used = share, L.tx = tx, L.ty = ty;
+        }
+        const size_t entries = (size_t)L.ty * (backward || !whole ? p->channels : L.vectors);
+        L.scratch = (int32_t)align16((2 * (size_t)p->groups + entries) * sizeof(float2));
+        const size_t slot = (size_t)threads * v * size * (backward ? 2 : 1);
+        const int64_t room = (int64_t)((most - L.scratch) / slot);
+        const int64_t slots = ceil_div(ceil_div(L.texels, L.splits), L.ty) * ceil_div(L.vectors, L.tx);
+        L.keep = (int32_t)(slots <= room ? slots : std::max<int64_t>(room - ring, 0));
+        smem = L.scratch + (slots <= room ? slots : L.keep + ring) * slot;
+        if (smem <= most || v == 1) break;
+    }
 
     const NormKernel kernel = backward ? backward_kernel(p->dtype, v, whole) : forward_kernel(p->dtype, v, whole);
     unsigned int *status = nullptr;

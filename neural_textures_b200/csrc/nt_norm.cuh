@@ -8,8 +8,10 @@
 //      first value and joined pairwise after that, so that a common offset costs no digits.
 //      Backward: per channel sums of e = dy act'(z) and e h.
 //   2. the result, from the image's joined sums.
-// What the first pass read is kept in shared memory as far as it goes (the oldest part), and the
-// second pass starts with the texels read last, which are still in L2.
+// A thread's vectors arrive by asynchronous copies in its own slots of shared memory, so that loads stay in
+// flight while it computes and no barrier is needed.  The slots hold a ring of a few vectors and, as far as
+// they go, the texels read first, for the second pass; that one begins with the texels read last, which
+// are still in L2.
 // Blocks of an image meet in a cluster (up to 8), where they read each other's sums from shared memory, or,
 // for large maps, at a barrier of the whole cooperative grid, with the sums in the workspace.
 // All sums are joined in a fixed order.
@@ -21,6 +23,7 @@ namespace nt {
 namespace norm {
 
 constexpr int kForwardThreads = 512;
+constexpr int kForwardRing = 6, kBackwardRing = 4;  // 96 KB in flight on an SM cover the latency of HBM
 constexpr int kBackwardThreads = 384;  // 84 registers a thread with two blocks on an SM: 64 spill
 constexpr int kMaxCluster = 8;
 constexpr uint32_t kSpinLimit = 1u << 24;
@@ -32,7 +35,7 @@ struct NormLaunch {
     int32_t cluster;    // 1: they form a cluster; 0: the grid meets at *barrier
     int32_t texels, vectors;  // vectors of V channels in a texel
     int32_t tx, ty;     // threads along channels and texels
-    int32_t keep;       // vectors of a thread (of x, and of dy) that stay in shared memory
+    int32_t keep;       // vectors of a thread (of x, and of dy) that stay in shared memory, in front of its ring
     int32_t scratch;    // bytes of shared memory in front of them
     float inv_count;    // 1 / values of a group
     float2 *groups_part;    // [image][group][split]
@@ -61,18 +64,19 @@ struct alignas(V * sizeof(T) > 16 ? 16 : V * sizeof(T)) Vec {
     T v[V];
 };
 
-// Streaming: read once (its second reading comes from shared memory).
+// A vector from global to shared memory: asynchronous, but for 2-byte vectors.
 template <class T, int V>
-__device__ __forceinline__ Vec<T, V> load_vec(const T *p, bool stream)
+__device__ __forceinline__ void fetch(Vec<T, V> *slot, const char *p)
 {
-    Vec<T, V> r;
     constexpr int bytes = V * sizeof(T);
-    if constexpr (bytes == 16) *reinterpret_cast<uint4 *>(&r) = stream ? __ldcs(reinterpret_cast<const uint4 *>(p)) : *reinterpret_cast<const uint4 *>(p);
-    else if constexpr (bytes == 8) *reinterpret_cast<uint2 *>(&r) = stream ? __ldcs(reinterpret_cast<const uint2 *>(p)) : *reinterpret_cast<const uint2 *>(p);
-    else if constexpr (bytes == 4) *reinterpret_cast<uint32_t *>(&r) = stream ? __ldcs(reinterpret_cast<const uint32_t *>(p)) : *reinterpret_cast<const uint32_t *>(p);
-    else *reinterpret_cast<uint16_t *>(&r) = stream ? __ldcs(reinterpret_cast<const uint16_t *>(p)) : *reinterpret_cast<const uint16_t *>(p);
-    return r;
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(slot);
+    if constexpr (bytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(p) : "memory");
+    else if constexpr (bytes >= 4) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(p), "n"(bytes) : "memory");
+    else *slot = *reinterpret_cast<const Vec<T, V> *>(p);
 }
+__device__ __forceinline__ void fetch_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void fetch_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 template <class T, int V>
 __device__ __forceinline__ void store_vec(T *p, const Vec<T, V> &r)
@@ -213,25 +217,11 @@ struct Threads {
     int rows, rest;  // ty texels: whole rows of the image, and the rest
 
     // The x coordinate of texel i of this thread, and where it lies in map f.
-    __device__ __forceinline__ int seek(const NtFeatureMap &f, int i, int c, char *&at) const
+    __device__ __forceinline__ int seek(const NtFeatureMap &f, int i, int c, const char *&at) const
     {
         const int t = lo + row + i * L.ty, y = t / L.p.width, x = t - y * L.p.width;
-        at = static_cast<char *>(f.data) + (n * f.image_stride + y * f.row_stride + x * f.texel_stride + c) * (int64_t)sizeof(T);
+        at = static_cast<const char *>(f.data) + (n * f.image_stride + y * f.row_stride + x * f.texel_stride + c) * (int64_t)sizeof(T);
         return x;
-    }
-    __device__ __forceinline__ bool forth(int &x) const
-    {
-        x += rest;
-        const bool over = x >= L.p.width;
-        if (over) x -= L.p.width;
-        return over;
-    }
-    __device__ __forceinline__ bool back(int &x) const
-    {
-        x -= rest;
-        const bool over = x < 0;
-        if (over) x += L.p.width;
-        return over;
     }
     // Per-channel values of a parameter, in pairs.
     __device__ __forceinline__ void channels(const float *param, float other, int c, float2 (&v)[P]) const
@@ -243,57 +233,145 @@ struct Threads {
     // Group of channel c + i (of the whole vector, when it lies in one).
     __device__ __forceinline__ int group(int c, int i) const { return (c + (WHOLE || i >= V ? 0 : i)) / L.per; }
 
+    // The slots of this thread: `near` kept vectors, then the ring.  In the backward pass a slot holds x and,
+    // NT vectors on, dy.
+    static constexpr int kMaps = BACKWARD ? 2 : 1;
+    static constexpr int kSlot = NT * kMaps;
+    static constexpr int kDepth = BACKWARD ? kBackwardRing : kForwardRing;
+    struct Source {
+        const Threads &t;
+        const char *x, *dy;
+        int at;  // x coordinate
+        Walk wx, wdy;
+        __device__ __forceinline__ Source(const Threads &t, int i, int c)
+            : t(t), dy(nullptr), wx(t.L.p.x, t.L.p.width, t.rows, t.rest, sizeof(T)),
+              wdy(t.L.p.dy, t.L.p.width, t.rows, t.rest, sizeof(T))
+        {
+            at = t.seek(t.L.p.x, i, c, x);
+            if (BACKWARD) t.seek(t.L.p.dy, i, c, dy);
+        }
+        __device__ __forceinline__ void get(Vec<T, V> *slot) const
+        {
+            fetch<T, V>(slot, x);
+            if (BACKWARD) fetch<T, V>(slot + NT, dy);
+        }
+        __device__ __forceinline__ void forth()
+        {
+            x += wx.step;
+            if (BACKWARD) dy += wdy.step;
+            at += t.rest;
+            if (at >= t.L.p.width) {
+                at -= t.L.p.width;
+                x += wx.wrap;
+                if (BACKWARD) dy += wdy.wrap;
+            }
+        }
+        __device__ __forceinline__ void back()
+        {
+            x -= wx.step;
+            if (BACKWARD) dy -= wdy.step;
+            at -= t.rest;
+            if (at < 0) {
+                at += t.L.p.width;
+                x -= wx.wrap;
+                if (BACKWARD) dy -= wdy.wrap;
+            }
+        }
+    };
+
+    // use(slot) for texels 0 .. count - 1.  Afterwards the last kDepth of them are still in the ring, texel i in
+    // slot (i - near) % kDepth.
+    template <class Use>
+    __device__ __forceinline__ void each_forth(int c, int count, int near, int slot0, Use use) const
+    {
+        Vec<T, V> *keep = kept + slot0 * kSlot + threadIdx.x, *const ring = kept + L.keep * kSlot + threadIdx.x;
+        Source src(*this, 0, c);
+        for (int i = 0; i < near; ++i, src.forth()) src.get(keep + i * kSlot);
+        fetch_commit();
+#pragma unroll
+        for (int u = 0; u < kDepth; ++u) {
+            if (near + u < count) {
+                src.get(ring + u * kSlot);
+                src.forth();
+            }
+            fetch_commit();
+        }
+        fetch_wait<kDepth>();
+#pragma unroll 2
+        for (int i = 0; i < near; ++i) use(keep + i * kSlot);
+        Vec<T, V> *slot = ring;
+#pragma unroll 2
+        for (int i = near; i < count; ++i) {
+            fetch_wait<kDepth - 1>();
+            use(slot);
+            // the next texel of this slot, unless this one stays for the second pass
+            if (i + kDepth < count) {
+                src.get(slot);
+                src.forth();
+            }
+            fetch_commit();
+            slot = slot == ring + (kDepth - 1) * kSlot ? ring : slot + kSlot;
+        }
+    }
+
+    // The same from count - 1 down to 0, the ring still as each_forth left it for this column, or `fresh`.
+    template <class Use>
+    __device__ __forceinline__ void each_back(int c, int count, int near, int slot0, bool fresh, Use use) const
+    {
+        const Vec<T, V> *keep = kept + slot0 * kSlot + threadIdx.x;
+        Vec<T, V> *const ring = kept + L.keep * kSlot + threadIdx.x, *const last = ring + (kDepth - 1) * kSlot;
+        if (count > near) {
+            Vec<T, V> *slot = ring + (count - 1 - near) % kDepth * kSlot;
+            const int first = fresh ? count - 1 : count - 1 - kDepth;
+            Source src(*this, max(first, 0), c);
+#pragma unroll
+            for (int u = 0; u < kDepth; ++u) {
+                if (fresh) {
+                    if (count - 1 - u >= near) {
+                        src.get(slot);
+                        src.back();
+                    }
+                    slot = slot == ring ? last : slot - kSlot;
+                }
+                fetch_commit();
+            }
+            slot = ring + (count - 1 - near) % kDepth * kSlot;
+#pragma unroll 2
+            for (int i = count - 1; i >= near; --i) {
+                fetch_wait<kDepth - 1>();
+                use(slot);
+                if (i - kDepth >= near) {
+                    src.get(slot);
+                    src.back();
+                }
+                fetch_commit();
+                slot = slot == ring ? last : slot - kSlot;
+            }
+        }
+#pragma unroll 2
+        for (int i = near - 1; i >= 0; --i) use(keep + i * kSlot);
+    }
+
     // ---- pass 1 ----
-    // `near` texels are kept from slot `slot0` on.
     __device__ __forceinline__ void forward_sums(int c, int count, int near, int slot0) const
     {
-        constexpr int U = 4;
         float2 pivot[P] = {}, s1[P] = {}, s2[P] = {};
-        char *at;
-        int x = seek(L.p.x, 0, c, at);
-        const Walk w(L.p.x, L.p.width, rows, rest, sizeof(T));
-        if (count > 0) unpack<T, V>(load_vec<T, V>(reinterpret_cast<const T *>(at), false), pivot);
-#pragma unroll
-        for (int j = 0; j < P; ++j) pivot[j] = make_float2(-pivot[j].x, -pivot[j].y);
-        auto load = [&](bool stream) {
-            const Vec<T, V> v = load_vec<T, V>(reinterpret_cast<const T *>(at), stream);
-            at += w.step;
-            if (forth(x)) at += w.wrap;
-            return v;
-        };
-        auto add = [&](const Vec<T, V> &v) {
+        bool begun = false;
+        each_forth(c, count, near, slot0, [&](const Vec<T, V> *slot) {
             float2 f[P];
-            unpack<T, V>(v, f);
+            unpack<T, V>(*slot, f);
+            if (!begun) {
+                begun = true;
+#pragma unroll
+                for (int j = 0; j < P; ++j) pivot[j] = make_float2(-f[j].x, -f[j].y);
+            }
 #pragma unroll
             for (int j = 0; j < P; ++j) {
                 const float2 d = __fadd2_rn(f[j], pivot[j]);
                 s1[j] = __fadd2_rn(s1[j], d);
                 s2[j] = __ffma2_rn(d, d, s2[j]);
             }
-        };
-        Vec<T, V> *keep = kept + slot0 * NT + threadIdx.x;
-        int i = 0;
-        for (; i + U <= near; i += U) {
-            Vec<T, V> v[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = load(true);
-#pragma unroll
-            for (int u = 0; u < U; ++u, keep += NT) *keep = v[u], add(v[u]);
-        }
-        for (; i < near; ++i, keep += NT) {
-            const Vec<T, V> v = load(true);
-            *keep = v;
-            add(v);
-        }
-        for (; i + U <= count; i += U) {
-            Vec<T, V> v[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = load(false);
-#pragma unroll
-            for (int u = 0; u < U; ++u) add(v[u]);
-        }
-        for (; i < count; ++i) add(load(false));
-        if (row >= L.ty) return;
+        });
         // (mean, centred squares) of the vector, or of each channel
         const float inv = count > 0 ? __fdividef(1.f, (float)count) : 0.f;
         Stats all = {0.f, 0.f, 0.f};
@@ -301,21 +379,20 @@ struct Threads {
         for (int j = 0; j < V; ++j) {
             const float a = j & 1 ? s1[j / 2].y : s1[j / 2].x, b = j & 1 ? s2[j / 2].y : s2[j / 2].x;
             const float k = -(j & 1 ? pivot[j / 2].y : pivot[j / 2].x);
-            const Stats one = {(float)max(count, 0), fmaf(a, inv, k), fmaxf(b - a * a * inv, 0.f)};
+            const Stats one = {(float)count, fmaf(a, inv, k), fmaxf(b - a * a * inv, 0.f)};
             if (WHOLE) all = join(all, one);
             else scratch[row * L.p.channels + c + j] = make_float2(one.mean, one.m2);
         }
         if (WHOLE) scratch[row * L.vectors + c / V] = make_float2(all.mean, all.m2);
     }
 
-    // The terms of the backward pass: h, z and e = dy act'(z).
+    // Terms of the backward pass: h and e = dy act'(z).
     template <int ACT>
-    __device__ __forceinline__ static void terms(const Vec<T, V> &a, const Vec<T, V> &b, const float2 (&shift)[P],
-                                                 const float2 (&rstd)[P], const float2 (&gamma)[P], const float2 (&beta)[P],
-                                                 int j, float2 fa, float2 fb, float2 &h, float2 &e)
+    __device__ __forceinline__ static void terms(float2 x, float2 dy, float2 shift, float2 rstd, float2 gamma, float2 beta, float2 &h,
+                                                 float2 &e)
     {
-        h = __fmul2_rn(__fadd2_rn(fa, shift[WHOLE ? 0 : j]), rstd[WHOLE ? 0 : j]);
-        e = ACT == NT_ACT_NONE ? fb : times_slope2<ACT>(fb, __ffma2_rn(gamma[j], h, beta[j]));
+        h = __fmul2_rn(__fadd2_rn(x, shift), rstd);
+        e = ACT == NT_ACT_NONE ? dy : times_slope2<ACT>(dy, __ffma2_rn(gamma, h, beta));
     }
 
     __device__ __forceinline__ void statistics(int c, float2 (&shift)[P], float2 (&rstd)[P]) const
@@ -332,67 +409,57 @@ struct Threads {
     template <int ACT>
     __device__ __forceinline__ void backward_sums(int c, int count, int near, int slot0) const
     {
-        constexpr int U = 2;
         float2 s1[P] = {}, s2[P] = {}, shift[P], rstd[P], gamma[P], beta[P];
         statistics(c, shift, rstd);
         channels(L.p.gamma, 1.f, c, gamma);
         channels(L.p.beta, 0.f, c, beta);
-        char *at, *gt;
-        int x = seek(L.p.x, 0, c, at);
-        seek(L.p.dy, 0, c, gt);
-        const Walk w(L.p.x, L.p.width, rows, rest, sizeof(T)), g(L.p.dy, L.p.width, rows, rest, sizeof(T));
-        auto load = [&](Vec<T, V> &a, Vec<T, V> &b, bool stream) {
-            a = load_vec<T, V>(reinterpret_cast<const T *>(at), stream);
-            b = load_vec<T, V>(reinterpret_cast<const T *>(gt), stream);
-            at += w.step;
-            gt += g.step;
-            if (forth(x)) at += w.wrap, gt += g.wrap;
-        };
-        auto add = [&](const Vec<T, V> &a, const Vec<T, V> &b) {
+        each_forth(c, count, near, slot0, [&](const Vec<T, V> *slot) {
             float2 fa[P], fb[P];
-            unpack<T, V>(a, fa);
-            unpack<T, V>(b, fb);
+            unpack<T, V>(slot[0], fa);
+            unpack<T, V>(slot[NT], fb);
 #pragma unroll
             for (int j = 0; j < P; ++j) {
                 float2 h, e;
-                terms<ACT>(a, b, shift, rstd, gamma, beta, j, fa[j], fb[j], h, e);
+                terms<ACT>(fa[j], fb[j], shift[WHOLE ? 0 : j], rstd[WHOLE ? 0 : j], gamma[j], beta[j], h, e);
                 s1[j] = __fadd2_rn(s1[j], e);
                 s2[j] = __ffma2_rn(e, h, s2[j]);
             }
-        };
-        Vec<T, V> *keep = kept + 2 * slot0 * NT + threadIdx.x;
-        int i = 0;
-        for (; i < near; ++i, keep += 2 * NT) {
-            Vec<T, V> a, b;
-            load(a, b, true);
-            keep[0] = a;
-            keep[NT] = b;
-            add(a, b);
-        }
-        for (; i + U <= count; i += U) {
-            Vec<T, V> a[U], b[U];
+        });
 #pragma unroll
-            for (int u = 0; u < U; ++u) load(a[u], b[u], false);
-#pragma unroll
-            for (int u = 0; u < U; ++u) add(a[u], b[u]);
-        }
-        for (; i < count; ++i) {
-            Vec<T, V> a, b;
-            load(a, b, false);
-            add(a, b);
-        }
-        if (row < L.ty)
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                scratch[row * L.p.channels + c + j] =
-                    j & 1 ? make_float2(s1[j / 2].y, s2[j / 2].y) : make_float2(s1[j / 2].x, s2[j / 2].x);
+        for (int j = 0; j < V; ++j)
+            scratch[row * L.p.channels + c + j] =
+                j & 1 ? make_float2(s1[j / 2].y, s2[j / 2].y) : make_float2(s1[j / 2].x, s2[j / 2].x);
     }
 
     // ---- pass 2, the texels read last first ----
+    // A result's way through its map, backwards.
+    struct Sink {
+        const Threads &t;
+        char *out;
+        int at;
+        Walk w;
+        __device__ __forceinline__ Sink(const Threads &t, const NtFeatureMap &f, int i, int c)
+            : t(t), w(f, t.L.p.width, t.rows, t.rest, sizeof(T))
+        {
+            const char *p;
+            at = t.seek(f, i, c, p);
+            out = const_cast<char *>(p);
+        }
+        __device__ __forceinline__ void put(const Vec<T, V> &v)
+        {
+            store_vec<T, V>(reinterpret_cast<T *>(out), v);
+            out -= w.step;
+            at -= t.rest;
+            if (at < 0) {
+                at += t.L.p.width;
+                out -= w.wrap;
+            }
+        }
+    };
+
     template <int ACT>
-    __device__ __forceinline__ void forward_apply(int c, int count, int near, int slot0) const
+    __device__ __forceinline__ void forward_apply(int c, int count, int near, int slot0, bool fresh) const
     {
-        constexpr int U = 4;
         float2 shift[P], scale[P], beta[P];
         channels(L.p.gamma, 1.f, c, scale);
         channels(L.p.beta, 0.f, c, beta);
@@ -402,44 +469,20 @@ struct Threads {
             shift[j] = make_float2(-a.x, -b.x);
             scale[j] = __fmul2_rn(scale[j], make_float2(a.y, b.y));
         }
-        char *at, *out;
-        int x = seek(L.p.x, count - 1, c, at);
-        seek(L.p.y, count - 1, c, out);
-        const Walk w(L.p.x, L.p.width, rows, rest, sizeof(T)), o(L.p.y, L.p.width, rows, rest, sizeof(T));
-        int xo = x;
-        auto load = [&] {
-            const Vec<T, V> v = load_vec<T, V>(reinterpret_cast<const T *>(at), true);
-            at -= w.step;
-            if (back(x)) at -= w.wrap;
-            return v;
-        };
-        auto put = [&](const Vec<T, V> &v) {
+        Sink sink(*this, L.p.y, count - 1, c);
+        each_back(c, count, near, slot0, fresh, [&](const Vec<T, V> *slot) {
             float2 f[P];
-            unpack<T, V>(v, f);
+            unpack<T, V>(*slot, f);
 #pragma unroll
             for (int j = 0; j < P; ++j)
                 f[j] = activate2<ACT>(__ffma2_rn(__fadd2_rn(f[j], shift[WHOLE ? 0 : j]), scale[j], beta[j]));
-            store_vec<T, V>(reinterpret_cast<T *>(out), pack<T, V>(f));
-            out -= o.step;
-            if (back(xo)) out -= o.wrap;
-        };
-        int i = count;
-        for (; i - U >= near; i -= U) {
-            Vec<T, V> v[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = load();
-#pragma unroll
-            for (int u = 0; u < U; ++u) put(v[u]);
-        }
-        for (; i > near; --i) put(load());
-        const Vec<T, V> *keep = kept + (slot0 + near - 1) * NT + threadIdx.x;
-        for (; i > 0; --i, keep -= NT) put(*keep);
+            sink.put(norm::pack<T, V>(f));
+        });
     }
 
     template <int ACT>
-    __device__ __forceinline__ void backward_apply(int c, int count, int near, int slot0) const
+    __device__ __forceinline__ void backward_apply(int c, int count, int near, int slot0, bool fresh) const
     {
-        constexpr int U = 2;
         float2 shift[P], rstd[P], gamma[P], beta[P], k1[P], k2[P];
         statistics(c, shift, rstd);
         channels(L.p.gamma, 1.f, c, gamma);
@@ -451,50 +494,20 @@ struct Threads {
             k1[j] = make_float2(-a.x * L.inv_count, -b.x * L.inv_count);
             k2[j] = make_float2(-a.y * L.inv_count, -b.y * L.inv_count);
         }
-        char *at, *gt, *out;
-        int x = seek(L.p.x, count - 1, c, at);
-        seek(L.p.dy, count - 1, c, gt);
-        seek(L.p.dx, count - 1, c, out);
-        const Walk w(L.p.x, L.p.width, rows, rest, sizeof(T)), g(L.p.dy, L.p.width, rows, rest, sizeof(T)),
-            o(L.p.dx, L.p.width, rows, rest, sizeof(T));
-        int xo = x;
-        auto load = [&](Vec<T, V> &a, Vec<T, V> &b) {
-            a = load_vec<T, V>(reinterpret_cast<const T *>(at), true);
-            b = load_vec<T, V>(reinterpret_cast<const T *>(gt), true);
-            at -= w.step;
-            gt -= g.step;
-            if (back(x)) at -= w.wrap, gt -= g.wrap;
-        };
-        auto put = [&](const Vec<T, V> &a, const Vec<T, V> &b) {
+        Sink sink(*this, L.p.dx, count - 1, c);
+        each_back(c, count, near, slot0, fresh, [&](const Vec<T, V> *slot) {
             float2 fa[P], fb[P];
-            unpack<T, V>(a, fa);
-            unpack<T, V>(b, fb);
+            unpack<T, V>(slot[0], fa);
+            unpack<T, V>(slot[NT], fb);
 #pragma unroll
             for (int j = 0; j < P; ++j) {
                 const int s = WHOLE ? 0 : j;
                 float2 h, e;
-                terms<ACT>(a, b, shift, rstd, gamma, beta, j, fa[j], fb[j], h, e);
+                terms<ACT>(fa[j], fb[j], shift[s], rstd[s], gamma[j], beta[j], h, e);
                 fa[j] = __fmul2_rn(rstd[s], __ffma2_rn(gamma[j], e, __ffma2_rn(h, k2[s], k1[s])));
             }
-            store_vec<T, V>(reinterpret_cast<T *>(out), pack<T, V>(fa));
-            out -= o.step;
-            if (back(xo)) out -= o.wrap;
-        };
-        int i = count;
-        for (; i - U >= near; i -= U) {
-            Vec<T, V> a[U], b[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) load(a[u], b[u]);
-#pragma unroll
-            for (int u = 0; u < U; ++u) put(a[u], b[u]);
-        }
-        for (; i > near; --i) {
-            Vec<T, V> a, b;
-            load(a, b);
-            put(a, b);
-        }
-        const Vec<T, V> *keep = kept + 2 * (slot0 + near - 1) * NT + threadIdx.x;
-        for (; i > 0; --i, keep -= 2 * NT) put(keep[0], keep[NT]);
+            sink.put(norm::pack<T, V>(fa));
+        });
     }
 
     template <int ACT>
@@ -504,10 +517,10 @@ struct Threads {
         else forward_sums(c, count, near, slot0);
     }
     template <int ACT>
-    __device__ __forceinline__ void second(int c, int count, int near, int slot0) const
+    __device__ __forceinline__ void second(int c, int count, int near, int slot0, bool fresh) const
     {
-        if constexpr (BACKWARD) backward_apply<ACT>(c, count, near, slot0);
-        else forward_apply<ACT>(c, count, near, slot0);
+        if constexpr (BACKWARD) backward_apply<ACT>(c, count, near, slot0, fresh);
+        else forward_apply<ACT>(c, count, near, slot0, fresh);
     }
 };
 
@@ -636,11 +649,12 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
         const int vec = v0 + col;
         if (vec >= L.vectors || mine == 0) continue;
         const int near = min(max(L.keep - slot0, 0), mine);
+        const bool fresh = v0 + L.tx < L.vectors;  // the ring holds the last columns of pass 1
         switch (p.activation) {
-        case NT_ACT_RELU: th.template second<NT_ACT_RELU>(vec * V, mine, near, slot0); break;
-        case NT_ACT_SILU: th.template second<NT_ACT_SILU>(vec * V, mine, near, slot0); break;
-        case NT_ACT_GELU: th.template second<NT_ACT_GELU>(vec * V, mine, near, slot0); break;
-        default: th.template second<NT_ACT_NONE>(vec * V, mine, near, slot0); break;
+        case NT_ACT_RELU: th.template second<NT_ACT_RELU>(vec * V, mine, near, slot0, fresh); break;
+        case NT_ACT_SILU: th.template second<NT_ACT_SILU>(vec * V, mine, near, slot0, fresh); break;
+        case NT_ACT_GELU: th.template second<NT_ACT_GELU>(vec * V, mine, near, slot0, fresh); break;
+        default: th.template second<NT_ACT_NONE>(vec * V, mine, near, slot0, fresh); break;
         }
     }
 }
