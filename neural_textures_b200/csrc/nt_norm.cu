@@ -69,6 +69,12 @@ int vector_width(const NtGroupNorm *p, int size, bool backward)
     return 1;
 }
 
+// Whether a map's texels are evenly spaced, `ty` of them by less than 2^31 bytes.
+bool flat(const NtFeatureMap &f, const NtGroupNorm *p, int size)
+{
+    return (p->height == 1 || f.row_stride == p->width * f.texel_stride) && f.texel_stride < ((int64_t)1 << 31) / (512 * size);
+}
+
 cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
 {
     const int size = layer_dtype_size(p->dtype);
@@ -81,6 +87,7 @@ cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
     L.per = p->channels / p->groups;
     L.splits = pl.splits;
     L.cluster = pl.cluster;
+    const bool even = flat(p->x, p, size) && flat(backward ? p->dy : p->y, p, size) && flat(backward ? p->dx : p->y, p, size);
     L.texels = p->height * p->width;
     L.inv_count = 1.f / ((float)L.texels * (float)L.per);
     L.barrier = reinterpret_cast<unsigned int *>(ws);
@@ -110,7 +117,7 @@ cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
         if (smem <= most || v == 1) break;
     }
 
-    const NormKernel kernel = backward ? backward_kernel(p->dtype, v, whole) : forward_kernel(p->dtype, v, whole);
+    const NormKernel kernel = backward ? backward_kernel(p->dtype, v, whole, even) : forward_kernel(p->dtype, v, whole, even);
     unsigned int *status = nullptr;
     cudaError_t e = cudaGetSymbolAddress(reinterpret_cast<void **>(&status), g_norm_status);
     if (e == cudaSuccess) e = set_smem_limit(reinterpret_cast<const void *>(kernel), 227 * 1024 - 1024);

@@ -23,7 +23,7 @@ namespace nt {
 namespace norm {
 
 constexpr int kForwardThreads = 512;
-constexpr int kForwardRing = 6, kBackwardRing = 4;  // 96 KB in flight on an SM cover the latency of HBM
+constexpr int kForwardRing = 4, kBackwardRing = 4;  // 64 and 96 KB in flight on an SM cover the latency of HBM
 constexpr int kBackwardThreads = 384;  // 84 registers a thread with two blocks on an SM: 64 spill
 constexpr int kMaxCluster = 8;
 constexpr uint32_t kSpinLimit = 1u << 24;
@@ -66,14 +66,50 @@ struct alignas(V * sizeof(T) > 16 ? 16 : V * sizeof(T)) Vec {
 
 // A vector from global to shared memory: asynchronous, but for 2-byte vectors.
 template <class T, int V>
-__device__ __forceinline__ void fetch(Vec<T, V> *slot, const char *p)
+__device__ __forceinline__ void fetch(uint32_t to, const char *p, uint64_t policy)
 {
     constexpr int bytes = V * sizeof(T);
-    const uint32_t to = (uint32_t)__cvta_generic_to_shared(slot);
-    if constexpr (bytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(p) : "memory");
-    else if constexpr (bytes >= 4) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(p), "n"(bytes) : "memory");
-    else *slot = *reinterpret_cast<const Vec<T, V> *>(p);
+    if constexpr (bytes == 16)
+        asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(to), "l"(p), "l"(policy) : "memory");
+    else if constexpr (bytes >= 4)
+        asm volatile("cp.async.ca.shared.global.L2::cache_hint [%0], [%1], %2, %3;" ::"r"(to), "l"(p), "n"(bytes), "l"(policy) : "memory");
+    else
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(*reinterpret_cast<const uint16_t *>(p)) : "memory");
 }
+
+template <class T, int V>
+__device__ __forceinline__ Vec<T, V> read_slot(uint32_t at)
+{
+    Vec<T, V> r;
+    constexpr int bytes = V * sizeof(T);
+    if constexpr (bytes == 16) {
+        uint4 &v = *reinterpret_cast<uint4 *>(&r);
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    } else if constexpr (bytes == 8) {
+        uint2 &v = *reinterpret_cast<uint2 *>(&r);
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+    } else if constexpr (bytes == 4) {
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(*reinterpret_cast<uint32_t *>(&r)) : "r"(at) : "memory");
+    } else {
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(*reinterpret_cast<uint16_t *>(&r)) : "r"(at) : "memory");
+    }
+    return r;
+}
+
+// L2 policies: what is read once (again), and what the second pass will read.
+__device__ __forceinline__ uint64_t policy_once()
+{
+    uint64_t p;
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ uint64_t policy_again()
+{
+    uint64_t p;
+    asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+
 __device__ __forceinline__ void fetch_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void fetch_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -112,16 +148,6 @@ __device__ __forceinline__ Vec<T, V> pack(const float2 (&f)[(V + 1) / 2])
     }
     return r;
 }
-
-// A thread's way through a map: every ty-th texel of its block's range, forwards or backwards.  Texels
-// advance by whole rows and a remainder; a texel past the end of its row wraps into the next.
-struct Walk {
-    int64_t step, wrap;  // bytes
-    __device__ __forceinline__ Walk(const NtFeatureMap &f, int width, int rows, int rest, int size)
-        : step((rows * f.row_stride + rest * f.texel_stride) * size), wrap((f.row_stride - width * f.texel_stride) * size)
-    {
-    }
-};
 
 // Count, mean and sum of squares about the mean.
 struct Stats {
@@ -204,7 +230,7 @@ __device__ __forceinline__ void join_channel(const NormLaunch &L, int c)
 }
 
 // What a thread's passes share.
-template <class T, int V, bool WHOLE, bool BACKWARD>
+template <class T, int V, bool WHOLE, bool FLAT, bool BACKWARD>
 struct Threads {
     static constexpr int P = (V + 1) / 2;
     static constexpr int NT = BACKWARD ? kBackwardThreads : kForwardThreads;
@@ -213,16 +239,27 @@ struct Threads {
     int lo, row, col, mine;  // first texel of the block; place of the thread; its texels
     const float2 *stat;
     float2 *scratch;
-    Vec<T, V> *kept;
-    int rows, rest;  // ty texels: whole rows of the image, and the rest
+    uint32_t kept;  // shared-memory address of the thread's first slot
 
-    // The x coordinate of texel i of this thread, and where it lies in map f.
-    __device__ __forceinline__ int seek(const NtFeatureMap &f, int i, int c, const char *&at) const
-    {
-        const int t = lo + row + i * L.ty, y = t / L.p.width, x = t - y * L.p.width;
-        at = static_cast<const char *>(f.data) + (n * f.image_stride + y * f.row_stride + x * f.texel_stride + c) * (int64_t)sizeof(T);
-        return x;
-    }
+    // Texel i of this thread in a map, from channel c.
+    struct Path {
+        const Threads &t;
+        const NtFeatureMap &f;
+        char *at;
+        int step;  // bytes
+        __device__ __forceinline__ Path(const Threads &t, const NtFeatureMap &f, int c) : t(t), f(f)
+        {
+            at = static_cast<char *>(f.data) + (t.n * f.image_stride + c) * (int64_t)sizeof(T);
+            if (FLAT) at += (t.lo + t.row) * f.texel_stride * (int64_t)sizeof(T);
+            step = (int)(t.L.ty * f.texel_stride * (int64_t)sizeof(T));
+        }
+        __device__ __forceinline__ char *operator()(int i) const
+        {
+            if (FLAT) return at + (int64_t)i * step;
+            const int k = t.lo + t.row + i * t.L.ty, y = k / t.L.p.width, x = k - y * t.L.p.width;
+            return at + (y * f.row_stride + x * f.texel_stride) * (int64_t)sizeof(T);
+        }
+    };
     // Per-channel values of a parameter, in pairs.
     __device__ __forceinline__ void channels(const float *param, float other, int c, float2 (&v)[P]) const
     {
@@ -233,49 +270,17 @@ struct Threads {
     // Group of channel c + i (of the whole vector, when it lies in one).
     __device__ __forceinline__ int group(int c, int i) const { return (c + (WHOLE || i >= V ? 0 : i)) / L.per; }
 
-    // The slots of this thread: `near` kept vectors, then the ring.  In the backward pass a slot holds x and,
-    // NT vectors on, dy.
-    static constexpr int kMaps = BACKWARD ? 2 : 1;
-    static constexpr int kSlot = NT * kMaps;
+    // The slots of this thread: kept vectors, then a ring of kDepth (a power of two).  In the backward pass a
+    // slot holds x and, kNext bytes on, dy.
+    static constexpr uint32_t kNext = NT * sizeof(Vec<T, V>), kSlot = kNext * (BACKWARD ? 2 : 1);
     static constexpr int kDepth = BACKWARD ? kBackwardRing : kForwardRing;
     struct Source {
-        const Threads &t;
-        const char *x, *dy;
-        int at;  // x coordinate
-        Walk wx, wdy;
-        __device__ __forceinline__ Source(const Threads &t, int i, int c)
-            : t(t), dy(nullptr), wx(t.L.p.x, t.L.p.width, t.rows, t.rest, sizeof(T)),
-              wdy(t.L.p.dy, t.L.p.width, t.rows, t.rest, sizeof(T))
+        Path x, dy;
+        __device__ __forceinline__ Source(const Threads &t, int c) : x(t, t.L.p.x, c), dy(t, t.L.p.dy, c) {}
+        __device__ __forceinline__ void get(uint32_t slot, int i, uint64_t policy) const
         {
-            at = t.seek(t.L.p.x, i, c, x);
-            if (BACKWARD) t.seek(t.L.p.dy, i, c, dy);
-        }
-        __device__ __forceinline__ void get(Vec<T, V> *slot) const
-        {
-            fetch<T, V>(slot, x);
-            if (BACKWARD) fetch<T, V>(slot + NT, dy);
-        }
-        __device__ __forceinline__ void forth()
-        {
-            x += wx.step;
-            if (BACKWARD) dy += wdy.step;
-            at += t.rest;
-            if (at >= t.L.p.width) {
-                at -= t.L.p.width;
-                x += wx.wrap;
-                if (BACKWARD) dy += wdy.wrap;
-            }
-        }
-        __device__ __forceinline__ void back()
-        {
-            x -= wx.step;
-            if (BACKWARD) dy -= wdy.step;
-            at -= t.rest;
-            if (at < 0) {
-                at += t.L.p.width;
-                x -= wx.wrap;
-                if (BACKWARD) dy -= wdy.wrap;
-            }
+            fetch<T, V>(slot, x(i), policy);
+            if (BACKWARD) fetch<T, V>(slot + kNext, dy(i), policy);
         }
     };
 
@@ -284,72 +289,54 @@ struct Threads {
     template <class Use>
     __device__ __forceinline__ void each_forth(int c, int count, int near, int slot0, Use use) const
     {
-        Vec<T, V> *keep = kept + slot0 * kSlot + threadIdx.x, *const ring = kept + L.keep * kSlot + threadIdx.x;
-        Source src(*this, 0, c);
-        for (int i = 0; i < near; ++i, src.forth()) src.get(keep + i * kSlot);
+        const uint32_t keep = kept + slot0 * kSlot, ring = kept + L.keep * kSlot;
+        const Source src(*this, c);
+        const uint64_t once = policy_once(), again = policy_again();
+        for (int i = 0; i < near; ++i) src.get(keep + i * kSlot, i, once);
         fetch_commit();
 #pragma unroll
         for (int u = 0; u < kDepth; ++u) {
-            if (near + u < count) {
-                src.get(ring + u * kSlot);
-                src.forth();
-            }
+            if (near + u < count) src.get(ring + u * kSlot, near + u, again);
             fetch_commit();
         }
         fetch_wait<kDepth>();
 #pragma unroll 2
         for (int i = 0; i < near; ++i) use(keep + i * kSlot);
-        Vec<T, V> *slot = ring;
 #pragma unroll 2
         for (int i = near; i < count; ++i) {
+            const uint32_t slot = ring + ((i - near) & (kDepth - 1)) * kSlot;
             fetch_wait<kDepth - 1>();
             use(slot);
-            // the next texel of this slot, unless this one stays for the second pass
-            if (i + kDepth < count) {
-                src.get(slot);
-                src.forth();
-            }
+            if (i + kDepth < count) src.get(slot, i + kDepth, again);
             fetch_commit();
-            slot = slot == ring + (kDepth - 1) * kSlot ? ring : slot + kSlot;
         }
     }
 
-    // The same from count - 1 down to 0, the ring still as each_forth left it for this column, or `fresh`.
+    // The same from count - 1 down to 0, the ring as each_forth left it for this column, or `fresh`.
     template <class Use>
     __device__ __forceinline__ void each_back(int c, int count, int near, int slot0, bool fresh, Use use) const
     {
-        const Vec<T, V> *keep = kept + slot0 * kSlot + threadIdx.x;
-        Vec<T, V> *const ring = kept + L.keep * kSlot + threadIdx.x, *const last = ring + (kDepth - 1) * kSlot;
+        const uint32_t keep = kept + slot0 * kSlot, ring = kept + L.keep * kSlot;
         if (count > near) {
-            Vec<T, V> *slot = ring + (count - 1 - near) % kDepth * kSlot;
-            const int first = fresh ? count - 1 : count - 1 - kDepth;
-            Source src(*this, max(first, 0), c);
+            const Source src(*this, c);
+            const uint64_t once = policy_once();
 #pragma unroll
             for (int u = 0; u < kDepth; ++u) {
-                if (fresh) {
-                    if (count - 1 - u >= near) {
-                        src.get(slot);
-                        src.back();
-                    }
-                    slot = slot == ring ? last : slot - kSlot;
-                }
+                const int i = count - 1 - u;
+                if (fresh && i >= near) src.get(ring + ((i - near) & (kDepth - 1)) * kSlot, i, once);
                 fetch_commit();
             }
-            slot = ring + (count - 1 - near) % kDepth * kSlot;
 #pragma unroll 2
             for (int i = count - 1; i >= near; --i) {
+                const uint32_t slot = ring + ((i - near) & (kDepth - 1)) * kSlot;
                 fetch_wait<kDepth - 1>();
-                use(slot);
-                if (i - kDepth >= near) {
-                    src.get(slot);
-                    src.back();
-                }
+                use(slot, i);
+                if (i - kDepth >= near) src.get(slot, i - kDepth, once);
                 fetch_commit();
-                slot = slot == ring ? last : slot - kSlot;
             }
         }
 #pragma unroll 2
-        for (int i = near - 1; i >= 0; --i) use(keep + i * kSlot);
+        for (int i = near - 1; i >= 0; --i) use(keep + i * kSlot, i);
     }
 
     // ---- pass 1 ----
@@ -357,9 +344,9 @@ struct Threads {
     {
         float2 pivot[P] = {}, s1[P] = {}, s2[P] = {};
         bool begun = false;
-        each_forth(c, count, near, slot0, [&](const Vec<T, V> *slot) {
+        each_forth(c, count, near, slot0, [&](uint32_t slot) {
             float2 f[P];
-            unpack<T, V>(*slot, f);
+            unpack<T, V>(read_slot<T, V>(slot), f);
             if (!begun) {
                 begun = true;
 #pragma unroll
@@ -413,10 +400,10 @@ struct Threads {
         statistics(c, shift, rstd);
         channels(L.p.gamma, 1.f, c, gamma);
         channels(L.p.beta, 0.f, c, beta);
-        each_forth(c, count, near, slot0, [&](const Vec<T, V> *slot) {
+        each_forth(c, count, near, slot0, [&](uint32_t slot) {
             float2 fa[P], fb[P];
-            unpack<T, V>(slot[0], fa);
-            unpack<T, V>(slot[NT], fb);
+            unpack<T, V>(read_slot<T, V>(slot), fa);
+            unpack<T, V>(read_slot<T, V>(slot + kNext), fb);
 #pragma unroll
             for (int j = 0; j < P; ++j) {
                 float2 h, e;
@@ -432,31 +419,6 @@ struct Threads {
     }
 
     // ---- pass 2, the texels read last first ----
-    // A result's way through its map, backwards.
-    struct Sink {
-        const Threads &t;
-        char *out;
-        int at;
-        Walk w;
-        __device__ __forceinline__ Sink(const Threads &t, const NtFeatureMap &f, int i, int c)
-            : t(t), w(f, t.L.p.width, t.rows, t.rest, sizeof(T))
-        {
-            const char *p;
-            at = t.seek(f, i, c, p);
-            out = const_cast<char *>(p);
-        }
-        __device__ __forceinline__ void put(const Vec<T, V> &v)
-        {
-            store_vec<T, V>(reinterpret_cast<T *>(out), v);
-            out -= w.step;
-            at -= t.rest;
-            if (at < 0) {
-                at += t.L.p.width;
-                out -= w.wrap;
-            }
-        }
-    };
-
     template <int ACT>
     __device__ __forceinline__ void forward_apply(int c, int count, int near, int slot0, bool fresh) const
     {
@@ -469,14 +431,14 @@ struct Threads {
             shift[j] = make_float2(-a.x, -b.x);
             scale[j] = __fmul2_rn(scale[j], make_float2(a.y, b.y));
         }
-        Sink sink(*this, L.p.y, count - 1, c);
-        each_back(c, count, near, slot0, fresh, [&](const Vec<T, V> *slot) {
+        const Path out(*this, L.p.y, c);
+        each_back(c, count, near, slot0, fresh, [&](uint32_t slot, int i) {
             float2 f[P];
-            unpack<T, V>(*slot, f);
+            unpack<T, V>(read_slot<T, V>(slot), f);
 #pragma unroll
             for (int j = 0; j < P; ++j)
                 f[j] = activate2<ACT>(__ffma2_rn(__fadd2_rn(f[j], shift[WHOLE ? 0 : j]), scale[j], beta[j]));
-            sink.put(norm::pack<T, V>(f));
+            store_vec<T, V>(reinterpret_cast<T *>(out(i)), norm::pack<T, V>(f));
         });
     }
 
@@ -494,11 +456,11 @@ struct Threads {
             k1[j] = make_float2(-a.x * L.inv_count, -b.x * L.inv_count);
             k2[j] = make_float2(-a.y * L.inv_count, -b.y * L.inv_count);
         }
-        Sink sink(*this, L.p.dx, count - 1, c);
-        each_back(c, count, near, slot0, fresh, [&](const Vec<T, V> *slot) {
+        const Path out(*this, L.p.dx, c);
+        each_back(c, count, near, slot0, fresh, [&](uint32_t slot, int i) {
             float2 fa[P], fb[P];
-            unpack<T, V>(slot[0], fa);
-            unpack<T, V>(slot[NT], fb);
+            unpack<T, V>(read_slot<T, V>(slot), fa);
+            unpack<T, V>(read_slot<T, V>(slot + kNext), fb);
 #pragma unroll
             for (int j = 0; j < P; ++j) {
                 const int s = WHOLE ? 0 : j;
@@ -506,7 +468,7 @@ struct Threads {
                 terms<ACT>(fa[j], fb[j], shift[s], rstd[s], gamma[j], beta[j], h, e);
                 fa[j] = __fmul2_rn(rstd[s], __ffma2_rn(gamma[j], e, __ffma2_rn(h, k2[s], k1[s])));
             }
-            sink.put(norm::pack<T, V>(fa));
+            store_vec<T, V>(reinterpret_cast<T *>(out(i)), norm::pack<T, V>(fa));
         });
     }
 
@@ -524,8 +486,8 @@ struct Threads {
     }
 };
 
-// WHOLE: a vector lies in one group.
-template <class T, int V, bool WHOLE, bool BACKWARD>
+// WHOLE: a vector lies in one group.  FLAT: the texels of every map are evenly spaced.
+template <class T, int V, bool WHOLE, bool FLAT, bool BACKWARD>
 __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads), WHOLE ? 2 : 1)
     norm_kernel(const __grid_constant__ NormLaunch L, unsigned int *status)
 {
@@ -541,9 +503,9 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
     const int row = tid / L.tx, col = tid % L.tx;
     const int mine = row < L.ty && lo + row < hi ? (hi - lo - row + L.ty - 1) / L.ty : 0;  // texels of this thread
     const int most = (hi - lo + L.ty - 1) / L.ty;                                        // and of any
-    const Threads<T, V, WHOLE, BACKWARD> th = {L,    n,       lo, row, col, mine,
-                                               stat, scratch, reinterpret_cast<Vec<T, V> *>(smem + L.scratch),
-                                               L.ty / p.width, L.ty % p.width};
+    const Threads<T, V, WHOLE, FLAT, BACKWARD> th = {L,    n,       lo, row, col, mine,
+                                               stat, scratch,
+                                               (uint32_t)__cvta_generic_to_shared(smem + L.scratch) + tid * (uint32_t)sizeof(Vec<T, V>)};
     int slot0 = 0;
     for (int v0 = 0; v0 < L.vectors; v0 += L.tx, slot0 += most) {
         const int vec = v0 + col;
@@ -662,30 +624,33 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
 using NormKernel = void (*)(NormLaunch, unsigned int *);
 
 template <class T, int V, bool BACKWARD>
-NormKernel pick_whole(bool whole)
+NormKernel pick_whole(bool whole, bool flat)
 {
-    if constexpr (V == 1) return norm_kernel<T, 1, true, BACKWARD>;
-    else return whole ? (NormKernel)norm_kernel<T, V, true, BACKWARD> : (NormKernel)norm_kernel<T, V, false, BACKWARD>;
+    if constexpr (V > 1)
+        if (!whole) return flat ? norm_kernel<T, V, false, true, BACKWARD> : norm_kernel<T, V, false, false, BACKWARD>;
+    return flat ? norm_kernel<T, V, true, true, BACKWARD> : norm_kernel<T, V, true, false, BACKWARD>;
 }
 
 template <class T, bool BACKWARD>
-NormKernel pick_width(int v, bool whole)
+NormKernel pick_width(int v, bool whole, bool flat)
 {
     if constexpr (sizeof(T) == 2)
-        if (v == 8) return pick_whole<T, 8, BACKWARD>(whole);
-    return v == 4 ? pick_whole<T, 4, BACKWARD>(whole) : v == 2 ? pick_whole<T, 2, BACKWARD>(whole) : pick_whole<T, 1, BACKWARD>(true);
+        if (v == 8) return pick_whole<T, 8, BACKWARD>(whole, flat);
+    return v == 4   ? pick_whole<T, 4, BACKWARD>(whole, flat)
+           : v == 2 ? pick_whole<T, 2, BACKWARD>(whole, flat)
+                    : pick_whole<T, 1, BACKWARD>(whole, flat);
 }
 
 template <bool BACKWARD>
-NormKernel pick_kernel(int32_t dtype, int v, bool whole)
+NormKernel pick_kernel(int32_t dtype, int v, bool whole, bool flat)
 {
-    return dtype == NT_DTYPE_F16    ? pick_width<__half, BACKWARD>(v, whole)
-           : dtype == NT_DTYPE_BF16 ? pick_width<__nv_bfloat16, BACKWARD>(v, whole)
-                                    : pick_width<float, BACKWARD>(v, whole);
+    return dtype == NT_DTYPE_F16    ? pick_width<__half, BACKWARD>(v, whole, flat)
+           : dtype == NT_DTYPE_BF16 ? pick_width<__nv_bfloat16, BACKWARD>(v, whole, flat)
+                                    : pick_width<float, BACKWARD>(v, whole, flat);
 }
 
-NormKernel forward_kernel(int32_t dtype, int v, bool whole);
-NormKernel backward_kernel(int32_t dtype, int v, bool whole);
+NormKernel forward_kernel(int32_t dtype, int v, bool whole, bool flat);
+NormKernel backward_kernel(int32_t dtype, int v, bool whole, bool flat);
 
 }  // namespace norm
 }  // namespace nt

@@ -3,6 +3,6 @@
 
 namespace nt {
 namespace norm {
-NormKernel forward_kernel(int32_t dtype, int v, bool whole) { return pick_kernel<false>(dtype, v, whole); }
+NormKernel forward_kernel(int32_t dtype, int v, bool whole, bool flat) { return pick_kernel<false>(dtype, v, whole, flat); }
 }  // namespace norm
 }  // namespace nt
