@@ -7,8 +7,6 @@
 namespace nt {
 namespace norm {
 
-__device__ unsigned int g_norm_status;  // bit 0: the wait at the grid's barrier gave up
-
 constexpr int kJoinWarps = 8;
 
 __global__ void __launch_bounds__(32 * kJoinWarps) join_channels_kernel(const NormLaunch L)
@@ -36,7 +34,7 @@ Plan plan(const NtGroupNorm *p)
     // at least 4 vectors of 8 channels for each of 512 threads
     const int64_t wanted = std::max<int64_t>(1, values / (512 * 32));
     const int64_t most = std::max<int64_t>(1, resident / p->images);
-    const int64_t splits = std::min({wanted, most, (int64_t)p->height * p->width});
+    const int64_t splits = std::min({wanted, most, (int64_t)p->height * p->width, (int64_t)kMaxSplits});
     if (splits <= 2 * kMaxCluster) return {(int)std::min<int64_t>(splits, kMaxCluster), true, per_sm};
     return {(int)splits, false, per_sm};
 }
@@ -118,9 +116,7 @@ cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
     }
 
     const NormKernel kernel = backward ? backward_kernel(p->dtype, v, whole, even) : forward_kernel(p->dtype, v, whole, even);
-    unsigned int *status = nullptr;
-    cudaError_t e = cudaGetSymbolAddress(reinterpret_cast<void **>(&status), g_norm_status);
-    if (e == cudaSuccess) e = set_smem_limit(reinterpret_cast<const void *>(kernel), 227 * 1024 - 1024);
+    cudaError_t e = set_smem_limit(reinterpret_cast<const void *>(kernel), 227 * 1024 - 1024);
     if (e != cudaSuccess) return e;
     if (!pl.cluster && (e = cudaMemsetAsync(ws, 0, 16, st)) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
@@ -138,11 +134,11 @@ cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
         attr[0].val.cooperative = 1;
     }
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, L, status);
+    cfg.numAttrs = pl.cluster && pl.splits == 1 ? 0 : 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, L);
     if (e != cudaSuccess) return e;
     count_launch();
-    if (backward && pl.cluster && (p->dgamma || p->dbeta)) {
+    if (backward && pl.cluster && p->images > 1 && (p->dgamma || p->dbeta)) {
         join_channels_kernel<<<(unsigned)ceil_div(p->channels, kJoinWarps), 32 * kJoinWarps, 0, st>>>(L);
         count_launch();
     }
@@ -224,10 +220,11 @@ nt_status run(const NtGroupNorm *p, bool backward, nt_stream_t stream)
 
 cudaError_t read_norm_status(uint32_t *status, bool clear)
 {
-    cudaError_t e = cudaMemcpyFromSymbol(status, norm::g_norm_status, sizeof(uint32_t));
-    if (e != cudaSuccess || !clear) return e;
-    const uint32_t zero = 0;
-    return cudaMemcpyToSymbol(norm::g_norm_status, &zero, sizeof(uint32_t));
+    uint32_t a = 0, b = 0;
+    cudaError_t e = norm::read_forward_status(&a, clear);
+    if (e == cudaSuccess) e = norm::read_backward_status(&b, clear);
+    *status = a | b;
+    return e;
 }
 
 }  // namespace nt

@@ -26,7 +26,10 @@ constexpr int kForwardThreads = 512;
 constexpr int kForwardRing = 4, kBackwardRing = 4;  // 64 and 96 KB in flight on an SM cover the latency of HBM
 constexpr int kBackwardThreads = 384;  // 84 registers a thread with two blocks on an SM: 64 spill
 constexpr int kMaxCluster = 8;
+constexpr int kMaxSplits = 320;  // thread blocks of an image
 constexpr uint32_t kSpinLimit = 1u << 24;
+
+static __device__ unsigned int g_norm_status;  // bit 0: the wait at the grid's barrier gave up
 
 struct NormLaunch {
     NtGroupNorm p;
@@ -149,25 +152,10 @@ __device__ __forceinline__ Vec<T, V> pack(const float2 (&f)[(V + 1) / 2])
     return r;
 }
 
-// Count, mean and sum of squares about the mean.
-struct Stats {
-    float count, mean, m2;
-};
-
-__device__ __forceinline__ Stats join(const Stats &a, const Stats &b)
-{
-    if (b.count == 0.f) return a;
-    if (a.count == 0.f) return b;
-    const float n = a.count + b.count, d = b.mean - a.mean, w = __fdividef(b.count, n);
-    return {n, fmaf(d, w, a.mean), a.m2 + b.m2 + d * d * a.count * w};
-}
-
-__device__ __forceinline__ Stats warp_join(Stats s)
+__device__ __forceinline__ float warp_sum_all(float s)
 {
 #pragma unroll
-    for (int w = 16; w > 0; w >>= 1)
-        s = join(s, {__shfl_down_sync(0xffffffffu, s.count, w), __shfl_down_sync(0xffffffffu, s.mean, w),
-                     __shfl_down_sync(0xffffffffu, s.m2, w)});
+    for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
     return s;
 }
 
@@ -359,18 +347,22 @@ struct Threads {
                 s2[j] = __ffma2_rn(d, d, s2[j]);
             }
         });
-        // (mean, centred squares) of the vector, or of each channel
+        // (mean, centred squares) of each channel, or of the vector about the mean of its channels
         const float inv = count > 0 ? __fdividef(1.f, (float)count) : 0.f;
-        Stats all = {0.f, 0.f, 0.f};
+        float mean[V], m2[V], shift = 0.f, sum = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const float a = j & 1 ? s1[j / 2].y : s1[j / 2].x, b = j & 1 ? s2[j / 2].y : s2[j / 2].x;
-            const float k = -(j & 1 ? pivot[j / 2].y : pivot[j / 2].x);
-            const Stats one = {(float)count, fmaf(a, inv, k), fmaxf(b - a * a * inv, 0.f)};
-            if (WHOLE) all = join(all, one);
-            else scratch[row * L.p.channels + c + j] = make_float2(one.mean, one.m2);
+            mean[j] = fmaf(a, inv, -(j & 1 ? pivot[j / 2].y : pivot[j / 2].x));
+            m2[j] = fmaxf(b - a * a * inv, 0.f);
+            if (!WHOLE) scratch[row * L.p.channels + c + j] = make_float2(mean[j], m2[j]);
+            shift += mean[j] - mean[0];
         }
-        if (WHOLE) scratch[row * L.vectors + c / V] = make_float2(all.mean, all.m2);
+        if (!WHOLE) return;
+        const float all = fmaf(shift, 1.f / V, mean[0]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum += fmaf((float)count * (mean[j] - all), mean[j] - all, m2[j]);
+        scratch[row * L.vectors + c / V] = make_float2(all, sum);
     }
 
     // Terms of the backward pass: h and e = dy act'(z).
@@ -489,7 +481,7 @@ struct Threads {
 // WHOLE: a vector lies in one group.  FLAT: the texels of every map are evenly spaced.
 template <class T, int V, bool WHOLE, bool FLAT, bool BACKWARD>
 __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads), WHOLE ? 2 : 1)
-    norm_kernel(const __grid_constant__ NormLaunch L, unsigned int *status)
+    norm_kernel(const __grid_constant__ NormLaunch L)
 {
     constexpr int NT = BACKWARD ? kBackwardThreads : kForwardThreads, kWarps = NT / 32;
     extern __shared__ __align__(16) uint8_t smem[];
@@ -497,12 +489,15 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t n = blockIdx.x / L.splits;
     const int split = blockIdx.x % L.splits;
-    const int lo = (int)((int64_t)L.texels * split / L.splits), hi = (int)((int64_t)L.texels * (split + 1) / L.splits);
+    // texels of a block: an equal share, the first blocks one more
+    const int share = L.texels / L.splits, extra = L.texels - share * L.splits;
+    const int lo = split * share + min(split, extra), hi = lo + share + (split < extra);
     // shared memory: group results [groups], group partials [groups], scratch, kept vectors
     float2 *stat = reinterpret_cast<float2 *>(smem), *part = stat + p.groups, *scratch = part + p.groups;
     const int row = tid / L.tx, col = tid % L.tx;
-    const int mine = row < L.ty && lo + row < hi ? (hi - lo - row + L.ty - 1) / L.ty : 0;  // texels of this thread
-    const int most = (hi - lo + L.ty - 1) / L.ty;                                        // and of any
+    const int turn = (hi - lo) / L.ty, left = hi - lo - turn * L.ty;
+    const int mine = row < L.ty ? turn + (row < left) : 0;  // texels of this thread
+    const int most = turn + (left > 0);                     // and of any
     const Threads<T, V, WHOLE, FLAT, BACKWARD> th = {L,    n,       lo, row, col, mine,
                                                stat, scratch,
                                                (uint32_t)__cvta_generic_to_shared(smem + L.scratch) + tid * (uint32_t)sizeof(Vec<T, V>)};
@@ -526,17 +521,24 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
     if constexpr (!BACKWARD) {
         const int step = WHOLE ? V : 1, entries = L.per / step, width = p.channels / step;
         for (int g = warp; g < p.groups; g += kWarps) {
-            Stats s = {0.f, 0.f, 0.f};
+            // two passes over the group's entries: the mean, from differences to one of them; the squares about it
+            const float2 *const of = scratch + g * entries;
+            const float origin = of[0].x;
+            float shift = 0.f, sum = 0.f;
             for (int e = lane; e < L.ty * entries; e += 32) {
-                const int r = e / entries;
-                const float2 v = scratch[r * width + g * entries + e - r * entries];
-                const int texels = lo + r < hi ? (hi - lo - r + L.ty - 1) / L.ty : 0;
-                s = join(s, {(float)texels * step, v.x, v.y});
+                const int r = entries == 1 ? e : e / entries;
+                shift = fmaf((float)(turn + (r < left)) * step, of[r * (width - entries) + e].x - origin, shift);
             }
-            s = warp_join(s);
+            const float mean = origin + warp_sum_all(shift) / ((float)(hi - lo) * L.per);
+            for (int e = lane; e < L.ty * entries; e += 32) {
+                const int r = entries == 1 ? e : e / entries;
+                const float2 v = of[r * (width - entries) + e];
+                sum += fmaf((float)(turn + (r < left)) * step * (v.x - mean), v.x - mean, v.y);
+            }
+            sum = warp_sum_all(sum);
             if (lane == 0) {
-                if (shared_out) shared_out[g] = make_float2(s.mean, s.m2);
-                else L.groups_part[(n * p.groups + g) * L.splits + split] = make_float2(s.mean, s.m2);
+                if (shared_out) shared_out[g] = make_float2(mean, sum);
+                else L.groups_part[(n * p.groups + g) * L.splits + split] = make_float2(mean, sum);
             }
         }
     } else {
@@ -550,7 +552,7 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
             }
             __syncthreads();
         }
-        if (p.dgamma || p.dbeta)
+        if ((p.dgamma || p.dbeta) && (p.images > 1 || !L.cluster))
             for (int c = tid; c < p.channels; c += NT) L.channels_part[(int64_t)c * parts + blockIdx.x] = scratch[c];
         for (int g = warp; g < p.groups; g += kWarps) {
             float2 s = make_float2(0.f, 0.f);
@@ -567,40 +569,63 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
             }
         }
     }
-    if (!L.cluster) grid_sync(L.barrier, status);
+    if (!L.cluster) grid_sync(L.barrier, &g_norm_status);
     else if (L.splits > 1) cluster_sync();
     else __syncthreads();
 
     // ---- the image's sums ----
     for (int g = warp; g < p.groups; g += kWarps) {
-        Stats s = {0.f, 0.f, 0.f};
-        float2 sum = make_float2(0.f, 0.f);
-        for (int i = lane; i < L.splits; i += 32) {
-            const float2 v = L.cluster ? (L.splits > 1 ? peer_f2(part + g, i) : part[g])
-                                       : __ldcg(L.groups_part + (n * p.groups + g) * L.splits + i);
-            if (BACKWARD) {
-                sum.x += v.x;
-                sum.y += v.y;
-            } else {
-                const int64_t texels = (int64_t)L.texels * (i + 1) / L.splits - (int64_t)L.texels * i / L.splits;
-                s = join(s, {(float)texels * L.per, v.x, v.y});
-            }
+        float2 v[kMaxSplits / 32];
+#pragma unroll
+        for (int k = 0; k < kMaxSplits / 32; ++k) {
+            const int i = lane + 32 * k;
+            v[k] = make_float2(0.f, 0.f);
+            if (i < L.splits)
+                v[k] = L.cluster ? (L.splits > 1 ? peer_f2(part + g, i) : part[g])
+                                 : __ldcg(L.groups_part + (n * p.groups + g) * L.splits + i);
         }
+        float a = 0.f, b = 0.f;
         if (BACKWARD) {
-            sum = warp_sum(sum);
-            if (lane == 0) stat[g] = sum;
+#pragma unroll
+            for (int k = 0; k < kMaxSplits / 32; ++k) a += v[k].x, b += v[k].y;
+            a = warp_sum_all(a);
+            b = warp_sum_all(b);
+            if (lane == 0) stat[g] = make_float2(a, b);
         } else {
-            s = warp_join(s);
+            const float origin = __shfl_sync(0xffffffffu, v[0].x, 0);
+#pragma unroll
+            for (int k = 0; k < kMaxSplits / 32; ++k)
+                if (lane + 32 * k < L.splits) a = fmaf((float)(share + (lane + 32 * k < extra)), v[k].x - origin, a);
+            const float mean = origin + warp_sum_all(a) / (float)L.texels;
+#pragma unroll
+            for (int k = 0; k < kMaxSplits / 32; ++k)
+                if (lane + 32 * k < L.splits)
+                    b += fmaf((float)(share + (lane + 32 * k < extra)) * L.per * (v[k].x - mean), v[k].x - mean, v[k].y);
+            b = warp_sum_all(b);
             if (lane == 0) {
-                const float rstd = 1.f / sqrtf(s.m2 * L.inv_count + p.epsilon);
-                stat[g] = make_float2(s.mean, rstd);
+                const float rstd = 1.f / sqrtf(b * L.inv_count + p.epsilon);
+                stat[g] = make_float2(mean, rstd);
                 if (split == 0) {
-                    if (p.mean) p.mean[n * p.groups + g] = s.mean;
+                    if (p.mean) p.mean[n * p.groups + g] = mean;
                     if (p.rstd) p.rstd[n * p.groups + g] = rstd;
                 }
             }
         }
     }
+    if (BACKWARD && L.cluster && p.images == 1 && (p.dgamma || p.dbeta))
+        for (int c = split * NT + tid; c < p.channels; c += L.splits * NT) {
+            float2 s = scratch[c];
+            if (L.splits > 1) {
+                s = make_float2(0.f, 0.f);
+                for (int i = 0; i < L.splits; ++i) {
+                    const float2 v = peer_f2(scratch + c, i);
+                    s.x += v.x;
+                    s.y += v.y;
+                }
+            }
+            if (p.dbeta) p.dbeta[c] = s.x;
+            if (p.dgamma) p.dgamma[c] = s.y;
+        }
     if (L.cluster && L.splits > 1) cluster_sync();  // a block's sums stay until its peers have read them
     else __syncthreads();
     if (BACKWARD && !L.cluster && (p.dgamma || p.dbeta))
@@ -621,7 +646,7 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
     }
 }
 
-using NormKernel = void (*)(NormLaunch, unsigned int *);
+using NormKernel = void (*)(NormLaunch);
 
 template <class T, int V, bool BACKWARD>
 NormKernel pick_whole(bool whole, bool flat)
@@ -651,6 +676,17 @@ NormKernel pick_kernel(int32_t dtype, int v, bool whole, bool flat)
 
 NormKernel forward_kernel(int32_t dtype, int v, bool whole, bool flat);
 NormKernel backward_kernel(int32_t dtype, int v, bool whole, bool flat);
+
+// This file's status word, read and cleared on request.
+static inline cudaError_t read_status(uint32_t *status, bool clear)
+{
+    cudaError_t e = cudaMemcpyFromSymbol(status, g_norm_status, sizeof(uint32_t));
+    if (e != cudaSuccess || !clear) return e;
+    const uint32_t zero = 0;
+    return cudaMemcpyToSymbol(g_norm_status, &zero, sizeof(uint32_t));
+}
+cudaError_t read_forward_status(uint32_t *status, bool clear);
+cudaError_t read_backward_status(uint32_t *status, bool clear);
 
 }  // namespace norm
 }  // namespace nt

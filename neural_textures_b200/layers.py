@@ -9,6 +9,7 @@ current stream of the tensors' device) and returns without waiting.  Results are
 """
 from __future__ import annotations
 
+import ctypes as C
 import struct
 
 from . import _native as N
@@ -44,19 +45,30 @@ def _activation(name: str) -> int:
     return a
 
 
-def _same_device(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not on {device}")
-
-
-def _vector(t, n: int, name: str) -> int | None:
-    """Data pointer of an optional contiguous fp32 vector of n elements."""
+def _vector(t, n: int, device, name: str) -> int:
+    """Data pointer of an optional contiguous fp32 vector of n elements, 0 for None."""
     if t is None:
-        return None
+        return 0
     if t.dtype is not _torch.float32 or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous float32 tensor of {n} elements")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
     return t.data_ptr()
+
+
+_shapes = {}
+
+
+def _new(shape, dtype, device):
+    """torch.empty(shape), at less than half its host time: empty_like of a one-element tensor
+    expanded to the shape, kept per shape."""
+    key = (shape, dtype, device)
+    t = _shapes.get(key)
+    if t is None:
+        if len(_shapes) > 4096:
+            _shapes.clear()
+        t = _shapes[key] = _torch.empty(1, dtype=dtype, device=device).expand(shape)
+    return _torch.empty_like(t)
 
 
 def _launch(device, stream, made, fn, *args):
@@ -86,41 +98,49 @@ def _launch(device, stream, made, fn, *args):
 # group normalisation
 
 _GROUP_NORM = struct.Struct("@7if" + "P3q" + "4P" + "P3q" * 3 + "3Pq")
-_NO_MAP = (0, 0, 0, 0)
-_workspace_sizes = {}
+_workspaces = {}
 
 
 def _map(t, shape, dtype, device, name: str):
     """(pointer, strides) of a channels-last map [N][H][W][C] or [H][W][C]."""
     if t.shape != shape or t.dtype is not dtype or t.device != device:
         raise ValueError(f"{name} must be {tuple(shape)} of {dtype} on {device}, not {tuple(t.shape)} of {t.dtype} on {t.device}")
+    return _strides(t, name)
+
+
+def _strides(t, name: str):
     s = t.stride()
-    if s[-1] != 1 and shape[-1] > 1:
+    if s[-1] != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name}: the channels must be contiguous (stride 1, not {s[-1]})")
     return (t.data_ptr(), s[0], s[1], s[2]) if len(s) == 4 else (t.data_ptr(), 0, s[0], s[1])
 
 
 def _norm_sizes(x, groups: int):
-    if x.dim() not in (3, 4):
-        raise ValueError(f"x must be [N][H][W][C] or [H][W][C], not {tuple(x.shape)}")
-    n, h, w, c = x.shape if x.dim() == 4 else (1, *x.shape)
-    return n, h, w, c, int(groups)
+    shape = x.shape
+    if len(shape) == 4:
+        return (*shape, int(groups))
+    if len(shape) != 3:
+        raise ValueError(f"x must be [N][H][W][C] or [H][W][C], not {tuple(shape)}")
+    return (1, *shape, int(groups))
 
 
-def _norm_call(entry, sizes, dtype: int, act: int, eps: float, x, gamma, beta, mean, rstd, y, dy, dx, dgamma, dbeta,
-               device, stream, made):
-    L = load()
-    backward = int(entry == "nt_group_norm_backward")
-    key = (sizes, dtype, backward)
-    need = _workspace_sizes.get(key)
-    pack = lambda ws, size: _GROUP_NORM.pack(*sizes, dtype, act, eps, *x, gamma or 0, beta or 0, mean, rstd, *y, *dy, *dx,
-                                             dgamma, dbeta, ws, size)
+def _norm_workspace(L, sizes, dtype: int, device, backward: int):
+    """(tensor or None, pointer, bytes) of the call's workspace."""
+    key = (sizes, dtype, backward, device)
+    need = _workspaces.get(key)
     if need is None:
-        if len(_workspace_sizes) > 4096:
-            _workspace_sizes.clear()
-        need = _workspace_sizes[key] = int(L.nt_group_norm_workspace_bytes(pack(0, 0), backward))
-    ws = _torch.empty(need, dtype=_torch.uint8, device=device) if need else None
-    _launch(device, stream, (ws, *made), getattr(L, entry), pack(ws.data_ptr() if need else 0, need))
+        if len(_workspaces) > 4096:
+            _workspaces.clear()
+        p = N.NtGroupNorm(*sizes, dtype, 0, 1.0)
+        if device.type == "cuda":
+            with _torch.cuda.device(device):
+                need = _workspaces[key] = int(L.nt_group_norm_workspace_bytes(C.byref(p), backward))
+        else:
+            need = 0
+    if not need:
+        return None, 0, 0
+    ws = _new((need,), _torch.uint8, device)
+    return ws, ws.data_ptr(), need
 
 
 def group_norm(x, groups: int, gamma=None, beta=None, activation: str = "none", eps: float = 1e-5, out=None, stream=None):
@@ -130,17 +150,22 @@ def group_norm(x, groups: int, gamma=None, beta=None, activation: str = "none", 
     (y, mean, rstd) with float32 statistics [N][groups], which group_norm_backward takes.  `out`
     receives y and may be x."""
     torch = _torch or _lazy_torch()
-    sizes, dtype = _norm_sizes(x, groups), _dtype(x, "x")
-    device, shape = x.device, x.shape
-    _same_device(device, gamma=gamma, beta=beta)
-    y = torch.empty(shape, dtype=x.dtype, device=device) if out is None else out
-    stats = torch.empty((2, sizes[0], max(sizes[4], 0)), dtype=torch.float32, device=device)
-    mean, rstd = stats[0], stats[1]
-    c = sizes[3]
-    _norm_call("nt_group_norm_forward", sizes, dtype, _activation(activation), eps,
-               _map(x, shape, x.dtype, device, "x"), _vector(gamma, c, "gamma"), _vector(beta, c, "beta"),
-               mean.data_ptr(), rstd.data_ptr(), _map(y, shape, x.dtype, device, "out"), _NO_MAP, _NO_MAP, 0, 0,
-               device, stream, (y if out is None else None, stats))
+    sizes, kind, device = _norm_sizes(x, groups), x.dtype, x.device
+    n, h, w, c, g = sizes
+    dtype, act, L = _dtype(x, "x"), _activation(activation), load()
+    xp, x0, x1, x2 = _strides(x, "x")
+    ga, be = _vector(gamma, c, device, "gamma"), _vector(beta, c, device, "beta")
+    if out is not None:
+        y = out
+        yp, y0, y1, y2 = _map(y, x.shape, kind, device, "out")
+    else:
+        y = torch.empty_like(x) if x.is_contiguous() else _new(x.shape, kind, device)
+        yp, y0, y1, y2 = _strides(y, "y")
+    mean, rstd = _new((n, max(g, 0)), torch.float32, device), _new((n, max(g, 0)), torch.float32, device)
+    ws, wp, size = _norm_workspace(L, sizes, dtype, device, 0)
+    _launch(device, stream, (None if out is not None else y, mean, rstd, ws), L.nt_group_norm_forward,
+            _GROUP_NORM.pack(n, h, w, c, g, dtype, act, eps, xp, x0, x1, x2, ga, be, mean.data_ptr(), rstd.data_ptr(),
+                             yp, y0, y1, y2, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, wp, size))
     return y, mean, rstd
 
 
@@ -149,18 +174,24 @@ def group_norm_backward(dy, x, mean, rstd, groups: int, gamma=None, beta=None, a
     dbeta).  dx has x's type; dgamma and dbeta are float32 [C], summed over images and texels.
     `out` receives dx and may be dy or x."""
     torch = _torch or _lazy_torch()
-    sizes, dtype = _norm_sizes(x, groups), _dtype(x, "x")
-    device, shape, c = x.device, x.shape, sizes[3]
-    _same_device(device, gamma=gamma, beta=beta, mean=mean, rstd=rstd)
-    dx = torch.empty(shape, dtype=x.dtype, device=device) if out is None else out
-    grads = torch.empty((2, c), dtype=torch.float32, device=device)
-    dgamma, dbeta = grads[0], grads[1]
-    stat = sizes[0] * sizes[4]
-    _norm_call("nt_group_norm_backward", sizes, dtype, _activation(activation), 1.0,
-               _map(x, shape, x.dtype, device, "x"), _vector(gamma, c, "gamma"), _vector(beta, c, "beta"),
-               _vector(mean, stat, "mean"), _vector(rstd, stat, "rstd"), _NO_MAP, _map(dy, shape, x.dtype, device, "dy"),
-               _map(dx, shape, x.dtype, device, "out"), dgamma.data_ptr(), dbeta.data_ptr(), device, stream,
-               (dx if out is None else None, grads))
+    sizes, kind, device = _norm_sizes(x, groups), x.dtype, x.device
+    n, h, w, c, g = sizes
+    dtype, act, L = _dtype(x, "x"), _activation(activation), load()
+    xp, x0, x1, x2 = _strides(x, "x")
+    gp, g0, g1, g2 = _map(dy, x.shape, kind, device, "dy")
+    ga, be = _vector(gamma, c, device, "gamma"), _vector(beta, c, device, "beta")
+    mp, rp = _vector(mean, n * g, device, "mean"), _vector(rstd, n * g, device, "rstd")
+    if out is not None:
+        dx = out
+        dp, d0, d1, d2 = _map(dx, x.shape, kind, device, "out")
+    else:
+        dx = torch.empty_like(x) if x.is_contiguous() else _new(x.shape, kind, device)
+        dp, d0, d1, d2 = _strides(dx, "dx")
+    dgamma, dbeta = _new((c,), torch.float32, device), _new((c,), torch.float32, device)
+    ws, wp, size = _norm_workspace(L, sizes, dtype, device, 1)
+    _launch(device, stream, (None if out is not None else dx, dgamma, dbeta, ws), L.nt_group_norm_backward,
+            _GROUP_NORM.pack(n, h, w, c, g, dtype, act, 1.0, xp, x0, x1, x2, ga, be, mp, rp, 0, 0, 0, 0, gp, g0, g1, g2,
+                             dp, d0, d1, d2, dgamma.data_ptr(), dbeta.data_ptr(), wp, size))
     return dx, dgamma, dbeta
 
 
@@ -178,30 +209,37 @@ class Mx4Tensor:
 
     def __init__(self, data, scales, rows: int, cols: int, block: int = 32):
         torch = _torch or _lazy_torch()
-        L = load()
         if block not in (16, 32):
             raise ValueError(f"block must be 16 or 32, not {block}")
         if rows < 0 or cols < 1:
             raise ValueError(f"{rows} x {cols} is not a matrix size")
-        if data.dtype is not torch.uint8 or data.dim() != 2 or data.shape[0] < rows or data.shape[1] < -(-cols // 32) * 16:
-            raise ValueError(f"data must be uint8 [{rows}][{-(-cols // 32) * 16}] or larger")
-        if data.shape[1] > 1 and data.stride(1) != 1:
+        pitch, size = -(-cols // 32) * 16, -(-rows // 128) * -(-cols // (4 * block)) * 512
+        shape = data.shape
+        if data.dtype is not torch.uint8 or len(shape) != 2 or shape[0] < rows or shape[1] < pitch:
+            raise ValueError(f"data must be uint8 [{rows}][{pitch}] or larger")
+        step, one = data.stride()
+        if one != 1:
             raise ValueError("data: the codes of a row must be contiguous")
-        if scales.dtype is not torch.uint8 or not scales.is_contiguous() or scales.numel() < -(-rows // 128) * -(-cols // (4 * block)) * 512:
-            raise ValueError(f"scales must be contiguous uint8 of {L.nt_mx4_scales_bytes(rows, cols, block)} bytes")
-        _same_device(data.device, scales=scales)
-        self.data, self.scales, self.rows, self.cols, self.block = data, scales, int(rows), int(cols), int(block)
-        self._packed = _MATRIX.pack(data.data_ptr(), scales.data_ptr(), data.stride(0) if rows > 1 else data.shape[1] // 16 * 16,
-                                    self.rows, self.cols, self.block)
+        if scales.dtype is not torch.uint8 or not scales.is_contiguous() or scales.numel() < size:
+            raise ValueError(f"scales must be contiguous uint8 of {size} bytes")
+        if scales.device != data.device:
+            raise ValueError(f"scales is on {scales.device}, not on {data.device}")
+        self._set(data, scales, int(rows), int(cols), int(block), step if rows > 1 else max(step, pitch) // 16 * 16)
+
+    def _set(self, data, scales, rows, cols, block, pitch):
+        self.data, self.scales, self.rows, self.cols, self.block = data, scales, rows, cols, block
+        self._packed = _MATRIX.pack(data.data_ptr(), scales.data_ptr(), pitch, rows, cols, block)
 
     @classmethod
     def empty(cls, rows: int, cols: int, block: int = 32, device="cuda"):
         torch = _torch or _lazy_torch()
         if block not in (16, 32) or rows < 0 or cols < 1:
             raise ValueError(f"{rows} x {cols} in blocks of {block} is not a 4-bit matrix")
-        pitch, scales = -(-cols // 32) * 16, -(-rows // 128) * -(-cols // (4 * block)) * 512
-        return cls(torch.empty((rows, pitch), dtype=torch.uint8, device=device),
-                   torch.empty(scales, dtype=torch.uint8, device=device), rows, cols, block)
+        pitch = -(-cols // 32) * 16
+        self = cls.__new__(cls)
+        self._set(_new((rows, pitch), torch.uint8, device),
+                  _new((-(-rows // 128) * -(-cols // (4 * block)) * 512,), torch.uint8, device), rows, cols, block, pitch)
+        return self
 
     @property
     def shape(self):
@@ -240,7 +278,7 @@ def mx4_quantize(x, block: int = 32, out: Mx4Tensor | None = None, stream=None) 
 def _output(out, rows: int, cols: int, dtype, device):
     """(tensor, row stride) of a matrix result: a new one of `dtype`, or `out` checked."""
     if out is None:
-        return _torch.empty((rows, cols), dtype=dtype, device=device), cols
+        return _new((rows, cols), dtype, device), cols
     if out.shape != (rows, cols) or out.dtype is not dtype or out.device != device or (cols > 1 and out.stride(1) != 1):
         raise ValueError(f"out must be [{rows}][{cols}] of {dtype} on {device} with contiguous columns")
     return out, out.stride(0)
@@ -263,8 +301,9 @@ def mx4_product(a: Mx4Tensor, b: Mx4Tensor, bias=None, activation: str = "none",
     torch = _torch or _lazy_torch()
     dtype = dtype or (out.dtype if out is not None else torch.float16)
     code, act, device = _dtype(dtype, "dtype"), _activation(activation), a.device
-    _same_device(device, b=b, bias=bias)
+    if b.data.device != device:
+        raise ValueError(f"b is on {b.device}, not on {device}")
     y, stride = _output(out, a.rows, b.rows, dtype, device)
     _launch(device, stream, (y if out is None else None,), load().nt_mx4_product, a._packed, b._packed,
-            _vector(bias, b.rows, "bias"), act, alpha, y.data_ptr(), code, stride)
+            _vector(bias, b.rows, device, "bias"), act, alpha, y.data_ptr(), code, stride)
     return y
