@@ -6,7 +6,8 @@
 //   warp 0      copies: TMA tiles of codes (128-byte rows, 128-byte swizzle; zeros past the matrix)
 //               and the scale tiles, which lie in memory as tensor memory wants them
 //   warp 1      per stage: scale tiles shared -> tensor memory, four products of K = 64, commit
-//   warps 4-7   epilogue: accumulator -> scale, bias, activation, rounding -> shared -> rows of d
+//   warps 4-11  epilogue: accumulator -> scale, bias, activation, rounding -> shared -> rows of d, two
+//               warps for each quarter of the lanes
 // Accumulators are doubled in tensor memory, so that the epilogue of a tile runs under the products
 // of the next; blocks take tiles gridDim apart.
 //
@@ -43,7 +44,7 @@ struct ProductLaunch {
     int64_t row_stride;
 };
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 384, kEpilogueWarps = 8;
 constexpr int kStageK = 256, kStageRow = 128;  // values and bytes of a row of a stage
 constexpr int kLaneBytes = 128 * kStageRow;
 constexpr int kMaxStages = 8;
@@ -59,7 +60,8 @@ struct Control {
 };
 
 struct Shared {
-    alignas(128) uint8_t staging[4 * 32 * kStagePitch];
+    alignas(128) uint8_t staging[kEpilogueWarps][32 * kStagePitch];
+    alignas(16) float bias[kEpilogueWarps][64];
     Control ctl;
 };
 
@@ -174,46 +176,55 @@ __device__ __forceinline__ uint32_t pack2(int dtype, float lo, float hi)
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// Lanes are b's rows: lane = column of d, accumulator columns = rows of d; a warp's store is contiguous.
-__device__ __forceinline__ void epilogue_swapped(const ProductLaunch &p, uint32_t tmem, int lane0, int col0)
+// Lanes are b's rows: lane = column of d, accumulator columns = rows of d; a warp's store is contiguous.  The two
+// warps of a quarter take every other 32 columns (`half`).
+template <int ACT>
+__device__ __forceinline__ void epilogue_swapped(const ProductLaunch &p, uint32_t tmem, int lane0, int col0, int half)
 {
     const int64_t n = lane0 + (threadIdx.x & 127);
     const float bias = p.bias && n < p.l_rows ? __ldg(p.bias + n) : 0.f;
-    for (int c0 = 0; c0 < p.bn; c0 += 32) {
+    for (int c0 = 32 * half; c0 < p.bn; c0 += 64) {
         uint32_t v[32];
         ld32(tmem + c0, v);
         umma::wait_ld();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
+        for (int i = 0; i < 32; i += 2) {
+            const float2 y = activate2<ACT>(__ffma2_rn(f2(p.alpha), make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), f2(bias)));
             const int64_t m = col0 + c0 + i;
-            if (c0 + i < p.bn && m < p.c_rows && n < p.l_rows)
-                store_one(p, m * p.row_stride + n, activate1(fmaf(p.alpha, __uint_as_float(v[i]), bias), p.activation));
+            if (n < p.l_rows) {
+                if (c0 + i < p.bn && m < p.c_rows) store_one(p, m * p.row_stride + n, y.x);
+                if (c0 + i + 1 < p.bn && m + 1 < p.c_rows) store_one(p, (m + 1) * p.row_stride + n, y.y);
+            }
         }
     }
 }
 
 // Lanes are a's rows: a warp turns 32 rows x 32 or 64 columns in shared memory and writes them row by row.
-__device__ __forceinline__ void epilogue_rows(const ProductLaunch &p, uint32_t tmem, int lane0, int col0, uint8_t *staging)
+// The two warps of a quarter take every other such column range.
+template <int ACT>
+__device__ __forceinline__ void epilogue_rows(const ProductLaunch &p, uint32_t tmem, int lane0, int col0, int half, uint8_t *mine,
+                                              float *bias)
 {
-    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) & 3;
+    const int lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) & 3;
     const int size = p.dtype == NT_DTYPE_F32 ? 4 : 2;
-    const int width = size == 2 && p.bn % 64 == 0 ? 64 : 32;  // columns of a pass
-    uint8_t *mine = staging + warp * 32 * kStagePitch;
-    for (int c0 = 0; c0 < p.bn; c0 += width) {
+    const int width = size == 2 && p.bn % 128 == 0 ? 64 : 32;  // columns of a pass
+    for (int c0 = width * half; c0 < p.bn; c0 += 2 * width) {
         if (col0 + c0 >= p.c_rows) break;
+        for (int i = lane; i < width; i += 32) bias[i] = p.bias && col0 + c0 + i < p.c_rows ? __ldg(p.bias + col0 + c0 + i) : 0.f;
+        __syncwarp();
         for (int s = 0; s < width; s += 32) {
             uint32_t v[32];
             ld32(tmem + c0 + s, v);
-            const int64_t nb = col0 + c0 + s + lane;
-            const float bias = p.bias && nb < p.c_rows ? __ldg(p.bias + nb) : 0.f;
             umma::wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-                const float2 b = make_float2(__shfl_sync(0xffffffffu, bias, i), __shfl_sync(0xffffffffu, bias, i + 1));
-                const float2 z = __ffma2_rn(f2(p.alpha), make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), b);
-                const float2 y = activate2(z, p.activation);
+            for (int i = 0; i < 32; i += 4) {
+                const float4 b = *reinterpret_cast<const float4 *>(bias + s + i);
+                float2 y = activate2<ACT>(__ffma2_rn(f2(p.alpha), make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), make_float2(b.x, b.y)));
                 v[i] = __float_as_uint(y.x);
                 v[i + 1] = __float_as_uint(y.y);
+                y = activate2<ACT>(__ffma2_rn(f2(p.alpha), make_float2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), make_float2(b.z, b.w)));
+                v[i + 2] = __float_as_uint(y.x);
+                v[i + 3] = __float_as_uint(y.y);
             }
             uint8_t *row = mine + lane * kStagePitch + s * size;
             if (size == 4) {
@@ -232,14 +243,16 @@ __device__ __forceinline__ void epilogue_rows(const ProductLaunch &p, uint32_t t
             }
         }
         __syncwarp();
-        const int64_t m0 = lane0 + warp * 32, n0 = col0 + c0;
+        const int64_t m0 = lane0 + quarter * 32, n0 = col0 + c0;
         const int rows = (int)min((int64_t)32, p.l_rows - m0);
         uint8_t *dst = static_cast<uint8_t *>(p.d) + (m0 * p.row_stride + n0) * size;
         if (p.vec && n0 + width <= p.c_rows) {
             const int per_row = width * size / 16, step = 32 / per_row;  // 4 or 8 lanes a row
-            for (int r = lane / per_row; r < rows; r += step)
-                *reinterpret_cast<uint4 *>(dst + r * p.row_stride * size + (lane % per_row) * 16) =
-                    *reinterpret_cast<const uint4 *>(mine + r * kStagePitch + (lane % per_row) * 16);
+            const int64_t pitch = p.row_stride * size;
+            const uint8_t *from = mine + (lane / per_row) * kStagePitch + (lane % per_row) * 16;
+            uint8_t *to = dst + (lane / per_row) * pitch + (lane % per_row) * 16;
+            for (int r = lane / per_row; r < rows; r += step, from += step * kStagePitch, to += step * pitch)
+                *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(from);
         } else {
             const int cols = (int)min((int64_t)width, p.c_rows - n0);
             for (int r = 0; r < rows; ++r)
@@ -255,6 +268,34 @@ __device__ __forceinline__ void epilogue_rows(const ProductLaunch &p, uint32_t t
         __syncwarp();
     }
 }
+
+template <int ACT>
+__device__ __forceinline__ void epilogue(const ProductLaunch &p, uint32_t tmem, int lane0, int col0, int half, uint8_t *mine, float *bias)
+{
+    if (p.swapped) epilogue_swapped<ACT>(p, tmem, lane0, col0, half);
+    else epilogue_rows<ACT>(p, tmem, lane0, col0, half, mine, bias);
+}
+
+// The tiles of a block, `step` apart in the order lane tiles first; kept as (lane tile, column tile) without
+// divisions.
+struct Tiles {
+    int l, c, dl, dc, l_tiles, c_tiles;
+    __device__ __forceinline__ Tiles(const ProductLaunch &p)
+    {
+        const unsigned first = blockIdx.x / p.split, step = gridDim.x / p.split;
+        l_tiles = p.l_tiles;
+        c_tiles = p.c_tiles;
+        l = (int)(first % (unsigned)l_tiles), c = (int)(first / (unsigned)l_tiles);
+        dl = (int)(step % (unsigned)l_tiles), dc = (int)(step / (unsigned)l_tiles);
+    }
+    __device__ __forceinline__ bool valid() const { return c < c_tiles; }
+    __device__ __forceinline__ void next()
+    {
+        l += dl;
+        c += dc;
+        if (l >= l_tiles) l -= l_tiles, ++c;
+    }
+};
 
 template <int BLOCK>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -272,8 +313,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int k_stages = (p.k + kStageK - 1) / kStageK, k_steps = (p.k + 63) / 64;
     const int rank = p.split > 1 ? blockIdx.x % p.split : 0;
     const int k_lo = (int)((int64_t)k_stages * rank / p.split), k_hi = (int)((int64_t)k_stages * (rank + 1) / p.split);
-    const int64_t tiles = (int64_t)p.l_tiles * p.c_tiles;
-    const int64_t tile0 = blockIdx.x / p.split, tile_step = gridDim.x / p.split;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.stages; ++i) {
@@ -282,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             umma::mbar_init(acc_full + 8 * i, 1);
-            umma::mbar_init(acc_empty + 8 * i, 4);
+            umma::mbar_init(acc_empty + 8 * i, kEpilogueWarps);
         }
         umma::mbar_fence_init();
     }
@@ -296,9 +335,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         int s = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for (int64_t t = tile0; ok && t < tiles; t += tile_step) {
-            const int lt = (int)(t % p.l_tiles), ct = (int)(t / p.l_tiles);
-            const int c0 = ct * p.bn;
+        for (Tiles t(p); ok && t.valid(); t.next()) {
+            const int lt = t.l, c0 = t.c * p.bn;
             for (int ks = k_lo; ks < k_hi; ++ks) {
                 if (!(ok = wait(empty + 8 * s, phase ^ 1))) break;
                 const uint32_t at = base + s * p.stage_bytes, bar = full + 8 * s;
@@ -317,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int s = 0, buf = 0, sbuf = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
-        for (int64_t t = tile0; ok && t < tiles; t += tile_step) {
+        for (Tiles t(p); ok && t.valid(); t.next()) {
             if (!(ok = wait(acc_empty + 8 * buf, acc_phase ^ 1))) break;
             umma::fence_after();
             const uint32_t acc = tmem + buf * kMaxBn;
@@ -348,15 +386,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp >= 4) {
         int buf = 0;
+        const int half = (warp - 4) >> 2;
+        uint8_t *const mine = sh.staging[warp - 4];
+        float *const bias = sh.bias[warp - 4];
         uint32_t acc_phase = 0;
-        for (int64_t t = tile0; t < tiles; t += tile_step) {
+        for (Tiles t(p); t.valid(); t.next()) {
             if (!__all_sync(0xffffffffu, wait(acc_full + 8 * buf, acc_phase))) break;
             umma::fence_after();
             const uint32_t acc = tmem + buf * kMaxBn + ((uint32_t)(warp & 3) << 21);
-            const int lane0 = (int)(t % p.l_tiles) * 128, col0 = (int)(t / p.l_tiles) * p.bn;
+            const int lane0 = t.l * 128, col0 = t.c * p.bn;
             if (p.split > 1) {  // partial sums [column][lane], a lane a bank
                 float *dump = reinterpret_cast<float *>(stages) + (threadIdx.x & 127);
-                for (int c0 = 0; c0 < p.bn; c0 += 32) {
+                for (int c0 = 32 * half; c0 < p.bn; c0 += 64) {
                     uint32_t v[32];
                     ld32(acc + c0, v);
                     umma::wait_ld();
@@ -364,10 +405,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int i = 0; i < 32; ++i)
                         if (c0 + i < p.bn) dump[(c0 + i) * 129] = __uint_as_float(v[i]);
                 }
-            } else if (p.swapped) {
-                epilogue_swapped(p, acc, lane0, col0);
             } else {
-                epilogue_rows(p, acc, lane0, col0, sh.staging);
+                switch (p.activation) {
+                case NT_ACT_RELU: epilogue<NT_ACT_RELU>(p, acc, lane0, col0, half, mine, bias); break;
+                case NT_ACT_SILU: epilogue<NT_ACT_SILU>(p, acc, lane0, col0, half, mine, bias); break;
+                case NT_ACT_GELU: epilogue<NT_ACT_GELU>(p, acc, lane0, col0, half, mine, bias); break;
+                default: epilogue<NT_ACT_NONE>(p, acc, lane0, col0, half, mine, bias); break;
+                }
             }
             umma::fence_before();
             __syncwarp();
@@ -380,7 +424,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (p.split > 1) {
         __syncthreads();
         cluster_sync();
-        const int lane0 = (int)(tile0 % p.l_tiles) * 128, col0 = (int)(tile0 / p.l_tiles) * p.bn;
+        const Tiles t(p);
+        const int lane0 = t.l * 128, col0 = t.c * p.bn;
         const int lo = p.bn * rank / p.split, cols = p.bn * (rank + 1) / p.split - lo;
         for (int i = threadIdx.x; i < cols * 128; i += kThreads) {
             // consecutive threads along d's rows
