@@ -138,6 +138,16 @@ __device__ __forceinline__ void ld32(uint32_t taddr, uint32_t (&r)[32])
         : "r"(taddr));
 }
 
+// One lane of a converged warp, the same one every time.  The issuing warps run their loops whole and only
+// their asynchronous instructions under this predicate: operands then stay in uniform registers, without
+// which every such instruction took 80 to 100 cycles to issue.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
+    return p != 0;
+}
+
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity)
 {
     if (umma::mbar_wait(bar, parity)) return true;
@@ -331,56 +341,65 @@ __global__ void __launch_bounds__(kThreads, 1)
     umma::fence_after();
     const uint32_t tmem = ctl.tmem;
 
-    if (warp == 0 && lane == 0) {
+    if (warp == 0) {
         int s = 0;
         uint32_t phase = 0;
         bool ok = true;
         for (Tiles t(p); ok && t.valid(); t.next()) {
             const int lt = t.l, c0 = t.c * p.bn;
             for (int ks = k_lo; ks < k_hi; ++ks) {
-                if (!(ok = wait(empty + 8 * s, phase ^ 1))) break;
+                if (!(ok = __all_sync(0xffffffffu, wait(empty + 8 * s, phase ^ 1)))) break;
                 const uint32_t at = base + s * p.stage_bytes, bar = full + 8 * s;
                 const int st = min(kTiles, p.scale_tiles - ks * kTiles);
-                expect_tx(bar, kLaneBytes + p.bn * kStageRow + 2 * st * kTileBytes);
-                tma_2d(at, &l_map, ks * kStageRow, lt * 128, bar);
-                tma_2d(at + c_off, &c_map, ks * kStageRow, c0, bar);
-                bulk_copy(at + ls_off, p.l_scales + ((int64_t)lt * p.scale_tiles + ks * kTiles) * kTileBytes, st * kTileBytes, bar);
-                bulk_copy(at + cs_off, p.c_scales + ((int64_t)(c0 >> 7) * p.scale_tiles + ks * kTiles) * kTileBytes, st * kTileBytes, bar);
+                if (elect_one()) {
+                    expect_tx(bar, kLaneBytes + p.bn * kStageRow + 2 * st * kTileBytes);
+                    tma_2d(at, &l_map, ks * kStageRow, lt * 128, bar);
+                    tma_2d(at + c_off, &c_map, ks * kStageRow, c0, bar);
+                    bulk_copy(at + ls_off, p.l_scales + ((int64_t)lt * p.scale_tiles + ks * kTiles) * kTileBytes, st * kTileBytes, bar);
+                    bulk_copy(at + cs_off, p.c_scales + ((int64_t)(c0 >> 7) * p.scale_tiles + ks * kTiles) * kTileBytes,
+                              st * kTileBytes, bar);
+                }
+                __syncwarp();
                 if (++s == p.stages) s = 0, phase ^= 1;
             }
         }
         if (!ok)  // the products have stopped: wait for the copies that nobody will wait for
             for (int i = 0; i < p.stages; ++i) umma::mbar_wait(full + 8 * i, i < s ? phase : phase ^ 1, 1u << 16);
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
         int s = 0, buf = 0, sbuf = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
         for (Tiles t(p); ok && t.valid(); t.next()) {
-            if (!(ok = wait(acc_empty + 8 * buf, acc_phase ^ 1))) break;
+            if (!(ok = __all_sync(0xffffffffu, wait(acc_empty + 8 * buf, acc_phase ^ 1)))) break;
             umma::fence_after();
             const uint32_t acc = tmem + buf * kMaxBn;
-            uint32_t more = 0;
             for (int ks = k_lo; ks < k_hi; ++ks) {
-                if (!(ok = wait(full + 8 * s, phase))) break;
+                if (!(ok = __all_sync(0xffffffffu, wait(full + 8 * s, phase)))) break;
                 umma::fence_after();
                 const uint32_t at = base + s * p.stage_bytes, sl = tmem + kScaleCol + sbuf * kScaleCols, sc = sl + 16;
-                const int steps = min(4, k_steps - ks * 4), st = BLOCK == 16 ? steps : (steps + 1) >> 1;
-                for (int i = 0; i < st; ++i) {
-                    copy_scale_tile(sl + 4 * i, at + ls_off + i * kTileBytes);
-                    copy_scale_tile(sc + 4 * i, at + cs_off + i * kTileBytes);
-                }
+                const int steps = min(4, k_steps - ks * 4);
                 const uint64_t da = codes_desc(at), db = codes_desc(at + c_off);
-                for (int i = 0; i < steps; ++i) {
-                    const int tile = BLOCK == 16 ? i : i >> 1;
-                    mma<BLOCK>(acc, da + 2 * i, db + 2 * i, idesc<BLOCK>(p.bn, BLOCK == 16 ? 0 : (i & 1) * 2), sl + 4 * tile,
-                               sc + 4 * tile, more);
-                    more = 1;
+                if (elect_one()) {
+#pragma unroll
+                    for (int i = 0; i < kTiles; ++i)
+                        if (i * (4 / kTiles) < steps) {
+                            copy_scale_tile(sl + 4 * i, at + ls_off + i * kTileBytes);
+                            copy_scale_tile(sc + 4 * i, at + cs_off + i * kTileBytes);
+                        }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (i < steps) {
+                            const int tile = BLOCK == 16 ? i : i >> 1;
+                            mma<BLOCK>(acc, da + 2 * i, db + 2 * i, idesc<BLOCK>(p.bn, BLOCK == 16 ? 0 : (i & 1) * 2), sl + 4 * tile,
+                                       sc + 4 * tile, ks > k_lo || i > 0);
+                        }
+                    umma::commit(empty + 8 * s);
+                    if (ks + 1 == k_hi) umma::commit(acc_full + 8 * buf);
                 }
-                umma::commit(empty + 8 * s);
+                __syncwarp();
                 if (++s == p.stages) s = 0, phase ^= 1;
                 sbuf ^= 1;
             }
-            if (ok) umma::commit(acc_full + 8 * buf);
             buf ^= 1;
             if (buf == 0) acc_phase ^= 1;
         }
