@@ -3,8 +3,8 @@
 //
 // One operand's rows are the accumulator's 128 lanes (the lane operand), the other's its bn columns
 // (the column operand).  A thread block computes 128 x bn tiles, 256 values of K a stage:
-//   warp 0      copies: TMA tiles of codes (128-byte rows, 128-byte swizzle; zeros past the matrix)
-//               and the scale tiles, which lie in memory as tensor memory wants them
+//   warp 0      copies: TMA tiles of codes (rows of 128 bytes, or 32 or 64 where K is no longer, swizzled;
+//               zeros past the matrix) and the scale tiles, which lie in memory as tensor memory wants them
 //   warp 1      per stage: scale tiles shared -> tensor memory, four products of K = 64, commit
 //   warps 4-11  epilogue: accumulator -> scale, bias, activation, rounding -> shared -> rows of d, two
 //               warps for each quarter of the lanes
@@ -34,6 +34,8 @@ struct ProductLaunch {
     int32_t bn, l_tiles, c_tiles;
     int32_t scale_tiles;       // scale tiles of 128 rows of either operand
     int32_t stages, stage_bytes;
+    int32_t row_bytes;         // codes of a row in a stage: 32, 64 or 128 bytes
+    uint64_t layout;           // their swizzle and group stride, as descriptor bits
     int32_t split;             // thread blocks of a cluster, each with a share of K
     int32_t swapped;           // 1: lanes are b's rows (d's columns)
     int32_t dtype, vec;        // vec: rows of d take 16-byte stores
@@ -45,8 +47,6 @@ struct ProductLaunch {
 };
 
 constexpr int kThreads = 384, kEpilogueWarps = 8;
-constexpr int kStageK = 256, kStageRow = 128;  // values and bytes of a row of a stage
-constexpr int kLaneBytes = 128 * kStageRow;
 constexpr int kMaxStages = 8;
 constexpr int kMaxBn = 128;
 constexpr int kStagePitch = 144;  // epilogue staging row: 128 bytes and a 16-byte shift of the banks
@@ -87,11 +87,8 @@ __device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes)
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 
-// Codes: rows of 128 bytes, 8-row groups 1024 bytes apart, 128-byte swizzle.
-__device__ __forceinline__ uint64_t codes_desc(uint32_t addr)
-{
-    return umma::desc(addr, 16, 1024) | (uint64_t)2 << 61;
-}
+// Codes: `layout` with the address of the first row.
+__device__ __forceinline__ uint64_t codes_desc(uint32_t addr, uint64_t layout) { return umma::desc(addr, 16, 0) | layout; }
 
 // A scale tile: 32 rows of 16 bytes -> 4 columns of all four lane quarters.
 __device__ __forceinline__ void copy_scale_tile(uint32_t tmem, uint32_t addr)
@@ -319,8 +316,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = smem_u32(stages), full = smem_u32(ctl.full), empty = smem_u32(ctl.empty),
                    acc_full = smem_u32(ctl.acc_full), acc_empty = smem_u32(ctl.acc_empty);
-    const int c_off = kLaneBytes, ls_off = c_off + p.bn * kStageRow, cs_off = ls_off + kTiles * kTileBytes;
-    const int k_stages = (p.k + kStageK - 1) / kStageK, k_steps = (p.k + 63) / 64;
+    const int c_off = 128 * p.row_bytes, ls_off = c_off + p.bn * p.row_bytes, cs_off = ls_off + kTiles * kTileBytes;
+    const int k_steps = (p.k + 63) / 64, stage_steps = p.row_bytes / 32, k_stages = (k_steps + stage_steps - 1) / stage_steps;
     const int rank = p.split > 1 ? blockIdx.x % p.split : 0;
     const int k_lo = (int)((int64_t)k_stages * rank / p.split), k_hi = (int)((int64_t)k_stages * (rank + 1) / p.split);
 
@@ -352,9 +349,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t at = base + s * p.stage_bytes, bar = full + 8 * s;
                 const int st = min(kTiles, p.scale_tiles - ks * kTiles);
                 if (elect_one()) {
-                    expect_tx(bar, kLaneBytes + p.bn * kStageRow + 2 * st * kTileBytes);
-                    tma_2d(at, &l_map, ks * kStageRow, lt * 128, bar);
-                    tma_2d(at + c_off, &c_map, ks * kStageRow, c0, bar);
+                    expect_tx(bar, ls_off + 2 * st * kTileBytes);
+                    tma_2d(at, &l_map, ks * p.row_bytes, lt * 128, bar);
+                    tma_2d(at + c_off, &c_map, ks * p.row_bytes, c0, bar);
                     bulk_copy(at + ls_off, p.l_scales + ((int64_t)lt * p.scale_tiles + ks * kTiles) * kTileBytes, st * kTileBytes, bar);
                     bulk_copy(at + cs_off, p.c_scales + ((int64_t)(c0 >> 7) * p.scale_tiles + ks * kTiles) * kTileBytes,
                               st * kTileBytes, bar);
@@ -377,8 +374,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!(ok = __all_sync(0xffffffffu, wait(full + 8 * s, phase)))) break;
                 umma::fence_after();
                 const uint32_t at = base + s * p.stage_bytes, sl = tmem + kScaleCol + sbuf * kScaleCols, sc = sl + 16;
-                const int steps = min(4, k_steps - ks * 4);
-                const uint64_t da = codes_desc(at), db = codes_desc(at + c_off);
+                const int steps = min(stage_steps, k_steps - ks * stage_steps);
+                const uint64_t da = codes_desc(at, p.layout), db = codes_desc(at + c_off, p.layout);
                 if (elect_one()) {
 #pragma unroll
                     for (int i = 0; i < kTiles; ++i)
@@ -483,15 +480,18 @@ EncodeTiled encode_tiled()
     return fn;
 }
 
-// Codes as a byte matrix, read in boxes of `box_rows` rows x 128 bytes.
-bool encode_codes(CUtensorMap *map, const NtMx4Matrix *m, int box_rows)
+// Codes as a byte matrix, read in boxes of `box_rows` rows x `row_bytes`.
+bool encode_codes(CUtensorMap *map, const NtMx4Matrix *m, int box_rows, int row_bytes)
 {
     const EncodeTiled encode = encode_tiled();
     if (!encode) return false;
     const cuuint64_t size[2] = {(cuuint64_t)row_pitch(m->cols), (cuuint64_t)m->rows}, stride[1] = {(cuuint64_t)m->pitch};
-    const cuuint32_t box[2] = {kStageRow, (cuuint32_t)box_rows}, step[2] = {1, 1};
+    const cuuint32_t box[2] = {(cuuint32_t)row_bytes, (cuuint32_t)box_rows}, step[2] = {1, 1};
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, m->data, size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+                  row_bytes == 32   ? CU_TENSOR_MAP_SWIZZLE_32B
+                  : row_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                    : CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -512,22 +512,25 @@ nt_status launch_product(const NtMx4Matrix *a, const NtMx4Matrix *b, ProductLaun
     p.l_rows = l->rows;
     p.c_rows = c->rows;
     p.k = a->cols;
+    // a box that reaches past the end of its rows is copied several times slower than a whole one
+    p.row_bytes = p.k <= 64 ? 32 : p.k <= 128 ? 64 : 128;
+    p.layout = (uint64_t)(p.row_bytes / 2) << 32 | (uint64_t)(p.row_bytes == 32 ? 6 : p.row_bytes == 64 ? 4 : 2) << 61;
     p.l_tiles = (int32_t)ceil_div(l->rows, 128);
     p.c_tiles = (int32_t)ceil_div(c->rows, p.bn);
     p.scale_tiles = tiles_per_row(p.k, BLOCK);
     p.l_scales = static_cast<const uint8_t *>(l->scales);
     p.c_scales = static_cast<const uint8_t *>(c->scales);
-    const int64_t tiles = (int64_t)p.l_tiles * p.c_tiles, k_stages = ceil_div(p.k, kStageK);
+    const int64_t tiles = (int64_t)p.l_tiles * p.c_tiles, k_stages = ceil_div(p.k, 2 * p.row_bytes);
     // split K while blocks stand idle and every share keeps two stages
     p.split = 1;
     while (p.split < 8 && p.bn <= 128 && tiles * p.split * 2 <= sms && k_stages >= p.split * 4) p.split *= 2;
-    p.stage_bytes = (int32_t)ceil_div(kLaneBytes + p.bn * kStageRow + 2 * kTiles * kTileBytes, 1024) * 1024;
+    p.stage_bytes = (int32_t)ceil_div((128 + p.bn) * p.row_bytes + 2 * kTiles * kTileBytes, 1024) * 1024;
     const int room = 227 * 1024 - 1024 - (int)sizeof(Shared);
     p.stages = std::min(kMaxStages, room / p.stage_bytes);
     const size_t smem = 1024 + std::max((size_t)p.stages * p.stage_bytes, p.split > 1 ? (size_t)p.bn * 129 * 4 : 0);
     const int64_t grid = p.split > 1 ? tiles * p.split : std::min<int64_t>(tiles, sms);
     CUtensorMap l_map, c_map;
-    if (!encode_codes(&l_map, l, 128) || !encode_codes(&c_map, c, p.bn))
+    if (!encode_codes(&l_map, l, 128, p.row_bytes) || !encode_codes(&c_map, c, p.bn, p.row_bytes))
         return set_error(NT_ERR_CUDA, "4-bit product: the tensor maps could not be encoded");
     const void *kernel = reinterpret_cast<const void *>(&product_kernel<BLOCK>);
     cudaError_t e = set_smem_limit(kernel, 227 * 1024 - sizeof(Shared));
