@@ -8,8 +8,9 @@
 //   warp 1      per stage: scale tiles shared -> tensor memory, four products of K = 64, commit
 //   warps 4-11  epilogue: accumulator -> scale, bias, activation, rounding -> shared -> rows of d, two
 //               warps for each quarter of the lanes
-// Accumulators are doubled in tensor memory, so that the epilogue of a tile runs under the products
-// of the next; blocks take tiles gridDim apart.
+// There are two accumulators in tensor memory, so that the epilogue of a tile runs under the products of the
+// next; blocks take tiles gridDim apart.  Two of 256 columns and the scales do not fit: they share 96
+// columns, which the epilogue reads first.
 //
 // Few rows (m <= 64): the weights' rows go to the lanes, and bn is m rounded up, so that a token costs no
 // empty columns.  Few tiles: a cluster of up to 8 blocks splits K, leaves its partial sums in shared
@@ -48,14 +49,15 @@ struct ProductLaunch {
 
 constexpr int kThreads = 384, kEpilogueWarps = 8;
 constexpr int kMaxStages = 8;
-constexpr int kMaxBn = 128;
+constexpr int kAccStep = 160;  // columns between the two accumulators
 constexpr int kStagePitch = 144;  // epilogue staging row: 128 bytes and a 16-byte shift of the banks
-constexpr uint32_t kTmemCols = 512, kScaleCol = 256, kScaleCols = 32;
+constexpr uint32_t kTmemCols = 512, kScaleCol = 416, kScaleCols = 48;
 
 struct Control {
     alignas(8) uint64_t full[kMaxStages];
     uint64_t empty[kMaxStages];
     uint64_t acc_full[2], acc_empty[2];
+    uint64_t acc_part[2];  // the columns that the other accumulator shares are free
     uint32_t tmem;
 };
 
@@ -207,16 +209,23 @@ __device__ __forceinline__ void epilogue_swapped(const ProductLaunch &p, uint32_
 }
 
 // Lanes are a's rows: a warp turns 32 rows x 32 or 64 columns in shared memory and writes them row by row.
-// The two warps of a quarter take every other such column range.
+// The two warps of a quarter take every other such column range; of 256 columns, those from `first` on come first,
+// and `part` is told when they have been read.
 template <int ACT>
-__device__ __forceinline__ void epilogue_rows(const ProductLaunch &p, uint32_t tmem, int lane0, int col0, int half, uint8_t *mine,
-                                              float *bias)
+__device__ __forceinline__ void epilogue_rows(const ProductLaunch &p, uint32_t tmem, int lane0, int col0, int half, int first, uint32_t part,
+                                              uint8_t *mine, float *bias)
 {
     const int lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) & 3;
     const int size = p.dtype == NT_DTYPE_F32 ? 4 : 2;
     const int width = size == 2 && p.bn % 128 == 0 ? 64 : 32;  // columns of a pass
-    for (int c0 = width * half; c0 < p.bn; c0 += 2 * width) {
-        if (col0 + c0 >= p.c_rows) break;
+    for (int i0 = width * half; i0 < p.bn; i0 += 2 * width) {
+        const int c0 = p.bn > kAccStep ? i0 ^ first : i0;
+        if (p.bn > kAccStep && i0 >= 128 && i0 < 128 + 2 * width) {  // 128 columns have been read, the shared ones among them
+            umma::fence_before();
+            __syncwarp();
+            if (lane == 0) umma::mbar_arrive(part);
+        }
+        if (col0 + c0 >= p.c_rows) continue;
         for (int i = lane; i < width; i += 32) bias[i] = p.bias && col0 + c0 + i < p.c_rows ? __ldg(p.bias + col0 + c0 + i) : 0.f;
         __syncwarp();
         for (int s = 0; s < width; s += 32) {
@@ -277,10 +286,11 @@ __device__ __forceinline__ void epilogue_rows(const ProductLaunch &p, uint32_t t
 }
 
 template <int ACT>
-__device__ __forceinline__ void epilogue(const ProductLaunch &p, uint32_t tmem, int lane0, int col0, int half, uint8_t *mine, float *bias)
+__device__ __forceinline__ void epilogue(const ProductLaunch &p, uint32_t tmem, int lane0, int col0, int half, int first, uint32_t part,
+                                         uint8_t *mine, float *bias)
 {
     if (p.swapped) epilogue_swapped<ACT>(p, tmem, lane0, col0, half);
-    else epilogue_rows<ACT>(p, tmem, lane0, col0, half, mine, bias);
+    else epilogue_rows<ACT>(p, tmem, lane0, col0, half, first, part, mine, bias);
 }
 
 // The tiles of a block, `step` apart in the order lane tiles first; kept as (lane tile, column tile) without
@@ -315,8 +325,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t *stages = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = smem_u32(stages), full = smem_u32(ctl.full), empty = smem_u32(ctl.empty),
-                   acc_full = smem_u32(ctl.acc_full), acc_empty = smem_u32(ctl.acc_empty);
+                   acc_full = smem_u32(ctl.acc_full), acc_empty = smem_u32(ctl.acc_empty), acc_part = smem_u32(ctl.acc_part);
     const int c_off = 128 * p.row_bytes, ls_off = c_off + p.bn * p.row_bytes, cs_off = ls_off + kTiles * kTileBytes;
+    const int c_scales = p.bn > 128 ? 2 : 1;  // row tiles of the column operand's scales
     const int k_steps = (p.k + 63) / 64, stage_steps = p.row_bytes / 32, k_stages = (k_steps + stage_steps - 1) / stage_steps;
     const int rank = p.split > 1 ? blockIdx.x % p.split : 0;
     const int k_lo = (int)((int64_t)k_stages * rank / p.split), k_hi = (int)((int64_t)k_stages * (rank + 1) / p.split);
@@ -329,6 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 2; ++i) {
             umma::mbar_init(acc_full + 8 * i, 1);
             umma::mbar_init(acc_empty + 8 * i, kEpilogueWarps);
+            umma::mbar_init(acc_part + 8 * i, kEpilogueWarps);
         }
         umma::mbar_fence_init();
     }
@@ -348,13 +360,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!(ok = __all_sync(0xffffffffu, wait(empty + 8 * s, phase ^ 1)))) break;
                 const uint32_t at = base + s * p.stage_bytes, bar = full + 8 * s;
                 const int st = min(kTiles, p.scale_tiles - ks * kTiles);
+                const int cs = min(c_scales, (p.c_rows - c0 + 127) >> 7);
                 if (elect_one()) {
-                    expect_tx(bar, ls_off + 2 * st * kTileBytes);
+                    expect_tx(bar, ls_off + (1 + cs) * st * kTileBytes);
                     tma_2d(at, &l_map, ks * p.row_bytes, lt * 128, bar);
                     tma_2d(at + c_off, &c_map, ks * p.row_bytes, c0, bar);
                     bulk_copy(at + ls_off, p.l_scales + ((int64_t)lt * p.scale_tiles + ks * kTiles) * kTileBytes, st * kTileBytes, bar);
-                    bulk_copy(at + cs_off, p.c_scales + ((int64_t)(c0 >> 7) * p.scale_tiles + ks * kTiles) * kTileBytes,
-                              st * kTileBytes, bar);
+                    for (int j = 0; j < cs; ++j)
+                        bulk_copy(at + cs_off + j * kTiles * kTileBytes,
+                                  p.c_scales + ((int64_t)((c0 >> 7) + j) * p.scale_tiles + ks * kTiles) * kTileBytes, st * kTileBytes,
+                                  bar);
                 }
                 __syncwarp();
                 if (++s == p.stages) s = 0, phase ^= 1;
@@ -364,12 +379,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < p.stages; ++i) umma::mbar_wait(full + 8 * i, i < s ? phase : phase ^ 1, 1u << 16);
     } else if (warp == 1) {
         int s = 0, buf = 0, sbuf = 0;
-        uint32_t phase = 0, acc_phase = 0;
-        bool ok = true;
+        uint32_t phase = 0, acc_phase = 0, part_phase = 0;
+        bool ok = true, first = true;
         for (Tiles t(p); ok && t.valid(); t.next()) {
             if (!(ok = __all_sync(0xffffffffu, wait(acc_empty + 8 * buf, acc_phase ^ 1)))) break;
+            if (p.bn > kAccStep && !first && !(ok = __all_sync(0xffffffffu, wait(acc_part + 8 * (buf ^ 1), part_phase)))) break;
+            if (buf == 0) part_phase ^= !first;
+            first = false;
             umma::fence_after();
-            const uint32_t acc = tmem + buf * kMaxBn;
+            const uint32_t acc = tmem + buf * kAccStep;
             for (int ks = k_lo; ks < k_hi; ++ks) {
                 if (!(ok = __all_sync(0xffffffffu, wait(full + 8 * s, phase)))) break;
                 umma::fence_after();
@@ -381,14 +399,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int i = 0; i < kTiles; ++i)
                         if (i * (4 / kTiles) < steps) {
                             copy_scale_tile(sl + 4 * i, at + ls_off + i * kTileBytes);
-                            copy_scale_tile(sc + 4 * i, at + cs_off + i * kTileBytes);
+                            copy_scale_tile(sc + 4 * i * c_scales, at + cs_off + i * kTileBytes);
+                            if (c_scales == 2) copy_scale_tile(sc + 8 * i + 4, at + cs_off + (kTiles + i) * kTileBytes);
                         }
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         if (i < steps) {
                             const int tile = BLOCK == 16 ? i : i >> 1;
                             mma<BLOCK>(acc, da + 2 * i, db + 2 * i, idesc<BLOCK>(p.bn, BLOCK == 16 ? 0 : (i & 1) * 2), sl + 4 * tile,
-                                       sc + 4 * tile, ks > k_lo || i > 0);
+                                       sc + 4 * tile * c_scales, ks > k_lo || i > 0);
                         }
                     umma::commit(empty + 8 * s);
                     if (ks + 1 == k_hi) umma::commit(acc_full + 8 * buf);
@@ -409,8 +428,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (Tiles t(p); t.valid(); t.next()) {
             if (!__all_sync(0xffffffffu, wait(acc_full + 8 * buf, acc_phase))) break;
             umma::fence_after();
-            const uint32_t acc = tmem + buf * kMaxBn + ((uint32_t)(warp & 3) << 21);
-            const int lane0 = t.l * 128, col0 = t.c * p.bn;
+            const uint32_t acc = tmem + buf * kAccStep + ((uint32_t)(warp & 3) << 21);
+            const int lane0 = t.l * 128, col0 = t.c * p.bn, shared_first = buf ? 0 : 128;
             if (p.split > 1) {  // partial sums [column][lane], a lane a bank
                 float *dump = reinterpret_cast<float *>(stages) + (threadIdx.x & 127);
                 for (int c0 = 32 * half; c0 < p.bn; c0 += 64) {
@@ -423,10 +442,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             } else {
                 switch (p.activation) {
-                case NT_ACT_RELU: epilogue<NT_ACT_RELU>(p, acc, lane0, col0, half, mine, bias); break;
-                case NT_ACT_SILU: epilogue<NT_ACT_SILU>(p, acc, lane0, col0, half, mine, bias); break;
-                case NT_ACT_GELU: epilogue<NT_ACT_GELU>(p, acc, lane0, col0, half, mine, bias); break;
-                default: epilogue<NT_ACT_NONE>(p, acc, lane0, col0, half, mine, bias); break;
+                case NT_ACT_RELU: epilogue<NT_ACT_RELU>(p, acc, lane0, col0, half, shared_first, acc_part + 8 * buf, mine, bias); break;
+                case NT_ACT_SILU: epilogue<NT_ACT_SILU>(p, acc, lane0, col0, half, shared_first, acc_part + 8 * buf, mine, bias); break;
+                case NT_ACT_GELU: epilogue<NT_ACT_GELU>(p, acc, lane0, col0, half, shared_first, acc_part + 8 * buf, mine, bias); break;
+                default: epilogue<NT_ACT_NONE>(p, acc, lane0, col0, half, shared_first, acc_part + 8 * buf, mine, bias); break;
                 }
             }
             umma::fence_before();
@@ -497,8 +516,14 @@ bool encode_codes(CUtensorMap *map, const NtMx4Matrix *m, int box_rows, int row_
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Columns of a tile when the lanes are a's rows.  Tiles of several start at a multiple of 128 columns, where
-// their scale tile starts; a narrower one is the only one.
-int choose_bn(int64_t n) { return n <= 32 ? 32 : n <= 64 ? 64 : 128; }
+// their scale tile starts; a narrower one is the only one.  256 columns read the lane operand half as
+// often; they are taken where that does not cost a wave of blocks.
+int choose_bn(int64_t m, int64_t n, int sms)
+{
+    if (n <= 128) return n <= 32 ? 32 : n <= 64 ? 64 : 128;
+    const int64_t rows = ceil_div(m, 128), wide = ceil_div(rows * ceil_div(n, 256), sms), narrow = ceil_div(rows * ceil_div(n, 128), sms);
+    return wide * 3 <= narrow * 2 ? 256 : 128;
+}
 
 template <int BLOCK>
 nt_status launch_product(const NtMx4Matrix *a, const NtMx4Matrix *b, ProductLaunch p, cudaStream_t st)
@@ -507,7 +532,7 @@ nt_status launch_product(const NtMx4Matrix *a, const NtMx4Matrix *b, ProductLaun
     const int sms = sm_count();
     p.swapped = a->rows <= 64;
     const NtMx4Matrix *l = p.swapped ? b : a, *c = p.swapped ? a : b;
-    p.bn = !p.swapped ? choose_bn(b->rows)
+    p.bn = !p.swapped ? choose_bn(a->rows, b->rows, sms)
            : a->rows <= 8 ? 8 : a->rows <= 16 ? 16 : a->rows <= 32 ? 32 : 64;
     p.l_rows = l->rows;
     p.c_rows = c->rows;
@@ -524,7 +549,7 @@ nt_status launch_product(const NtMx4Matrix *a, const NtMx4Matrix *b, ProductLaun
     // split K while blocks stand idle and every share keeps two stages
     p.split = 1;
     while (p.split < 8 && p.bn <= 128 && tiles * p.split * 2 <= sms && k_stages >= p.split * 4) p.split *= 2;
-    p.stage_bytes = (int32_t)ceil_div((128 + p.bn) * p.row_bytes + 2 * kTiles * kTileBytes, 1024) * 1024;
+    p.stage_bytes = (int32_t)ceil_div((128 + p.bn) * p.row_bytes + (p.bn > 128 ? 3 : 2) * kTiles * kTileBytes, 1024) * 1024;
     const int room = 227 * 1024 - 1024 - (int)sizeof(Shared);
     p.stages = std::min(kMaxStages, room / p.stage_bytes);
     const size_t smem = 1024 + std::max((size_t)p.stages * p.stage_bytes, p.split > 1 ? (size_t)p.bn * 129 * 4 : 0);
