@@ -6,8 +6,9 @@
 //   warp 0      copies: TMA tiles of codes (rows of 128 bytes, or 32 or 64 where K is no longer, swizzled;
 //               zeros past the matrix) and the scale tiles, which lie in memory as tensor memory wants them
 //   warp 1      per stage: scale tiles shared -> tensor memory, four products of K = 64, commit
-//   warps 4-11  epilogue: accumulator -> scale, bias, activation, rounding -> shared -> rows of d, two
-//               warps for each quarter of the lanes
+//   warps 4-11  epilogue: accumulator -> scale, bias, activation, rounding -> shared -> rows of d by TMA.  Two
+//               warps for each quarter of the lanes: they halve a tile's columns, or, of tiles of 64 columns
+//               and less, take every other tile
 // There are two accumulators in tensor memory, so that the epilogue of a tile runs under the products of the
 // next; blocks take tiles gridDim apart.  Two of 256 columns and the scales do not fit: they share 96
 // columns, which the epilogue reads first.
@@ -39,7 +40,8 @@ struct ProductLaunch {
     uint64_t layout;           // their swizzle and group stride, as descriptor bits
     int32_t split;             // thread blocks of a cluster, each with a share of K
     int32_t swapped;           // 1: lanes are b's rows (d's columns)
-    int32_t dtype, vec;        // vec: rows of d take 16-byte stores
+    int32_t dtype, tma_store;  // tma_store: d's address and rows suit a tensor map
+    int32_t turns;             // epilogue warps of a quarter take turns, tile by tile
     const float *bias;
     int32_t activation;
     float alpha;
@@ -50,7 +52,7 @@ struct ProductLaunch {
 constexpr int kThreads = 384, kEpilogueWarps = 8;
 constexpr int kMaxStages = 8;
 constexpr int kAccStep = 160;  // columns between the two accumulators
-constexpr int kStagePitch = 144;  // epilogue staging row: 128 bytes and a 16-byte shift of the banks
+constexpr int kStaging = 32 * 128;  // epilogue staging of a warp: 32 rows of 128 bytes, swizzled as TMA expects
 constexpr uint32_t kTmemCols = 512, kScaleCol = 416, kScaleCols = 48;
 
 struct Control {
@@ -62,7 +64,7 @@ struct Control {
 };
 
 struct Shared {
-    alignas(128) uint8_t staging[kEpilogueWarps][32 * kStagePitch];
+    alignas(1024) uint8_t staging[kEpilogueWarps][kStaging];
     alignas(16) float bias[kEpilogueWarps][64];
     Control ctl;
 };
@@ -88,6 +90,15 @@ __device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes)
 {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, int x, int y, uint32_t src)
+{
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n\t"
+                 "cp.async.bulk.commit_group;" ::"l"(map), "r"(x), "r"(y), "r"(src)
+                 : "memory");
+}
+__device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // Codes: `layout` with the address of the first row.
 __device__ __forceinline__ uint64_t codes_desc(uint32_t addr, uint64_t layout) { return umma::desc(addr, 16, 0) | layout; }
@@ -208,27 +219,30 @@ __device__ __forceinline__ void epilogue_swapped(const ProductLaunch &p, uint32_
     }
 }
 
-// Lanes are a's rows: a warp turns 32 rows x 32 or 64 columns in shared memory and writes them row by row.
-// The two warps of a quarter take every other such column range; of 256 columns, those from `first` on come first,
-// and `part` is told when they have been read.
+// Lanes are a's rows: a warp stages 32 rows x 128 bytes (64 columns, or 32 of fp32) and writes them row by row.
+// `i0` is its first column range and `di` the distance to its next; of 256 columns, those from `first` on come
+// first, and `part` is told when they have been read.  `bias_at`: the columns that `bias` holds.
 template <int ACT>
-__device__ __forceinline__ void epilogue_rows(const ProductLaunch &p, uint32_t tmem, int lane0, int col0, int half, int first, uint32_t part,
-                                              uint8_t *mine, float *bias)
+__device__ __forceinline__ void epilogue_rows(const ProductLaunch &p, const CUtensorMap *d_map, uint32_t tmem, int lane0, int col0, int i0,
+                                              int di, int first, uint32_t part, uint8_t *mine, float *bias, int &bias_at)
 {
     const int lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) & 3;
-    const int size = p.dtype == NT_DTYPE_F32 ? 4 : 2;
-    const int width = size == 2 && p.bn % 128 == 0 ? 64 : 32;  // columns of a pass
-    for (int i0 = width * half; i0 < p.bn; i0 += 2 * width) {
-        const int c0 = p.bn > kAccStep ? i0 ^ first : i0;
-        if (p.bn > kAccStep && i0 >= 128 && i0 < 128 + 2 * width) {  // 128 columns have been read, the shared ones among them
+    const int size = p.dtype == NT_DTYPE_F32 ? 4 : 2, width = 128 / size;
+    for (; i0 < p.bn; i0 += di) {
+        const int c0 = p.bn > kAccStep ? i0 ^ first : i0, n0 = col0 + c0;
+        if (p.bn > kAccStep && i0 >= 128 && i0 < 128 + di) {  // 128 columns have been read, the shared ones among them
             umma::fence_before();
             __syncwarp();
             if (lane == 0) umma::mbar_arrive(part);
         }
-        if (col0 + c0 >= p.c_rows) continue;
-        for (int i = lane; i < width; i += 32) bias[i] = p.bias && col0 + c0 + i < p.c_rows ? __ldg(p.bias + col0 + c0 + i) : 0.f;
-        __syncwarp();
-        for (int s = 0; s < width; s += 32) {
+        if (n0 >= p.c_rows) continue;
+        if (p.bias && bias_at != n0) {
+            for (int i = lane; i < width; i += 32) bias[i] = n0 + i < p.c_rows ? __ldg(p.bias + n0 + i) : 0.f;
+            bias_at = n0;
+            __syncwarp();
+        }
+        uint8_t *const row = mine + lane * 128;
+        for (int s = 0; s < width && c0 + s < p.bn; s += 32) {
             uint32_t v[32];
             ld32(tmem + c0 + s, v);
             umma::wait_ld();
@@ -242,11 +256,14 @@ __device__ __forceinline__ void epilogue_rows(const ProductLaunch &p, uint32_t t
                 v[i + 2] = __float_as_uint(y.x);
                 v[i + 3] = __float_as_uint(y.y);
             }
-            uint8_t *row = mine + lane * kStagePitch + s * size;
+            if (s == 0) {  // the last store has read this buffer
+                if (p.tma_store && elect_one()) store_wait_read();
+                __syncwarp();
+            }
             if (size == 4) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    *reinterpret_cast<uint4 *>(row + 16 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                    *reinterpret_cast<uint4 *>(row + ((i ^ (lane & 7)) << 4)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -254,43 +271,38 @@ __device__ __forceinline__ void epilogue_rows(const ProductLaunch &p, uint32_t t
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         h[e] = pack2(p.dtype, __uint_as_float(v[8 * i + 2 * e]), __uint_as_float(v[8 * i + 2 * e + 1]));
-                    *reinterpret_cast<uint4 *>(row + 16 * i) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4 *>(row + (((s >> 3) + i ^ (lane & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
                 }
             }
         }
-        __syncwarp();
-        const int64_t m0 = lane0 + quarter * 32, n0 = col0 + c0;
-        const int rows = (int)min((int64_t)32, p.l_rows - m0);
-        uint8_t *dst = static_cast<uint8_t *>(p.d) + (m0 * p.row_stride + n0) * size;
-        if (p.vec && n0 + width <= p.c_rows) {
-            const int per_row = width * size / 16, step = 32 / per_row;  // 4 or 8 lanes a row
-            const int64_t pitch = p.row_stride * size;
-            const uint8_t *from = mine + (lane / per_row) * kStagePitch + (lane % per_row) * 16;
-            uint8_t *to = dst + (lane / per_row) * pitch + (lane % per_row) * 16;
-            for (int r = lane / per_row; r < rows; r += step, from += step * kStagePitch, to += step * pitch)
-                *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(from);
-        } else {
-            const int cols = (int)min((int64_t)width, p.c_rows - n0);
-            for (int r = 0; r < rows; ++r)
-                for (int c = lane; c < cols; c += 32) {
-                    if (size == 4)
-                        *reinterpret_cast<uint32_t *>(dst + (r * p.row_stride + c) * 4) =
-                            *reinterpret_cast<const uint32_t *>(mine + r * kStagePitch + c * 4);
-                    else
-                        *reinterpret_cast<uint16_t *>(dst + (r * p.row_stride + c) * 2) =
-                            *reinterpret_cast<const uint16_t *>(mine + r * kStagePitch + c * 2);
-                }
+        const int64_t m0 = lane0 + quarter * 32;
+        if (p.tma_store) {
+            umma::fence_async_smem();
+            __syncwarp();
+            if (m0 < p.l_rows && elect_one()) tma_store_2d(d_map, n0, (int)m0, smem_u32(mine));
+            __syncwarp();
+            continue;
         }
         __syncwarp();
+        const int rows = (int)min((int64_t)32, p.l_rows - m0), cols = min(min(width, p.bn - c0), p.c_rows - n0);
+        for (int r0 = 0; r0 < rows; r0 += 4)
+            for (int c = lane; c < cols; c += 32) {
+                uint32_t v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint8_t *from = mine + (r0 + r) * 128 + (((c * size >> 4) ^ (r0 + r & 7)) << 4) + (c * size & 15);
+                    v[r] = size == 4 ? *reinterpret_cast<const uint32_t *>(from) : *reinterpret_cast<const uint16_t *>(from);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (r0 + r >= rows) break;
+                    const int64_t at = (m0 + r0 + r) * p.row_stride + n0 + c;
+                    if (size == 4) static_cast<uint32_t *>(p.d)[at] = v[r];
+                    else static_cast<uint16_t *>(p.d)[at] = (uint16_t)v[r];
+                }
+            }
+        __syncwarp();
     }
-}
-
-template <int ACT>
-__device__ __forceinline__ void epilogue(const ProductLaunch &p, uint32_t tmem, int lane0, int col0, int half, int first, uint32_t part,
-                                         uint8_t *mine, float *bias)
-{
-    if (p.swapped) epilogue_swapped<ACT>(p, tmem, lane0, col0, half);
-    else epilogue_rows<ACT>(p, tmem, lane0, col0, half, first, part, mine, bias);
 }
 
 // The tiles of a block, `step` apart in the order lane tiles first; kept as (lane tile, column tile) without
@@ -316,7 +328,8 @@ struct Tiles {
 
 template <int BLOCK>
 __global__ void __launch_bounds__(kThreads, 1)
-    product_kernel(const __grid_constant__ CUtensorMap l_map, const __grid_constant__ CUtensorMap c_map, const ProductLaunch p)
+    product_kernel(const __grid_constant__ CUtensorMap l_map, const __grid_constant__ CUtensorMap c_map,
+                   const __grid_constant__ CUtensorMap d_map, const ProductLaunch p)
 {
     constexpr int kTiles = BLOCK == 16 ? 4 : 2;  // scale tiles of a stage
     extern __shared__ uint8_t raw[];
@@ -339,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             umma::mbar_init(acc_full + 8 * i, 1);
-            umma::mbar_init(acc_empty + 8 * i, kEpilogueWarps);
+            umma::mbar_init(acc_empty + 8 * i, p.turns ? kEpilogueWarps / 2 : kEpilogueWarps);
             umma::mbar_init(acc_part + 8 * i, kEpilogueWarps);
         }
         umma::mbar_fence_init();
@@ -420,40 +433,54 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (buf == 0) acc_phase ^= 1;
         }
     } else if (warp >= 4) {
-        int buf = 0;
-        const int half = (warp - 4) >> 2;
+        int buf = 0, bias_at = -1;
+        const int half = (warp - 4) >> 2, width = p.dtype == NT_DTYPE_F32 ? 32 : 64;
+        const int i0 = p.turns ? 0 : half * width, di = p.turns ? width : 2 * width;
         uint8_t *const mine = sh.staging[warp - 4];
         float *const bias = sh.bias[warp - 4];
+        bias[lane] = bias[lane + 32] = 0.f;
+        __syncwarp();
         uint32_t acc_phase = 0;
         for (Tiles t(p); t.valid(); t.next()) {
-            if (!__all_sync(0xffffffffu, wait(acc_full + 8 * buf, acc_phase))) break;
-            umma::fence_after();
-            const uint32_t acc = tmem + buf * kAccStep + ((uint32_t)(warp & 3) << 21);
-            const int lane0 = t.l * 128, col0 = t.c * p.bn, shared_first = buf ? 0 : 128;
-            if (p.split > 1) {  // partial sums [column][lane], a lane a bank
-                float *dump = reinterpret_cast<float *>(stages) + (threadIdx.x & 127);
-                for (int c0 = 32 * half; c0 < p.bn; c0 += 64) {
-                    uint32_t v[32];
-                    ld32(acc + c0, v);
-                    umma::wait_ld();
+            const uint32_t acc = tmem + buf * kAccStep + ((uint32_t)(warp & 3) << 21), part = acc_part + 8 * buf;
+            const int lane0 = t.l * 128, col0 = t.c * p.bn, first = buf ? 0 : 128;
+            if (!p.turns || buf == half) {
+                if (!__all_sync(0xffffffffu, wait(acc_full + 8 * buf, acc_phase))) break;
+                umma::fence_after();
+                if (p.split > 1) {  // partial sums [column][lane], a lane a bank
+                    float *dump = reinterpret_cast<float *>(stages) + (threadIdx.x & 127);
+                    for (int c0 = 32 * half; c0 < p.bn; c0 += 64) {
+                        uint32_t v[32];
+                        ld32(acc + c0, v);
+                        umma::wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (c0 + i < p.bn) dump[(c0 + i) * 129] = __uint_as_float(v[i]);
+                        for (int i = 0; i < 32; ++i)
+                            if (c0 + i < p.bn) dump[(c0 + i) * 129] = __uint_as_float(v[i]);
+                    }
+                } else if (p.swapped) {
+                    switch (p.activation) {
+                    case NT_ACT_RELU: epilogue_swapped<NT_ACT_RELU>(p, acc, lane0, col0, half); break;
+                    case NT_ACT_SILU: epilogue_swapped<NT_ACT_SILU>(p, acc, lane0, col0, half); break;
+                    case NT_ACT_GELU: epilogue_swapped<NT_ACT_GELU>(p, acc, lane0, col0, half); break;
+                    default: epilogue_swapped<NT_ACT_NONE>(p, acc, lane0, col0, half); break;
+                    }
+                } else {
+                    switch (p.activation) {
+                    case NT_ACT_RELU: epilogue_rows<NT_ACT_RELU>(p, &d_map, acc, lane0, col0, i0, di, first, part, mine, bias, bias_at); break;
+                    case NT_ACT_SILU: epilogue_rows<NT_ACT_SILU>(p, &d_map, acc, lane0, col0, i0, di, first, part, mine, bias, bias_at); break;
+                    case NT_ACT_GELU: epilogue_rows<NT_ACT_GELU>(p, &d_map, acc, lane0, col0, i0, di, first, part, mine, bias, bias_at); break;
+                    default: epilogue_rows<NT_ACT_NONE>(p, &d_map, acc, lane0, col0, i0, di, first, part, mine, bias, bias_at); break;
+                    }
                 }
-            } else {
-                switch (p.activation) {
-                case NT_ACT_RELU: epilogue<NT_ACT_RELU>(p, acc, lane0, col0, half, shared_first, acc_part + 8 * buf, mine, bias); break;
-                case NT_ACT_SILU: epilogue<NT_ACT_SILU>(p, acc, lane0, col0, half, shared_first, acc_part + 8 * buf, mine, bias); break;
-                case NT_ACT_GELU: epilogue<NT_ACT_GELU>(p, acc, lane0, col0, half, shared_first, acc_part + 8 * buf, mine, bias); break;
-                default: epilogue<NT_ACT_NONE>(p, acc, lane0, col0, half, shared_first, acc_part + 8 * buf, mine, bias); break;
-                }
+                umma::fence_before();
+                __syncwarp();
+                if (lane == 0) umma::mbar_arrive(acc_empty + 8 * buf);
             }
-            umma::fence_before();
-            __syncwarp();
-            if (lane == 0) umma::mbar_arrive(acc_empty + 8 * buf);
             buf ^= 1;
             if (buf == 0) acc_phase ^= 1;
         }
+        if (p.tma_store && elect_one()) store_wait();
+        __syncwarp();
     }
     __syncwarp();  // the single lanes of warps 0 and 1 rejoin the others
     if (p.split > 1) {
@@ -497,6 +524,19 @@ EncodeTiled encode_tiled()
         return reinterpret_cast<EncodeTiled>(f);
     }();
     return fn;
+}
+
+// d, written in boxes of 32 rows x 128 bytes.
+bool encode_output(CUtensorMap *map, const ProductLaunch &p)
+{
+    const EncodeTiled encode = encode_tiled();
+    if (!encode) return false;
+    const int size = p.dtype == NT_DTYPE_F32 ? 4 : 2;
+    const cuuint64_t shape[2] = {(cuuint64_t)p.c_rows, (cuuint64_t)p.l_rows}, stride[1] = {(cuuint64_t)p.row_stride * size};
+    const cuuint32_t box[2] = {128u / size, 32}, step[2] = {1, 1};
+    return encode(map, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.d, shape, stride, box, step,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Codes as a byte matrix, read in boxes of `box_rows` rows x `row_bytes`.
@@ -549,14 +589,17 @@ nt_status launch_product(const NtMx4Matrix *a, const NtMx4Matrix *b, ProductLaun
     // split K while blocks stand idle and every share keeps two stages
     p.split = 1;
     while (p.split < 8 && p.bn <= 128 && tiles * p.split * 2 <= sms && k_stages >= p.split * 4) p.split *= 2;
+    p.turns = !p.swapped && p.split == 1 && p.bn <= 64;
     p.stage_bytes = (int32_t)ceil_div((128 + p.bn) * p.row_bytes + (p.bn > 128 ? 3 : 2) * kTiles * kTileBytes, 1024) * 1024;
     const int room = 227 * 1024 - 1024 - (int)sizeof(Shared);
     p.stages = std::min(kMaxStages, room / p.stage_bytes);
     const size_t smem = 1024 + std::max((size_t)p.stages * p.stage_bytes, p.split > 1 ? (size_t)p.bn * 129 * 4 : 0);
     const int64_t grid = p.split > 1 ? tiles * p.split : std::min<int64_t>(tiles, sms);
-    CUtensorMap l_map, c_map;
+    CUtensorMap l_map, c_map, d_map = {};
     if (!encode_codes(&l_map, l, 128, p.row_bytes) || !encode_codes(&c_map, c, p.bn, p.row_bytes))
         return set_error(NT_ERR_CUDA, "4-bit product: the tensor maps could not be encoded");
+    // d by TMA where 16-byte rows allow it, and 64 columns of a tile fill a row of the staging
+    p.tma_store = p.tma_store && !p.swapped && p.split == 1 && (p.bn >= 64 || p.dtype == NT_DTYPE_F32) && encode_output(&d_map, p);
     const void *kernel = reinterpret_cast<const void *>(&product_kernel<BLOCK>);
     cudaError_t e = set_smem_limit(kernel, 227 * 1024 - sizeof(Shared));
     if (e == cudaSuccess) {
@@ -571,7 +614,7 @@ nt_status launch_product(const NtMx4Matrix *a, const NtMx4Matrix *b, ProductLaun
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        e = cudaLaunchKernelEx(&cfg, product_kernel<BLOCK>, l_map, c_map, p);
+        e = cudaLaunchKernelEx(&cfg, product_kernel<BLOCK>, l_map, c_map, d_map, p);
     }
     if (e != cudaSuccess) return set_error(NT_ERR_CUDA, "4-bit product: %s", cudaGetErrorString(e));
     count_launch();
@@ -618,7 +661,7 @@ extern "C" nt_status nt_mx4_product(const NtMx4Matrix *a, const NtMx4Matrix *b, 
     p.d = d;
     p.dtype = dtype;
     p.row_stride = row_stride;
-    p.vec = is_aligned(d, 16) && row_stride * size % 16 == 0;
+    p.tma_store = is_aligned(d, 16) && row_stride * size % 16 == 0 && row_stride * size < (int64_t)1 << 40;
     return a->block == 16 ? mx4::launch_product<16>(a, b, p, (cudaStream_t)stream)
                           : mx4::launch_product<32>(a, b, p, (cudaStream_t)stream);
 }
