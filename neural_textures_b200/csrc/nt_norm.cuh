@@ -12,7 +12,7 @@
 // flight while it computes and no barrier is needed.  The slots hold a ring of a few vectors and, as far as
 // they go, the texels read first, for the second pass; that one begins with the texels read last, which
 // are still in L2.
-// Blocks of an image meet in a cluster (up to 8), where they read each other's sums from shared memory, or,
+// Blocks of an image meet in a cluster (up to 16), where they read each other's sums from shared memory, or,
 // for large maps, at a barrier of the whole cooperative grid, with the sums in the workspace.
 // All sums are joined in a fixed order.
 #pragma once
@@ -25,7 +25,7 @@ namespace norm {
 constexpr int kForwardThreads = 512;
 constexpr int kForwardRing = 4, kBackwardRing = 4;  // 64 and 96 KB in flight on an SM cover the latency of HBM
 constexpr int kBackwardThreads = 384;  // 84 registers a thread with two blocks on an SM: 64 spill
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 16;
 constexpr int kMaxSplits = 320;  // thread blocks of an image
 constexpr uint32_t kSpinLimit = 1u << 24;
 
@@ -182,6 +182,8 @@ __device__ __forceinline__ float2 peer_f2(const float2 *mine, uint32_t rank)
     asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(remote) : "memory");
     return v;
 }
+
+__device__ __forceinline__ void prefetch(const void *p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
 
 // All blocks of a cooperative launch; *counter is zero before it.
 __device__ __forceinline__ void grid_sync(unsigned int *counter, unsigned int *status)
@@ -506,6 +508,10 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
         const int vec = v0 + col;
         if (vec >= L.vectors || row >= L.ty) continue;
         const int near = min(max(L.keep - slot0, 0), mine);
+        if (!BACKWARD) {  // the second pass wants them soon
+            if (p.gamma) prefetch(p.gamma + vec * V);
+            if (p.beta) prefetch(p.beta + vec * V);
+        }
         switch (BACKWARD ? p.activation : NT_ACT_NONE) {
         case NT_ACT_RELU: th.template first<NT_ACT_RELU>(vec * V, mine, near, slot0); break;
         case NT_ACT_SILU: th.template first<NT_ACT_SILU>(vec * V, mine, near, slot0); break;
@@ -516,6 +522,14 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
     __syncthreads();
 
     // ---- the block's sums, per group (and per channel) ----
+    auto finish = [&](int g, float mean, float squares) {
+        const float rstd = 1.f / sqrtf(squares * L.inv_count + p.epsilon);
+        stat[g] = make_float2(mean, rstd);
+        if (split == 0) {
+            if (p.mean) p.mean[n * p.groups + g] = mean;
+            if (p.rstd) p.rstd[n * p.groups + g] = rstd;
+        }
+    };
     float2 *const shared_out = L.cluster ? part : nullptr;
     const int parts = p.images * L.splits;
     if constexpr (!BACKWARD) {
@@ -537,7 +551,8 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
             }
             sum = warp_sum_all(sum);
             if (lane == 0) {
-                if (shared_out) shared_out[g] = make_float2(mean, sum);
+                if (L.splits == 1) finish(g, mean, sum);
+                else if (shared_out) shared_out[g] = make_float2(mean, sum);
                 else L.groups_part[(n * p.groups + g) * L.splits + split] = make_float2(mean, sum);
             }
         }
@@ -564,7 +579,8 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
             }
             s = warp_sum(s);
             if (lane == 0) {
-                if (shared_out) shared_out[g] = s;
+                if (L.splits == 1) stat[g] = s;
+                else if (shared_out) shared_out[g] = s;
                 else L.groups_part[(n * p.groups + g) * L.splits + split] = s;
             }
         }
@@ -574,14 +590,14 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
     else __syncthreads();
 
     // ---- the image's sums ----
-    for (int g = warp; g < p.groups; g += kWarps) {
+    for (int g = warp; g < p.groups && L.splits > 1; g += kWarps) {
         float2 v[kMaxSplits / 32];
 #pragma unroll
         for (int k = 0; k < kMaxSplits / 32; ++k) {
             const int i = lane + 32 * k;
             v[k] = make_float2(0.f, 0.f);
             if (i < L.splits)
-                v[k] = L.cluster ? (L.splits > 1 ? peer_f2(part + g, i) : part[g])
+                v[k] = L.cluster ? peer_f2(part + g, i)
                                  : __ldcg(L.groups_part + (n * p.groups + g) * L.splits + i);
         }
         float a = 0.f, b = 0.f;
@@ -602,14 +618,7 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
                 if (lane + 32 * k < L.splits)
                     b += fmaf((float)(share + (lane + 32 * k < extra)) * L.per * (v[k].x - mean), v[k].x - mean, v[k].y);
             b = warp_sum_all(b);
-            if (lane == 0) {
-                const float rstd = 1.f / sqrtf(b * L.inv_count + p.epsilon);
-                stat[g] = make_float2(mean, rstd);
-                if (split == 0) {
-                    if (p.mean) p.mean[n * p.groups + g] = mean;
-                    if (p.rstd) p.rstd[n * p.groups + g] = rstd;
-                }
-            }
+            if (lane == 0) finish(g, mean, b);
         }
     }
     if (BACKWARD && L.cluster && p.images == 1 && (p.dgamma || p.dbeta))
@@ -627,7 +636,7 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
             if (p.dgamma) p.dgamma[c] = s.y;
         }
     if (L.cluster && L.splits > 1) cluster_sync();  // a block's sums stay until its peers have read them
-    else __syncthreads();
+    else if (L.splits > 1) __syncthreads();
     if (BACKWARD && !L.cluster && (p.dgamma || p.dbeta))
         for (int64_t c = (int64_t)warp * gridDim.x + blockIdx.x; c < p.channels; c += (int64_t)kWarps * gridDim.x) join_channel(L, (int)c);
 
