@@ -100,6 +100,8 @@ cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
     L.cluster = pl.cluster;
     const bool even = flat(p->x, p, size) && flat(backward ? p->dy : p->y, p, size) && flat(backward ? p->dx : p->y, p, size);
     L.texels = p->height * p->width;
+    L.share = L.texels / L.splits;
+    L.extra = L.texels % L.splits;
     L.inv_count = 1.f / ((float)L.texels * (float)L.per);
     L.barrier = reinterpret_cast<unsigned int *>(ws);
     L.groups_part = reinterpret_cast<float2 *>(ws + at.groups_at);
@@ -128,6 +130,12 @@ cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
         if (smem <= most || v == 1) break;
     }
 
+    L.turns = L.share / L.ty;
+    L.left = L.share % L.ty;
+    L.by_tx = (uint32_t)ceil_div(1 << 18, L.tx);
+    const int units = whole ? L.per / v : L.per;
+    L.by_group = units == 1 ? 0 : (uint32_t)ceil_div((int64_t)1 << 32, units);
+
     const NormKernel kernel = backward ? backward_kernel(p->dtype, v, whole, even) : forward_kernel(p->dtype, v, whole, even);
     cudaError_t e = set_smem_limit(reinterpret_cast<const void *>(kernel), 227 * 1024 - 1024);
     if (e != cudaSuccess) return e;
@@ -137,7 +145,7 @@ cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((int64_t)p->images * pl.splits));
+    cfg.gridDim = dim3((unsigned)pl.splits, (unsigned)p->images);
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;

@@ -38,6 +38,10 @@ struct NormLaunch {
     int32_t cluster;    // 1: they form a cluster; 0: the grid meets at *barrier
     int32_t texels, vectors;  // vectors of V channels in a texel
     int32_t tx, ty;     // threads along channels and texels
+    int32_t share, extra;   // texels of a block: share, the first `extra` blocks one more
+    int32_t turns, left;    // share / ty and its remainder
+    uint32_t by_tx;         // ceil(2^18 / tx): thread / tx without a division
+    uint32_t by_group;      // ceil(2^32 / (units of a group)), 0 for one; a unit is a vector, or a channel where vectors cross groups
     int32_t keep;       // vectors of a thread (of x, and of dy) that stay in shared memory, in front of its ring
     int32_t scratch;    // bytes of shared memory in front of them
     float inv_count;    // 1 / values of a group
@@ -193,11 +197,12 @@ __device__ __forceinline__ void grid_sync(unsigned int *counter, unsigned int *s
         __threadfence();
         atomicAdd(counter, 1u);
         uint32_t seen = 0;
+        const uint32_t blocks = gridDim.x * gridDim.y;
         for (uint32_t i = 0; i < kSpinLimit; ++i) {
             asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(counter) : "memory");
-            if (seen >= gridDim.x) break;
+            if (seen >= blocks) break;
         }
-        if (seen < gridDim.x) atomicOr(status, 1u);
+        if (seen < blocks) atomicOr(status, 1u);
     }
     __syncthreads();
 }
@@ -253,12 +258,25 @@ struct Threads {
     // Per-channel values of a parameter, in pairs.
     __device__ __forceinline__ void channels(const float *param, float other, int c, float2 (&v)[P]) const
     {
+        if (param && V >= 4 && (reinterpret_cast<uintptr_t>(param) & 15) == 0) {
+#pragma unroll
+            for (int j = 0; j < P; j += 2) {
+                const float4 q = __ldg(reinterpret_cast<const float4 *>(param + c) + j / 2);
+                v[j] = make_float2(q.x, q.y);
+                if (j + 1 < P) v[j + 1] = make_float2(q.z, q.w);
+            }
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < P; ++j)
             v[j] = make_float2(param ? __ldg(param + c + 2 * j) : other, V > 1 && param ? __ldg(param + c + 2 * j + 1) : other);
     }
     // Group of channel c + i (of the whole vector, when it lies in one).
-    __device__ __forceinline__ int group(int c, int i) const { return (c + (WHOLE || i >= V ? 0 : i)) / L.per; }
+    __device__ __forceinline__ int group(int c, int i) const
+    {
+        const uint32_t unit = WHOLE ? (uint32_t)c / V : (uint32_t)(c + (i >= V ? 0 : i));
+        return (int)(L.by_group ? __umulhi(unit, L.by_group) : unit);
+    }
 
     // The slots of this thread: kept vectors, then a ring of kDepth (a power of two).  In the backward pass a
     // slot holds x and, kNext bytes on, dy.
@@ -489,15 +507,15 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
     extern __shared__ __align__(16) uint8_t smem[];
     const NtGroupNorm &p = L.p;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t n = blockIdx.x / L.splits;
-    const int split = blockIdx.x % L.splits;
-    // texels of a block: an equal share, the first blocks one more
-    const int share = L.texels / L.splits, extra = L.texels - share * L.splits;
+    const int64_t n = blockIdx.y;
+    const int split = blockIdx.x;
+    const int share = L.share, extra = L.extra;
     const int lo = split * share + min(split, extra), hi = lo + share + (split < extra);
     // shared memory: group results [groups], group partials [groups], scratch, kept vectors
     float2 *stat = reinterpret_cast<float2 *>(smem), *part = stat + p.groups, *scratch = part + p.groups;
-    const int row = tid / L.tx, col = tid % L.tx;
-    const int turn = (hi - lo) / L.ty, left = hi - lo - turn * L.ty;
+    const int row = (int)(tid * L.by_tx >> 18), col = tid - row * L.tx;
+    int turn = L.turns, left = L.left + (split < extra);
+    if (left == L.ty) ++turn, left = 0;
     const int mine = row < L.ty ? turn + (row < left) : 0;  // texels of this thread
     const int most = turn + (left > 0);                     // and of any
     const Threads<T, V, WHOLE, FLAT, BACKWARD> th = {L,    n,       lo, row, col, mine,
@@ -523,7 +541,7 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
 
     // ---- the block's sums, per group (and per channel) ----
     auto finish = [&](int g, float mean, float squares) {
-        const float rstd = 1.f / sqrtf(squares * L.inv_count + p.epsilon);
+        const float rstd = rsqrtf(fmaf(squares, L.inv_count, p.epsilon));
         stat[g] = make_float2(mean, rstd);
         if (split == 0) {
             if (p.mean) p.mean[n * p.groups + g] = mean;
@@ -543,7 +561,7 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
                 const int r = entries == 1 ? e : e / entries;
                 shift = fmaf((float)(turn + (r < left)) * step, of[r * (width - entries) + e].x - origin, shift);
             }
-            const float mean = origin + warp_sum_all(shift) / ((float)(hi - lo) * L.per);
+            const float mean = origin + __fdividef(warp_sum_all(shift), (float)(hi - lo) * L.per);
             for (int e = lane; e < L.ty * entries; e += 32) {
                 const int r = entries == 1 ? e : e / entries;
                 const float2 v = of[r * (width - entries) + e];
@@ -568,7 +586,7 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
             __syncthreads();
         }
         if ((p.dgamma || p.dbeta) && (p.images > 1 || !L.cluster))
-            for (int c = tid; c < p.channels; c += NT) L.channels_part[(int64_t)c * parts + blockIdx.x] = scratch[c];
+            for (int c = tid; c < p.channels; c += NT) L.channels_part[(int64_t)c * parts + blockIdx.y * L.splits + blockIdx.x] = scratch[c];
         for (int g = warp; g < p.groups; g += kWarps) {
             float2 s = make_float2(0.f, 0.f);
             for (int e = lane; e < L.per; e += 32) {
@@ -612,7 +630,7 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
 #pragma unroll
             for (int k = 0; k < kMaxSplits / 32; ++k)
                 if (lane + 32 * k < L.splits) a = fmaf((float)(share + (lane + 32 * k < extra)), v[k].x - origin, a);
-            const float mean = origin + warp_sum_all(a) / (float)L.texels;
+            const float mean = origin + __fdividef(warp_sum_all(a), (float)L.texels);
 #pragma unroll
             for (int k = 0; k < kMaxSplits / 32; ++k)
                 if (lane + 32 * k < L.splits)
@@ -638,7 +656,7 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
     if (L.cluster && L.splits > 1) cluster_sync();  // a block's sums stay until its peers have read them
     else if (L.splits > 1) __syncthreads();
     if (BACKWARD && !L.cluster && (p.dgamma || p.dbeta))
-        for (int64_t c = (int64_t)warp * gridDim.x + blockIdx.x; c < p.channels; c += (int64_t)kWarps * gridDim.x) join_channel(L, (int)c);
+        for (int c = warp * parts + blockIdx.y * L.splits + blockIdx.x; c < p.channels; c += kWarps * parts) join_channel(L, c);
 
     for (int v0 = (L.vectors - 1) / L.tx * L.tx; v0 >= 0; v0 -= L.tx) {
         slot0 -= most;
