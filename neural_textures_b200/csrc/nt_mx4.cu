@@ -16,12 +16,17 @@ struct QuantizeLaunch {
     int32_t rows, cols, tiles, groups;  // scale tiles a row of tiles; column groups
 };
 
+// How a row's values are read: 16 bytes at a time, through shared memory (rows that are not aligned: a warp reads
+// 32 consecutive values of a row at a time), or one by one at any stride.
+enum Access { kVector, kStaged, kStrided };
+constexpr int kStagePitch = kGroupCols + 4;
+
 // 16 values of a row from column c (0 past the matrix).
-template <class T, bool VEC>
+template <class T, Access ACCESS>
 __device__ __forceinline__ void load16(const QuantizeLaunch &p, int64_t row, int64_t c, T (&v)[16])
 {
     const T *src = static_cast<const T *>(p.src) + row * p.row_stride;
-    if (VEC && row < p.rows && c + 16 <= p.cols) {
+    if (ACCESS == kVector && row < p.rows && c + 16 <= p.cols) {
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T); ++i)
             reinterpret_cast<uint4 *>(v)[i] = __ldg(reinterpret_cast<const uint4 *>(src + c) + i);
@@ -60,9 +65,10 @@ __device__ __forceinline__ void quantize_codes(const T (&v)[N], uint32_t byte, u
 // Rows along the memory.  A thread block takes 128 rows x 128 columns.  BLOCK / 4 lanes share a row
 // (16 values each), so that they hold the four scales of one word; a lane takes rows r, r + 32,
 // r + 64 and r + 96, whose words are the 16 bytes of row r in the scale tile: one store.
-template <class T, int BLOCK, bool VEC>
+template <class T, int BLOCK, Access ACCESS>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeLaunch p)
 {
+    __shared__ T stage[ACCESS == kStaged ? 32 * kStagePitch : 1];
     constexpr int LPR = BLOCK / 4, RPW = 32 / LPR;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t tile = blockIdx.x / p.groups;
@@ -71,12 +77,28 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeL
     const int residue = (BLOCK == 16 ? warp & 3 : warp) * RPW + lane / LPR;
     const int64_t c = (int64_t)group * kGroupCols + half * 64 + (lane % LPR) * 16;
     uint32_t words[4];
-    constexpr int U = sizeof(T) == 2 ? 4 : 2;  // rows in flight
+    constexpr int U = ACCESS == kStaged ? 1 : sizeof(T) == 2 ? 4 : 2;  // rows in flight
 #pragma unroll
     for (int j0 = 0; j0 < 4; j0 += U) {
         alignas(16) T v[U][16];
 #pragma unroll
-        for (int u = 0; u < U; ++u) load16<T, VEC>(p, tile * kTileRows + (j0 + u) * 32 + residue, c, v[u]);
+        for (int u = 0; u < U; ++u)
+            if (ACCESS != kStaged) load16<T, ACCESS>(p, tile * kTileRows + (j0 + u) * 32 + residue, c, v[u]);
+        if (ACCESS == kStaged) {
+            const int64_t row0 = tile * kTileRows + j0 * 32 + warp * 4, col0 = (int64_t)group * kGroupCols + lane;
+            T w[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const bool in = row0 + i / 4 < p.rows && col0 + i % 4 * 32 < p.cols;
+                w[i] = in ? static_cast<const T *>(p.src)[(row0 + i / 4) * p.row_stride + col0 + i % 4 * 32] : from_f32<T>(0.f);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) stage[(warp * 4 + i / 4) * kStagePitch + i % 4 * 32 + lane] = w[i];
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[0][i] = stage[residue * kStagePitch + (int)(c - (int64_t)group * kGroupCols) + i];
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t row = tile * kTileRows + (j0 + u) * 32 + residue;
@@ -100,48 +122,41 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeL
 }
 
 // Columns along the memory (a transposed matrix): lane = row, so that a warp's load of one column is
-// contiguous; a thread quantises 64 columns of its row, 32 bytes of codes, without any exchange.
+// contiguous; a thread quantises 32 columns of its row, 16 bytes of codes, without any exchange.
+constexpr int kColumnsGroup = 64;  // columns of a thread block
+
 template <class T, int BLOCK>
 __global__ void __launch_bounds__(kThreads) quantize_columns_kernel(const QuantizeLaunch p)
 {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t tile = blockIdx.x / p.groups;
     const int group = blockIdx.x % p.groups;
-    const int j = warp & 3, half = warp >> 2;
+    const int j = warp & 3;
     const int64_t row = tile * kTileRows + j * 32 + lane;
-    const int64_t c0 = (int64_t)group * kGroupCols + half * 64;
+    const int64_t c0 = (int64_t)group * kColumnsGroup + (warp >> 2) * 32;
     const T *src = static_cast<const T *>(p.src) + row;
-    uint32_t word = 0;
+    T v[32];
 #pragma unroll
-    for (int b = 0; b < 64 / 32; ++b) {
-        T v[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const int64_t c = c0 + 32 * b + i;
-            v[i] = row < p.rows && c < p.cols ? src[c * p.col_stride] : from_f32<T>(0.f);
-        }
-        uint32_t codes[4];
-        if (BLOCK == 32) {
-            const uint32_t byte = scale_byte<32>(amax_bits(v));
-            quantize_codes<T, 32>(v, byte, codes);
-            word |= byte << (8 * b);
-        } else {
-            T(&lo)[16] = *reinterpret_cast<T(*)[16]>(&v[0]);
-            T(&hi)[16] = *reinterpret_cast<T(*)[16]>(&v[16]);
-            const uint32_t b0 = scale_byte<16>(amax_bits(lo)), b1 = scale_byte<16>(amax_bits(hi));
-            quantize_codes<T, 16>(lo, b0, *reinterpret_cast<uint32_t(*)[2]>(&codes[0]));
-            quantize_codes<T, 16>(hi, b1, *reinterpret_cast<uint32_t(*)[2]>(&codes[2]));
-            word |= (b0 | b1 << 8) << (16 * b);
-        }
-        const int64_t c = c0 + 32 * b;
-        if (row < p.rows && c < row_pitch(p.cols) * 2)
-            *reinterpret_cast<uint4 *>(p.data + row * p.pitch + (c >> 1)) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+    for (int i = 0; i < 32; ++i) v[i] = row < p.rows && c0 + i < p.cols ? src[(c0 + i) * p.col_stride] : from_f32<T>(0.f);
+    uint32_t codes[4], bytes;
+    if (BLOCK == 32) {
+        bytes = scale_byte<32>(amax_bits(v));
+        quantize_codes<T, 32>(v, bytes, codes);
+    } else {
+        T(&lo)[16] = *reinterpret_cast<T(*)[16]>(&v[0]);
+        T(&hi)[16] = *reinterpret_cast<T(*)[16]>(&v[16]);
+        const uint32_t b0 = scale_byte<16>(amax_bits(lo)), b1 = scale_byte<16>(amax_bits(hi));
+        quantize_codes<T, 16>(lo, b0, *reinterpret_cast<uint32_t(*)[2]>(&codes[0]));
+        quantize_codes<T, 16>(hi, b1, *reinterpret_cast<uint32_t(*)[2]>(&codes[2]));
+        bytes = b0 | b1 << 8;
     }
-    const int tcol = BLOCK == 16 ? group * 2 + half : group;
-    if (tcol < p.tiles) {
-        uint8_t *at = p.scales + (tile * p.tiles + tcol) * kTileBytes + lane * 16 + j * 4;
-        if (BLOCK == 16) *reinterpret_cast<uint32_t *>(at) = word;
-        else *reinterpret_cast<uint16_t *>(at + 2 * half) = (uint16_t)word;
+    if (row < p.rows && c0 < row_pitch(p.cols) * 2)
+        *reinterpret_cast<uint4 *>(p.data + row * p.pitch + (c0 >> 1)) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+    const int k = (int)(c0 / BLOCK);  // first block
+    if ((k >> 2) < p.tiles) {
+        uint8_t *at = p.scales + (tile * p.tiles + (k >> 2)) * kTileBytes + lane * 16 + j * 4 + (k & 3);
+        if (BLOCK == 16) *reinterpret_cast<uint16_t *>(at) = (uint16_t)bytes;
+        else *at = (uint8_t)bytes;
     }
 }
 
@@ -149,13 +164,17 @@ template <class T, int BLOCK>
 cudaError_t launch_quantize(QuantizeLaunch p, cudaStream_t st)
 {
     p.tiles = tiles_per_row(p.cols, BLOCK);
-    p.groups = (int32_t)(((int64_t)p.cols + kGroupCols - 1) / kGroupCols);
+    const bool unit = p.col_stride == 1 || p.cols == 1, columns = !unit && p.row_stride == 1;
+    // a scale tile's padding is written too: whole tiles of 4 blocks
+    const int64_t width = columns ? kColumnsGroup : kGroupCols;
+    p.groups = (int32_t)(((int64_t)p.tiles * 4 * BLOCK + width - 1) / width);
     const int64_t blocks = ((int64_t)p.rows + kTileRows - 1) / kTileRows * p.groups;
     if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    const bool vec = p.col_stride == 1 && is_aligned(p.src, 16) && p.row_stride * sizeof(T) % 16 == 0;
-    if (vec) quantize_rows_kernel<T, BLOCK, true><<<(unsigned)blocks, kThreads, 0, st>>>(p);
-    else if (p.row_stride == 1 && p.col_stride != 1) quantize_columns_kernel<T, BLOCK><<<(unsigned)blocks, kThreads, 0, st>>>(p);
-    else quantize_rows_kernel<T, BLOCK, false><<<(unsigned)blocks, kThreads, 0, st>>>(p);
+    const bool vec = unit && is_aligned(p.src, 16) && (p.rows == 1 || p.row_stride * sizeof(T) % 16 == 0);
+    if (columns) quantize_columns_kernel<T, BLOCK><<<(unsigned)blocks, kThreads, 0, st>>>(p);
+    else if (vec) quantize_rows_kernel<T, BLOCK, kVector><<<(unsigned)blocks, kThreads, 0, st>>>(p);
+    else if (unit) quantize_rows_kernel<T, BLOCK, kStaged><<<(unsigned)blocks, kThreads, 0, st>>>(p);
+    else quantize_rows_kernel<T, BLOCK, kStrided><<<(unsigned)blocks, kThreads, 0, st>>>(p);
     count_launch();
     return cudaGetLastError();
 }
@@ -184,12 +203,15 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const DequantizeLa
     const int64_t row0 =
         (int64_t)(blockIdx.x / p.col_blocks) * rows_per_pass * kDequantRows + (threadIdx.x >> p.lanes_log2);
     const int64_t c = ((int64_t)(blockIdx.x % p.col_blocks) * lanes + sub) * 8;
-    if (c >= p.cols) return;
+    __shared__ alignas(16) T turn[kThreads / 32][256];
+    const bool in = c < p.cols;  // every lane of a warp stays for its exchange
     uint32_t codes[kDequantRows], bytes[kDequantRows];
 #pragma unroll
     for (int j = 0; j < kDequantRows; ++j) {
         const int64_t row = row0 + (int64_t)j * rows_per_pass;
         if (row >= p.rows) break;
+        codes[j] = bytes[j] = 0;
+        if (!in) continue;
         codes[j] = __ldg(reinterpret_cast<const uint32_t *>(p.data + row * p.pitch + (c >> 1)));
         bytes[j] = __ldg(p.scales + scale_at(row, (int)(c / BLOCK), p.tiles));
     }
@@ -208,7 +230,19 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const DequantizeLa
             out[2 * i + 1] = from_f32<T>(f.y * s);
         }
         T *dst = static_cast<T *>(p.dst) + row * p.row_stride + c;
-        if (p.vec && c + 8 <= p.cols) {
+        if (!p.vec && lanes == 32) {  // unaligned rows: a warp's 256 values through shared memory, 32 consecutive ones at a time
+            T *const mine = turn[threadIdx.x >> 5];
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+                reinterpret_cast<uint4 *>(mine + 8 * sub)[i] = reinterpret_cast<const uint4 *>(out)[i];
+            __syncwarp();
+            T *const first = dst - 8 * sub;
+            const int64_t left = p.cols - (c - 8 * sub);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (32 * i + sub < left) first[32 * i + sub] = mine[32 * i + sub];
+        } else if (p.vec && c + 8 <= p.cols) {
 #pragma unroll
             for (int i = 0; i < (int)sizeof(T) / 2; ++i)
                 reinterpret_cast<uint4 *>(dst)[i] = reinterpret_cast<const uint4 *>(out)[i];
