@@ -39,14 +39,29 @@ __device__ __forceinline__ void load16(const QuantizeLaunch &p, int64_t row, int
     }
 }
 
-// The bits of max |v| as fp32; NaN and infinity compare above every number as integers.
+// Larger magnitudes of two packed 16-bit values, as fp16 / bf16 bits without signs.  As integers NaN and
+// infinity compare above every number.
+__device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t v) { return __vmaxu2(m, v & 0x7fff7fffu); }
+template <class T>
+__device__ __forceinline__ uint32_t f32_bits(uint32_t v)  // of one 16-bit value
+{
+    return __float_as_uint(to_f32(*reinterpret_cast<const T *>(&v)));
+}
+
+// The bits of max |v| as fp32.
 template <class T, int N>
 __device__ __forceinline__ uint32_t amax_bits(const T (&v)[N])
 {
     uint32_t m = 0;
+    if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) m = max(m, __float_as_uint(to_f32(v[i])) & 0x7fffffffu);
-    return m;
+        for (int i = 0; i < N / 2; ++i) m = max_abs2(m, reinterpret_cast<const uint32_t *>(v)[i]);
+        return f32_bits<T>(max(m & 0xffffu, m >> 16));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+        return m;
+    }
 }
 
 template <class T, int BLOCK, int N>
@@ -57,7 +72,11 @@ __device__ __forceinline__ void quantize_codes(const T (&v)[N], uint32_t byte, u
     for (int q = 0; q < N / 8; ++q) {
         float f[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = scaled<BLOCK, sizeof(T) == 4>(to_f32(v[8 * q + i]), inv, s);
+        for (int i = 0; i < 8; i += 2) {
+            const float2 y = scaled2<BLOCK, sizeof(T) == 4>(make_float2(to_f32(v[8 * q + i]), to_f32(v[8 * q + i + 1])), inv, s);
+            f[i] = y.x;
+            f[i + 1] = y.y;
+        }
         codes[q] = codes8(f);
     }
 }
@@ -121,30 +140,21 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeL
             make_uint4(words[0], words[1], words[2], words[3]);
 }
 
-// Columns along the memory (a transposed matrix): lane = row, so that a warp's load of one column is
-// contiguous; a thread quantises 32 columns of its row, 16 bytes of codes, without any exchange.
-constexpr int kColumnsGroup = 64;  // columns of a thread block
+// Columns along the memory (a transposed matrix): lanes along the rows, so that a warp's load of one column is
+// contiguous; a thread quantises 32 columns of its row, 16 bytes of codes, without any exchange.  PAIRS: of two
+// neighbouring rows of a 16-bit matrix, for loads of 4 bytes.
+constexpr int kColumnsGroup = 64;  // columns of a thread block, twice that for pairs
 
 template <class T, int BLOCK>
-__global__ void __launch_bounds__(kThreads) quantize_columns_kernel(const QuantizeLaunch p)
+__device__ __forceinline__ void quantize_column_run(const QuantizeLaunch &p, const T (&v)[32], int64_t row, int64_t c0)
 {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t tile = blockIdx.x / p.groups;
-    const int group = blockIdx.x % p.groups;
-    const int j = warp & 3;
-    const int64_t row = tile * kTileRows + j * 32 + lane;
-    const int64_t c0 = (int64_t)group * kColumnsGroup + (warp >> 2) * 32;
-    const T *src = static_cast<const T *>(p.src) + row;
-    T v[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = row < p.rows && c0 + i < p.cols ? src[(c0 + i) * p.col_stride] : from_f32<T>(0.f);
     uint32_t codes[4], bytes;
     if (BLOCK == 32) {
         bytes = scale_byte<32>(amax_bits(v));
         quantize_codes<T, 32>(v, bytes, codes);
     } else {
-        T(&lo)[16] = *reinterpret_cast<T(*)[16]>(&v[0]);
-        T(&hi)[16] = *reinterpret_cast<T(*)[16]>(&v[16]);
+        const T(&lo)[16] = *reinterpret_cast<const T(*)[16]>(&v[0]);
+        const T(&hi)[16] = *reinterpret_cast<const T(*)[16]>(&v[16]);
         const uint32_t b0 = scale_byte<16>(amax_bits(lo)), b1 = scale_byte<16>(amax_bits(hi));
         quantize_codes<T, 16>(lo, b0, *reinterpret_cast<uint32_t(*)[2]>(&codes[0]));
         quantize_codes<T, 16>(hi, b1, *reinterpret_cast<uint32_t(*)[2]>(&codes[2]));
@@ -153,10 +163,47 @@ __global__ void __launch_bounds__(kThreads) quantize_columns_kernel(const Quanti
     if (row < p.rows && c0 < row_pitch(p.cols) * 2)
         *reinterpret_cast<uint4 *>(p.data + row * p.pitch + (c0 >> 1)) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
     const int k = (int)(c0 / BLOCK);  // first block
-    if ((k >> 2) < p.tiles) {
-        uint8_t *at = p.scales + (tile * p.tiles + (k >> 2)) * kTileBytes + lane * 16 + j * 4 + (k & 3);
+    if ((k >> 2) < p.tiles) {  // rows past the matrix too: their scales are 0
+        uint8_t *at = p.scales + ((row >> 7) * p.tiles + (k >> 2)) * kTileBytes + (row & 31) * 16 + (row >> 5 & 3) * 4 + (k & 3);
         if (BLOCK == 16) *reinterpret_cast<uint16_t *>(at) = (uint16_t)bytes;
         else *at = (uint8_t)bytes;
+    }
+}
+
+template <class T, int BLOCK, bool PAIRS>
+__global__ void __launch_bounds__(kThreads) quantize_columns_kernel(const QuantizeLaunch p)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t tile = blockIdx.x / p.groups;
+    const int group = blockIdx.x % p.groups;
+    if constexpr (PAIRS) {
+        const int64_t row = tile * kTileRows + (warp & 1) * 64 + 2 * lane;
+        const int64_t c0 = (int64_t)group * 2 * kColumnsGroup + (warp >> 1) * 32;
+        const T *src = static_cast<const T *>(p.src) + row;
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            w[i] = 0;
+            if (c0 + i >= p.cols) continue;
+            if (row + 1 < p.rows) w[i] = *reinterpret_cast<const uint32_t *>(src + (c0 + i) * p.col_stride);
+            else if (row < p.rows) w[i] = *reinterpret_cast<const uint16_t *>(src + (c0 + i) * p.col_stride);
+        }
+        alignas(4) T v[32];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                reinterpret_cast<uint32_t *>(v)[i] = __byte_perm(w[2 * i], w[2 * i + 1], h ? 0x7632 : 0x5410);
+            quantize_column_run<T, BLOCK>(p, v, row + h, c0);
+        }
+    } else {
+        const int64_t row = tile * kTileRows + (warp & 3) * 32 + lane;
+        const int64_t c0 = (int64_t)group * kColumnsGroup + (warp >> 2) * 32;
+        const T *src = static_cast<const T *>(p.src) + row;
+        alignas(4) T v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = row < p.rows && c0 + i < p.cols ? src[(c0 + i) * p.col_stride] : from_f32<T>(0.f);
+        quantize_column_run<T, BLOCK>(p, v, row, c0);
     }
 }
 
@@ -166,13 +213,20 @@ cudaError_t launch_quantize(QuantizeLaunch p, cudaStream_t st)
     p.tiles = tiles_per_row(p.cols, BLOCK);
     const bool unit = p.col_stride == 1 || p.cols == 1, columns = !unit && p.row_stride == 1;
     // a scale tile's padding is written too: whole tiles of 4 blocks
-    const int64_t width = columns ? kColumnsGroup : kGroupCols;
+    const bool pairs = sizeof(T) == 2 && is_aligned(p.src, 4) && p.col_stride % 2 == 0;
+    const int64_t width = columns ? (pairs ? 2 : 1) * kColumnsGroup : kGroupCols;
     p.groups = (int32_t)(((int64_t)p.tiles * 4 * BLOCK + width - 1) / width);
     const int64_t blocks = ((int64_t)p.rows + kTileRows - 1) / kTileRows * p.groups;
     if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
     const bool vec = unit && is_aligned(p.src, 16) && (p.rows == 1 || p.row_stride * sizeof(T) % 16 == 0);
-    if (columns) quantize_columns_kernel<T, BLOCK><<<(unsigned)blocks, kThreads, 0, st>>>(p);
-    else if (vec) quantize_rows_kernel<T, BLOCK, kVector><<<(unsigned)blocks, kThreads, 0, st>>>(p);
+    if (columns) {
+        if constexpr (sizeof(T) == 2) {
+            if (pairs) quantize_columns_kernel<T, BLOCK, true><<<(unsigned)blocks, kThreads, 0, st>>>(p);
+            else quantize_columns_kernel<T, BLOCK, false><<<(unsigned)blocks, kThreads, 0, st>>>(p);
+        } else {
+            quantize_columns_kernel<T, BLOCK, false><<<(unsigned)blocks, kThreads, 0, st>>>(p);
+        }
+    } else if (vec) quantize_rows_kernel<T, BLOCK, kVector><<<(unsigned)blocks, kThreads, 0, st>>>(p);
     else if (unit) quantize_rows_kernel<T, BLOCK, kStaged><<<(unsigned)blocks, kThreads, 0, st>>>(p);
     else quantize_rows_kernel<T, BLOCK, kStrided><<<(unsigned)blocks, kThreads, 0, st>>>(p);
     count_launch();

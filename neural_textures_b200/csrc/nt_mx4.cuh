@@ -84,22 +84,30 @@ __device__ __forceinline__ float inverse_scale(uint32_t byte)
     return s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
 }
 
-// x / s, near enough to round to the code of the exact quotient.  A code changes at quotients
+// x / s of two values, near enough to round to the code of the exact quotient.  A code changes at quotients
 // t = 1/4 .. 5, and there t * s is exact in 7 bits.
-//  - 16-bit x: x has at most 11 bits, so |x| is t * s or at least 2^-11 of it away.  |x| times the
+//  - 16-bit x: x has at most 11 bits, so |x| is t * s or at least 2^-11 of it away.  x times the
 //    rounded 1 / s is within 2^-22 of the quotient: rounding it to a multiple of 2^-16 (adding and
 //    subtracting 192) makes ties exact again and moves no other quotient across its t.
-//  - fp32 x (`kExact`): x can be one rounding step beside t * s, so the quotient is rounded
-//    towards zero and its last bit set when a remainder is left: enough to order it against t.
+//  - fp32 x (`kExact`): x can be one rounding step beside t * s.  The quotient is corrected once with its
+//    remainder x - q s (exact: s has 4 bits), truncated by the sign of the new remainder, and its last bit set
+//    when that is not zero: enough to order it against t.
 template <int BLOCK, bool kExact>
-__device__ __forceinline__ float scaled(float x, float inv, float s)
+__device__ __forceinline__ float2 scaled2(float2 x, float inv, float s)
 {
-    if (BLOCK == 32) return x * inv;
-    if (!kExact) return copysignf(__fsub_rn(__fmaf_rn(fabsf(x), inv, 192.f), 192.f), x);
-    if (!(s > 0.f)) return copysignf(0.f, x);
-    const float q = __fdiv_rz(fabsf(x), s);
-    const bool rest = __fmaf_rn(-q, s, fabsf(x)) != 0.f;
-    return copysignf(__uint_as_float(__float_as_uint(q) | (rest ? 1u : 0u)), x);
+    const float2 i2 = make_float2(inv, inv);
+    if (BLOCK == 32) return __fmul2_rn(x, i2);
+    if (!kExact) {
+        const float2 q = __fadd2_rn(__ffma2_rn(x, i2, make_float2(192.f, 192.f)), make_float2(-192.f, -192.f));
+        return make_float2(copysignf(q.x, x.x), copysignf(q.y, x.y));
+    }
+    const float2 a = make_float2(fabsf(x.x), fabsf(x.y)), n = make_float2(-s, -s);
+    float2 q = __fmul2_rn(a, i2);
+    q = __ffma2_rn(__ffma2_rn(q, n, a), i2, q);
+    const float2 r = __ffma2_rn(q, n, a);
+    const int lo = __float_as_int(q.x) + (__float_as_int(r.x) >> 31) | (r.x != 0.f);
+    const int hi = __float_as_int(q.y) + (__float_as_int(r.y) >> 31) | (r.y != 0.f);
+    return make_float2(copysignf(__int_as_float(lo), x.x), copysignf(__int_as_float(hi), x.y));
 }
 
 }  // namespace mx4
