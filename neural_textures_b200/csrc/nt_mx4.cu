@@ -83,17 +83,19 @@ __device__ __forceinline__ void quantize_codes(const T (&v)[N], uint32_t byte, u
 
 // Rows along the memory.  A thread block takes 128 rows x 128 columns.  BLOCK / 4 lanes share a row
 // (16 values each), so that they hold the four scales of one word; a lane takes rows r, r + 32,
-// r + 64 and r + 96, whose words are the 16 bytes of row r in the scale tile: one store.
-template <class T, int BLOCK, Access ACCESS>
+// r + 64 and r + 96, whose words are the 16 bytes of row r in the scale tile: one store.  NARROW: no more than 64
+// columns, and two tiles of rows instead.
+template <class T, int BLOCK, Access ACCESS, bool NARROW>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeLaunch p)
 {
     __shared__ T stage[ACCESS == kStaged ? 32 * kStagePitch : 1];
-    constexpr int LPR = BLOCK / 4, RPW = 32 / LPR;
+    constexpr int LPR = NARROW ? 4 : BLOCK / 4, RPW = 32 / LPR;
+    constexpr bool kHalves = NARROW || BLOCK == 16;  // four warps cover the rows of a tile
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t tile = blockIdx.x / p.groups;
-    const int group = blockIdx.x % p.groups;
-    const int half = BLOCK == 16 ? warp >> 2 : 0;
-    const int residue = (BLOCK == 16 ? warp & 3 : warp) * RPW + lane / LPR;
+    const int64_t tile = NARROW ? 2 * (int64_t)blockIdx.x + (warp >> 2) : blockIdx.x / p.groups;
+    const int group = NARROW ? 0 : blockIdx.x % p.groups;
+    const int half = kHalves && !NARROW ? warp >> 2 : 0;
+    const int residue = (kHalves ? warp & 3 : warp) * RPW + lane / LPR;
     const int64_t c = (int64_t)group * kGroupCols + half * 64 + (lane % LPR) * 16;
     uint32_t words[4];
     constexpr int U = ACCESS == kStaged ? 1 : sizeof(T) == 2 ? 4 : 2;  // rows in flight
@@ -135,7 +137,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeL
         }
     }
     const int tcol = BLOCK == 16 ? group * 2 + half : group;
-    if (lane % LPR == 0 && tcol < p.tiles)
+    if (lane % LPR == 0 && tcol < p.tiles && (!NARROW || tile * kTileRows < p.rows))
         *reinterpret_cast<uint4 *>(p.scales + (tile * p.tiles + tcol) * kTileBytes + residue * 16) =
             make_uint4(words[0], words[1], words[2], words[3]);
 }
@@ -226,9 +228,12 @@ cudaError_t launch_quantize(QuantizeLaunch p, cudaStream_t st)
         } else {
             quantize_columns_kernel<T, BLOCK, false><<<(unsigned)blocks, kThreads, 0, st>>>(p);
         }
-    } else if (vec) quantize_rows_kernel<T, BLOCK, kVector><<<(unsigned)blocks, kThreads, 0, st>>>(p);
-    else if (unit) quantize_rows_kernel<T, BLOCK, kStaged><<<(unsigned)blocks, kThreads, 0, st>>>(p);
-    else quantize_rows_kernel<T, BLOCK, kStrided><<<(unsigned)blocks, kThreads, 0, st>>>(p);
+    } else if (vec && p.cols <= 64) {
+        const unsigned pairs_of_tiles = (unsigned)(((int64_t)p.rows + 2 * kTileRows - 1) / (2 * kTileRows));
+        quantize_rows_kernel<T, BLOCK, kVector, true><<<pairs_of_tiles, kThreads, 0, st>>>(p);
+    } else if (vec) quantize_rows_kernel<T, BLOCK, kVector, false><<<(unsigned)blocks, kThreads, 0, st>>>(p);
+    else if (unit) quantize_rows_kernel<T, BLOCK, kStaged, false><<<(unsigned)blocks, kThreads, 0, st>>>(p);
+    else quantize_rows_kernel<T, BLOCK, kStrided, false><<<(unsigned)blocks, kThreads, 0, st>>>(p);
     count_launch();
     return cudaGetLastError();
 }
@@ -296,6 +301,15 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const DequantizeLa
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (32 * i + sub < left) first[32 * i + sub] = mine[32 * i + sub];
+        } else if (sizeof(T) == 4 && lanes == 32 && c - 8 * sub + 256 <= p.cols) {  // the same for whole aligned rows, 512 bytes at a time
+            T *const mine = turn[threadIdx.x >> 5];
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 2; ++i) reinterpret_cast<uint4 *>(mine + 8 * sub)[i] = reinterpret_cast<const uint4 *>(out)[i];
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                reinterpret_cast<uint4 *>(dst - 8 * sub)[32 * i + sub] = reinterpret_cast<const uint4 *>(mine)[32 * i + sub];
         } else if (p.vec && c + 8 <= p.cols) {
 #pragma unroll
             for (int i = 0; i < (int)sizeof(T) / 2; ++i)
