@@ -3,7 +3,8 @@
     python -m neural_textures_b200.build [--force] [--jobs N]
 
 Each .cu under csrc/ compiles to an object in _build/ (in parallel), then one link step
-produces neural_textures_b200/lib/libnt_b200.so.  The build is incremental on file
+produces neural_textures_b200/lib/libnt_b200.so; csrc/nt_torch.cpp (the texel layers' shortcut from torch
+tensors to that library) becomes lib/nt_torch.so.  The build is incremental on file
 modification times (any header change rebuilds everything).
 """
 from __future__ import annotations
@@ -11,9 +12,11 @@ from __future__ import annotations
 import argparse
 import concurrent.futures as cf
 import glob
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -21,6 +24,7 @@ CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIBDIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIBDIR, "libnt_b200.so")
+TORCH_LIB = os.path.join(LIBDIR, "nt_torch.so")
 NVCC = os.environ.get("NVCC", os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "bin", "nvcc"))
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -72,7 +76,27 @@ def build(force: bool = False, jobs: int | None = None, verbose_ptxas: bool = Fa
         os.replace(tmp, LIB)
     if verbose_ptxas:
         sys.stderr.write("".join(logs))
+    _build_torch(force)
     return LIB
+
+
+def _build_torch(force: bool) -> None:
+    src = os.path.join(CSRC, "nt_torch.cpp")
+    needs = [src, os.path.join(ROOT, "include", "nt_capi.h"), __file__]
+    if not force and os.path.exists(TORCH_LIB) and os.path.getmtime(TORCH_LIB) >= max(os.path.getmtime(n) for n in needs):
+        return
+    torch_dir = importlib.util.find_spec("torch").submodule_search_locations[0]  # without importing it
+    cuda = os.path.dirname(os.path.dirname(NVCC))
+    tmp = TORCH_LIB + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           "-I", os.path.join(ROOT, "include"), "-I", sysconfig.get_paths()["include"],
+           "-I", os.path.join(torch_dir, "include"), "-I", os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+           "-I", os.path.join(cuda, "include"), src, "-o", tmp, "-L", LIBDIR, "-l:libnt_b200.so", "-Wl,-rpath,$ORIGIN",
+           "-L", os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cuda", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for nt_torch.cpp:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, TORCH_LIB)
 
 
 def main(argv=None):

@@ -10,22 +10,33 @@ current stream of the tensors' device) and returns without waiting.  Results are
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
+import os
 import struct
 
 from . import _native as N
+from . import build as _build
 from ._native import check, load
 
 ACTIVATIONS = {"none": N.NT_ACT_NONE, "relu": N.NT_ACT_RELU, "silu": N.NT_ACT_SILU, "gelu": N.NT_ACT_GELU}
 
 _torch = None
+_fast = None  # lib/nt_torch.so: the usual calls, at a third of the host time; None from it: not a usual call
 _DTYPES = {}
 
 
 def _lazy_torch():
-    """torch, imported at the first call as everywhere in this package."""
-    global _torch
+    """torch, imported at the first call as everywhere in this package, and the shortcut module."""
+    global _torch, _fast
     if _torch is None:
         import torch
+        load()
+        path = _build.TORCH_LIB
+        if not os.path.exists(path):
+            raise OSError(f"{path} is missing: build it with `python -m neural_textures_b200.build`")
+        spec = importlib.util.spec_from_file_location("nt_torch", path)
+        _fast = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_fast)
         _DTYPES.update({torch.float16: N.NT_DTYPE_F16, torch.bfloat16: N.NT_DTYPE_BF16, torch.float32: N.NT_DTYPE_F32})
         _torch = torch
     return _torch
@@ -150,6 +161,10 @@ def group_norm(x, groups: int, gamma=None, beta=None, activation: str = "none", 
     (y, mean, rstd) with float32 statistics [N][groups], which group_norm_backward takes.  `out`
     receives y and may be x."""
     torch = _torch or _lazy_torch()
+    if out is None and stream is None:
+        made = _fast.group_norm(x, groups, gamma, beta, ACTIVATIONS.get(activation), eps)
+        if made is not None:
+            return made
     sizes, kind, device = _norm_sizes(x, groups), x.dtype, x.device
     n, h, w, c, g = sizes
     dtype, act, L = _dtype(x, "x"), _activation(activation), load()
@@ -174,6 +189,10 @@ def group_norm_backward(dy, x, mean, rstd, groups: int, gamma=None, beta=None, a
     dbeta).  dx has x's type; dgamma and dbeta are float32 [C], summed over images and texels.
     `out` receives dx and may be dy or x."""
     torch = _torch or _lazy_torch()
+    if out is None and stream is None:
+        made = _fast.group_norm_backward(dy, x, mean, rstd, groups, gamma, beta, ACTIVATIONS.get(activation))
+        if made is not None:
+            return made
     sizes, kind, device = _norm_sizes(x, groups), x.dtype, x.device
     n, h, w, c, g = sizes
     dtype, act, L = _dtype(x, "x"), _activation(activation), load()
@@ -198,9 +217,6 @@ def group_norm_backward(dy, x, mean, rstd, groups: int, gamma=None, beta=None, a
 # ---------------------------------------------------------------------------------------
 # 4-bit microscaled matrices
 
-_MATRIX = struct.Struct("@2Pq3i4x")
-
-
 class Mx4Tensor:
     """A rows x cols matrix in 4-bit microscaled form (NtMx4Matrix): `data`, the uint8 codes
     [rows][pitch], two to a byte, and `scales`, a byte per block of `block` columns (32: powers of
@@ -209,26 +225,23 @@ class Mx4Tensor:
 
     def __init__(self, data, scales, rows: int, cols: int, block: int = 32):
         torch = _torch or _lazy_torch()
+        self.data, self.scales, self.rows, self.cols, self.block = data, scales, rows, cols, block
+        self._packed = _fast.mx4_pack(data, scales, rows, cols, block)
+        if self._packed is not None:
+            return
+        # not a matrix: say why
         if block not in (16, 32):
             raise ValueError(f"block must be 16 or 32, not {block}")
-        if rows < 0 or cols < 1:
+        if not 0 <= rows <= 0x7fffff00 or not 1 <= cols <= 0x7fffff00:
             raise ValueError(f"{rows} x {cols} is not a matrix size")
         pitch, size = -(-cols // 32) * 16, -(-rows // 128) * -(-cols // (4 * block)) * 512
-        shape = data.shape
-        if data.dtype is not torch.uint8 or len(shape) != 2 or shape[0] < rows or shape[1] < pitch:
-            raise ValueError(f"data must be uint8 [{rows}][{pitch}] or larger")
-        step, one = data.stride()
-        if one != 1:
-            raise ValueError("data: the codes of a row must be contiguous")
+        if data.dtype is not torch.uint8 or data.dim() != 2 or data.shape[0] < rows or data.shape[1] < pitch or rows and data.stride(1) != 1:
+            raise ValueError(f"data must be uint8 [{rows}][{pitch}] or larger, the codes of a row contiguous")
         if scales.dtype is not torch.uint8 or not scales.is_contiguous() or scales.numel() < size:
             raise ValueError(f"scales must be contiguous uint8 of {size} bytes")
         if scales.device != data.device:
             raise ValueError(f"scales is on {scales.device}, not on {data.device}")
-        self._set(data, scales, int(rows), int(cols), int(block), step if rows > 1 else max(step, pitch) // 16 * 16)
-
-    def _set(self, data, scales, rows, cols, block, pitch):
-        self.data, self.scales, self.rows, self.cols, self.block = data, scales, rows, cols, block
-        self._packed = _MATRIX.pack(data.data_ptr(), scales.data_ptr(), pitch, rows, cols, block)
+        raise TypeError("data and scales must be torch tensors, rows, cols and block integers")
 
     @classmethod
     def empty(cls, rows: int, cols: int, block: int = 32, device="cuda"):
@@ -236,10 +249,8 @@ class Mx4Tensor:
         if block not in (16, 32) or rows < 0 or cols < 1:
             raise ValueError(f"{rows} x {cols} in blocks of {block} is not a 4-bit matrix")
         pitch = -(-cols // 32) * 16
-        self = cls.__new__(cls)
-        self._set(_new((rows, pitch), torch.uint8, device),
-                  _new((-(-rows // 128) * -(-cols // (4 * block)) * 512,), torch.uint8, device), rows, cols, block, pitch)
-        return self
+        return cls(_new((rows, pitch), torch.uint8, device),
+                   _new((-(-rows // 128) * -(-cols // (4 * block)) * 512,), torch.uint8, device), rows, cols, block)
 
     @property
     def shape(self):
@@ -261,6 +272,13 @@ def mx4_quantize(x, block: int = 32, out: Mx4Tensor | None = None, stream=None) 
     """The float16, bfloat16 or float32 matrix x (2-D, any strides: x.t() is read in place) in 4-bit
     microscaled form, blocks along its columns (nt_mx4_quantize)."""
     _torch or _lazy_torch()
+    if out is None and stream is None:
+        made = _fast.mx4_quantize(x, block)
+        if made is not None:
+            out = Mx4Tensor.__new__(Mx4Tensor)
+            (out.rows, out.cols), out.block = x.shape, block
+            out.data, out.scales, out._packed = made
+            return out
     dtype = _dtype(x, "x")
     if x.dim() != 2:
         raise ValueError(f"x must be a matrix, not {tuple(x.shape)}")
@@ -289,6 +307,10 @@ def mx4_dequantize(q: Mx4Tensor, dtype=None, out=None, stream=None):
     torch = _torch or _lazy_torch()
     dtype = dtype or (out.dtype if out is not None else torch.float16)
     code = _dtype(dtype, "dtype")
+    if out is None and stream is None:
+        y = _fast.mx4_dequantize(q._packed, q.data, code)
+        if y is not None:
+            return y
     y, stride = _output(out, q.rows, q.cols, dtype, q.device)
     _launch(q.device, stream, (y if out is None else None,), load().nt_mx4_dequantize, q._packed, y.data_ptr(), code, stride)
     return y
@@ -300,7 +322,12 @@ def mx4_product(a: Mx4Tensor, b: Mx4Tensor, bias=None, activation: str = "none",
     output for texels a and weights b [out][in], bias float32 [out] or None."""
     torch = _torch or _lazy_torch()
     dtype = dtype or (out.dtype if out is not None else torch.float16)
-    code, act, device = _dtype(dtype, "dtype"), _activation(activation), a.device
+    code, act = _dtype(dtype, "dtype"), _activation(activation)
+    if out is None and stream is None:
+        y = _fast.mx4_product(a._packed, a.data, b._packed, b.data, bias, act, alpha, code)
+        if y is not None:
+            return y
+    device = a.device
     if b.data.device != device:
         raise ValueError(f"b is on {b.device}, not on {device}")
     y, stride = _output(out, a.rows, b.rows, dtype, device)

@@ -12,7 +12,10 @@ from tests import layer_oracle as O
 def test_parameter_blocks_match(native):
     from neural_textures_b200 import _native as N, layers
     assert C.sizeof(N.NtGroupNorm) == layers._GROUP_NORM.size
-    assert C.sizeof(N.NtMx4Matrix) == layers._MATRIX.size
+    import neural_textures_b200 as nt
+    q = nt.Mx4Tensor.empty(5, 70, 16, device="cpu")
+    m = N.NtMx4Matrix.from_buffer_copy(q._packed)
+    assert (m.data, m.scales, m.pitch, m.rows, m.cols, m.block) == (q.data.data_ptr(), q.scales.data_ptr(), 48, 5, 70, 16)
     packed = layers._GROUP_NORM.pack(*range(1, 8), 0.5, *range(8, 32))
     p = N.NtGroupNorm.from_buffer_copy(packed)
     assert (p.images, p.activation, p.epsilon, p.x.data, p.x.texel_stride, p.gamma, p.rstd) == (1, 7, 0.5, 8, 11, 12, 15)
