@@ -89,6 +89,7 @@ template <class T, int BLOCK, Access ACCESS, bool NARROW>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeLaunch p)
 {
     __shared__ T stage[ACCESS == kStaged ? 32 * kStagePitch : 1];
+    after_previous();
     constexpr int LPR = NARROW ? 4 : BLOCK / 4, RPW = 32 / LPR;
     constexpr bool kHalves = NARROW || BLOCK == 16;  // four warps cover the rows of a tile
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -175,6 +176,7 @@ __device__ __forceinline__ void quantize_column_run(const QuantizeLaunch &p, con
 template <class T, int BLOCK, bool PAIRS>
 __global__ void __launch_bounds__(kThreads) quantize_columns_kernel(const QuantizeLaunch p)
 {
+    after_previous();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t tile = blockIdx.x / p.groups;
     const int group = blockIdx.x % p.groups;
@@ -218,24 +220,23 @@ cudaError_t launch_quantize(QuantizeLaunch p, cudaStream_t st)
     const bool pairs = sizeof(T) == 2 && is_aligned(p.src, 4) && p.col_stride % 2 == 0;
     const int64_t width = columns ? (pairs ? 2 : 1) * kColumnsGroup : kGroupCols;
     p.groups = (int32_t)(((int64_t)p.tiles * 4 * BLOCK + width - 1) / width);
-    const int64_t blocks = ((int64_t)p.rows + kTileRows - 1) / kTileRows * p.groups;
+    int64_t blocks = ((int64_t)p.rows + kTileRows - 1) / kTileRows * p.groups;
     if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
     const bool vec = unit && is_aligned(p.src, 16) && (p.rows == 1 || p.row_stride * sizeof(T) % 16 == 0);
+    void (*kernel)(QuantizeLaunch) = quantize_rows_kernel<T, BLOCK, kStrided, false>;
     if (columns) {
-        if constexpr (sizeof(T) == 2) {
-            if (pairs) quantize_columns_kernel<T, BLOCK, true><<<(unsigned)blocks, kThreads, 0, st>>>(p);
-            else quantize_columns_kernel<T, BLOCK, false><<<(unsigned)blocks, kThreads, 0, st>>>(p);
-        } else {
-            quantize_columns_kernel<T, BLOCK, false><<<(unsigned)blocks, kThreads, 0, st>>>(p);
-        }
+        kernel = quantize_columns_kernel<T, BLOCK, false>;
+        if constexpr (sizeof(T) == 2)
+            if (pairs) kernel = quantize_columns_kernel<T, BLOCK, true>;
     } else if (vec && p.cols <= 64) {
-        const unsigned pairs_of_tiles = (unsigned)(((int64_t)p.rows + 2 * kTileRows - 1) / (2 * kTileRows));
-        quantize_rows_kernel<T, BLOCK, kVector, true><<<pairs_of_tiles, kThreads, 0, st>>>(p);
-    } else if (vec) quantize_rows_kernel<T, BLOCK, kVector, false><<<(unsigned)blocks, kThreads, 0, st>>>(p);
-    else if (unit) quantize_rows_kernel<T, BLOCK, kStaged, false><<<(unsigned)blocks, kThreads, 0, st>>>(p);
-    else quantize_rows_kernel<T, BLOCK, kStrided, false><<<(unsigned)blocks, kThreads, 0, st>>>(p);
-    count_launch();
-    return cudaGetLastError();
+        blocks = ((int64_t)p.rows + 2 * kTileRows - 1) / (2 * kTileRows);
+        kernel = quantize_rows_kernel<T, BLOCK, kVector, true>;
+    } else if (vec) {
+        kernel = quantize_rows_kernel<T, BLOCK, kVector, false>;
+    } else if (unit) {
+        kernel = quantize_rows_kernel<T, BLOCK, kStaged, false>;
+    }
+    return launch_next(kernel, dim3((unsigned)blocks), kThreads, 0, st, 1, p);
 }
 
 // ---- back --------------------------------------------------------------------------------
@@ -256,6 +257,7 @@ constexpr int kDequantRows = 4;  // rows of one lane
 template <class T, int BLOCK>
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const DequantizeLaunch p)
 {
+    after_previous();
     const int lanes = 1 << p.lanes_log2;
     const int sub = threadIdx.x & (lanes - 1);
     const int rows_per_pass = kThreads >> p.lanes_log2;
@@ -334,9 +336,7 @@ cudaError_t launch_dequantize(DequantizeLaunch p, cudaStream_t st)
     const int64_t rows_per_block = (int64_t)(kThreads >> p.lanes_log2) * kDequantRows;
     const int64_t grid = ((int64_t)p.rows + rows_per_block - 1) / rows_per_block * p.col_blocks;
     if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    dequantize_kernel<T, BLOCK><<<(unsigned)grid, kThreads, 0, st>>>(p);
-    count_launch();
-    return cudaGetLastError();
+    return launch_next(dequantize_kernel<T, BLOCK>, dim3((unsigned)grid), kThreads, 0, st, 1, p);
 }
 
 // Shared checks of a matrix argument.

@@ -362,6 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     umma::fence_after();
     const uint32_t tmem = ctl.tmem;
+    after_previous();
 
     if (warp == 0) {
         int s = 0;
@@ -602,22 +603,9 @@ nt_status launch_product(const NtMx4Matrix *a, const NtMx4Matrix *b, ProductLaun
     p.tma_store = p.tma_store && !p.swapped && p.split == 1 && (p.bn >= 64 || p.dtype == NT_DTYPE_F32) && encode_output(&d_map, p);
     const void *kernel = reinterpret_cast<const void *>(&product_kernel<BLOCK>);
     cudaError_t e = set_smem_limit(kernel, 227 * 1024 - sizeof(Shared));
-    if (e == cudaSuccess) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)grid);
-        cfg.blockDim = dim3(kThreads);
-        cfg.dynamicSmemBytes = smem;
-        cfg.stream = st;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = (unsigned)p.split;
-        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        e = cudaLaunchKernelEx(&cfg, product_kernel<BLOCK>, l_map, c_map, d_map, p);
-    }
+    if (e == cudaSuccess)
+        e = launch_next(product_kernel<BLOCK>, dim3((unsigned)grid), kThreads, smem, st, (unsigned)p.split, l_map, c_map, d_map, p);
     if (e != cudaSuccess) return set_error(NT_ERR_CUDA, "4-bit product: %s", cudaGetErrorString(e));
-    count_launch();
     return NT_OK;
 }
 

@@ -11,6 +11,7 @@ constexpr int kJoinWarps = 8;
 
 __global__ void __launch_bounds__(32 * kJoinWarps) join_channels_kernel(const NormLaunch L)
 {
+    after_previous();
     const int c = blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
     if (c < L.p.channels) join_channel(L, c);
 }
@@ -30,7 +31,7 @@ struct Plan {
 // passes) takes about 0.35 us forward and 0.6 us backward.  So an image is split until a block has four turns,
 // and goes to the grid where the largest cluster would leave it more than kTurns.  128 x 128 x 64 fp16, forward:
 // 21.1 us on a cluster of 8, 13.6 us on one of 16, 12.6 us on the grid; 64 x 64 x 64: 8.8, 7.8, 12 us.
-constexpr int kForwardTurns = 14, kBackwardTurns = 8;
+constexpr int kForwardTurns = 20, kBackwardTurns = 10;
 
 Plan plan(const NtGroupNorm *p, bool backward)
 {
@@ -139,35 +140,29 @@ cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
     const NormKernel kernel = backward ? backward_kernel(p->dtype, v, whole, even) : forward_kernel(p->dtype, v, whole, even);
     cudaError_t e = set_smem_limit(reinterpret_cast<const void *>(kernel), 227 * 1024 - 1024);
     if (e != cudaSuccess) return e;
-    if (!pl.cluster && (e = cudaMemsetAsync(ws, 0, 16, st)) != cudaSuccess) return e;
-    if (pl.cluster && pl.splits > 8) {
-        e = cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (pl.cluster) {
+        if (pl.splits > 8) e = cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
+        e = launch_next(kernel, dim3((unsigned)pl.splits, (unsigned)p->images), threads, smem, st, (unsigned)pl.splits, L);
+        if (e == cudaSuccess && backward && p->images > 1 && (p->dgamma || p->dbeta))
+            e = launch_next(join_channels_kernel, dim3((unsigned)ceil_div(p->channels, kJoinWarps)), 32 * kJoinWarps, 0, st, 1, L);
+        return e;
     }
+    // the blocks wait for one another: a cooperative launch, with its counter cleared in front of it
+    if ((e = cudaMemsetAsync(ws, 0, 16, st)) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)pl.splits, (unsigned)p->images);
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
-    if (pl.cluster) {
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = (unsigned)pl.splits;
-        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    } else {
-        attr[0].id = cudaLaunchAttributeCooperative;
-        attr[0].val.cooperative = 1;
-    }
+    attr[0].id = cudaLaunchAttributeCooperative;
+    attr[0].val.cooperative = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = pl.cluster && pl.splits == 1 ? 0 : 1;
+    cfg.numAttrs = 1;
     e = cudaLaunchKernelEx(&cfg, kernel, L);
-    if (e != cudaSuccess) return e;
-    count_launch();
-    if (backward && pl.cluster && p->images > 1 && (p->dgamma || p->dbeta)) {
-        join_channels_kernel<<<(unsigned)ceil_div(p->channels, kJoinWarps), 32 * kJoinWarps, 0, st>>>(L);
-        count_launch();
-    }
-    return cudaGetLastError();
+    if (e == cudaSuccess) count_launch();
+    return e;
 }
 
 nt_status check_map(const NtFeatureMap &f, const char *name, const NtGroupNorm *p, int size, bool written)

@@ -521,6 +521,7 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
     const Threads<T, V, WHOLE, FLAT, BACKWARD> th = {L,    n,       lo, row, col, mine,
                                                stat, scratch,
                                                (uint32_t)__cvta_generic_to_shared(smem + L.scratch) + tid * (uint32_t)sizeof(Vec<T, V>)};
+    after_previous();
     int slot0 = 0;
     for (int v0 = 0; v0 < L.vectors; v0 += L.tx, slot0 += most) {
         const int vec = v0 + col;
