@@ -33,8 +33,10 @@ from .api import (  # noqa: F401
     run_forward_pass_test,
     train_step,
 )
+from .encoder import LatentEncoder  # noqa: F401
 from .layers import (  # noqa: F401
     Mx4Tensor,
+    TexelLayer,
     group_norm,
     group_norm_backward,
     mx4_dequantize,

@@ -447,6 +447,32 @@ class NeuralTexture:
         self.blocks = None
         self.latent_format = N.NT_LATENT_GRID_F16
 
+    # -- latents in 4 bits ----------------------------------------------------------------
+    @_on_device
+    def export_mx4(self, block: int = 16, stream=None):
+        """The fp16 grids (all levels) in 4-bit microscaled form, one Mx4Tensor per grid of rows of one texel row's
+        values (level 0) or of 256 (chains): 4.5 bits a value in blocks of 16, 4.25 in blocks of 32."""
+        from .layers import mx4_quantize
+        if self.latent_format != N.NT_LATENT_GRID_F16:
+            raise RuntimeError("export_mx4 stores fp16 grids")
+        return [mx4_quantize(self._mx4_rows(g), block=block, stream=stream) for g in range(2)]
+
+    @_on_device
+    def from_mx4(self, packed, stream=None):
+        """Grids from export_mx4's tensors (of a texture of the same sizes)."""
+        from .layers import mx4_dequantize
+        if self.latent_format != N.NT_LATENT_GRID_F16:
+            raise RuntimeError("from_mx4 fills fp16 grids")
+        for g, q in enumerate(packed):
+            mx4_dequantize(q, out=self._mx4_rows(g), stream=stream)
+
+    def _mx4_rows(self, g: int):
+        w, h = self.grid_sizes[g]
+        if self.num_mips[g] == 1:
+            return self.grid_chains[g].view(h, w * self.C)
+        n = self.grid_chains[g].numel()
+        return self.grid_chains[g].view(-1, 256 if n % 256 == 0 else self.C)
+
     # -- initialisation -------------------------------------------------------------------
     @_on_device
     def init(self, seed: int = 0, target_seed: int | None = None, pbr_normals: bool = False,

@@ -44,7 +44,7 @@ Plan plan(const NtGroupNorm *p, bool backward)
     const int64_t most = std::min<int64_t>(texels, kMaxSplits);
     const int largest = (int64_t)p->images * kMaxCluster <= sms * 7 / 8 ? kMaxCluster : 8;  // of 16: one in most of the GPCs
     int64_t splits = 1;
-    while (splits < largest && splits * 2 <= most && turns > 4 * splits) splits *= 2;
+    while (splits < largest && splits * 2 <= most && turns > 4 * splits && splits * p->images <= sms) splits *= 2;
     const int64_t resident = (int64_t)per_sm * sms / p->images;
     if (turns <= (backward ? kBackwardTurns : kForwardTurns) * splits || resident <= splits) {
         const int64_t all = splits * p->images;

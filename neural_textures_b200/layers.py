@@ -334,3 +334,56 @@ def mx4_product(a: Mx4Tensor, b: Mx4Tensor, bias=None, activation: str = "none",
     _launch(device, stream, (y if out is None else None,), load().nt_mx4_product, a._packed, b._packed,
             _vector(bias, b.rows, device, "bias"), act, alpha, y.data_ptr(), code, stride)
     return y
+
+
+# ---------------------------------------------------------------------------------------
+# a layer
+
+class TexelLayer:
+    """One layer of a network over a channels-last map: group norm, activation, then a product with a
+    4-bit weight matrix, texel by texel:  out = act(norm(x)) W^T + bias.
+
+    The fp32 masters are `weight` [out][in], `bias` [out], `gamma` and `beta` [in]; `pack` lays the weights out
+    in 4 bits, once after each change.  forward(keep=True) keeps what backward needs.  backward takes the
+    gradient of the output and returns that of x; those of the parameters are in `grads`, in `parameters`' order.
+    Its products run in 4 bits too, on matrices quantised along the other axis, in blocks of 32: their
+    power-of-two scales hold gradients of any size, where E4M3 scales end at 2^-9.  The rounding to 4 bits is
+    passed straight through."""
+
+    def __init__(self, channels_in: int, channels_out: int, groups: int, activation: str = "silu", block: int = 16,
+                 device="cuda", seed: int = 0):
+        torch = _torch or _lazy_torch()
+        g = torch.Generator().manual_seed(seed)
+        self.groups, self.activation, self.block = groups, activation, block
+        f32 = dict(dtype=torch.float32, device=device)
+        self.weight = (torch.randn((channels_out, channels_in), generator=g) * channels_in ** -0.5).to(**f32)
+        self.bias = torch.zeros(channels_out, **f32)
+        self.gamma, self.beta = torch.ones(channels_in, **f32), torch.zeros(channels_in, **f32)
+        self.grads = None
+        self.pack()
+
+    @property
+    def parameters(self):
+        return [self.weight, self.bias, self.gamma, self.beta]
+
+    def pack(self):
+        self.packed = mx4_quantize(self.weight, block=self.block)
+
+    def forward(self, x, keep: bool = False):
+        y, mean, rstd = group_norm(x, self.groups, self.gamma, self.beta, activation=self.activation)
+        rows = y.view(-1, y.shape[-1])
+        out = mx4_product(mx4_quantize(rows, block=self.block), self.packed, bias=self.bias, dtype=x.dtype)
+        if keep:
+            self._kept = (x, rows, mean, rstd)
+        return out.view(*x.shape[:-1], out.shape[-1])
+
+    def backward(self, dout):
+        torch = _torch
+        x, rows, mean, rstd = self._kept
+        d = dout.reshape(-1, dout.shape[-1])
+        dy = mx4_product(mx4_quantize(d), mx4_quantize(self.weight.t()), dtype=x.dtype)
+        dweight = mx4_product(mx4_quantize(d.t()), mx4_quantize(rows.t()), dtype=torch.float32)
+        dx, dgamma, dbeta = group_norm_backward(dy.view(x.shape), x, mean, rstd, self.groups, self.gamma, self.beta,
+                                                activation=self.activation)
+        self.grads = [dweight, d.float().sum(dim=0), dgamma, dbeta]
+        return dx

@@ -63,6 +63,12 @@ NORM_SIZES = [
     (2, 2, 3, 4100, 4, 0),     # more channels than threads
     (1, 3, 2, 8192, 8192, 0),
     (1, 512, 509, 16, 2, 0),
+    # more texels than a block keeps in shared memory
+    (160, 64, 40, 32, 4, 0),
+    (150, 200, 100, 3, 1, 0),   # single channels
+    (150, 33, 31, 20, 10, 4),   # vectors across groups, unaligned
+    (150, 4, 3, 8192, 16, 0),   # several turns along a texel
+    (1, 1000, 1100, 24, 3, 0),  # the whole grid
 ]
 
 
@@ -286,6 +292,28 @@ def test_mx4_fp32_neighbours_of_ties(cuda):
     check_quantized(nt, x.cuda(), 16)
 
 
+@pytest.mark.parametrize("dtype", ALL, ids=["f16", "bf16", "f32"])
+@pytest.mark.parametrize("m,n,k,block", [
+    (4000, 2500, 160, 16),   # tiles of 256 columns, several to a block
+    (4000, 2501, 96, 32),    # rows of d that no tensor map takes
+    (40000, 64, 64, 32),     # epilogue warps in turns, several tiles to a block
+    (40001, 50, 30, 16), (20000, 24, 130, 32), (5000, 128, 300, 16)])
+def test_mx4_product_of_many_tiles(cuda, m, n, k, block, dtype):
+    """Against 64-bit products on the device; the tolerance of test_mx4_product."""
+    import neural_textures_b200 as nt
+    g = torch.Generator(device="cuda").manual_seed(m + n)
+    qa = nt.mx4_quantize(torch.randn((m, k), generator=g, device="cuda"), block=block)
+    qb = nt.mx4_quantize(torch.randn((n, k), generator=g, device="cuda"), block=block)
+    bias = torch.randn(n, generator=g, device="cuda")
+    d = nt.mx4_product(qa, qb, bias=bias, activation="relu", alpha=0.5, dtype=dtype)
+    a, b = nt.mx4_dequantize(qa, torch.float32).double(), nt.mx4_dequantize(qb, torch.float32).double()
+    want = torch.relu(0.5 * (a @ b.t()) + bias.double())
+    size = 0.5 * (a.abs() @ b.abs().t()) + bias.double().abs()
+    tol = (k / 16 + 8) * U * size
+    tol = tol + O.HALF_ULP[dtype] * (want + tol) + O.TINY[dtype]
+    assert bool(((d.double() - want).abs() <= tol).all())
+
+
 @pytest.mark.parametrize("block", [16, 32])
 @pytest.mark.parametrize("m,n,k", [
     (1, 1, 1), (1, 5, 16), (1, 300, 4096), (7, 129, 100), (33, 64, 64), (128, 128, 256), (130, 257, 1111), (1000, 24, 48),
@@ -379,3 +407,30 @@ def test_layers_in_a_graph(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, layer()))
+
+
+def test_offsets_past_32_bits(cuda):
+    """Rows and images 2^31 elements apart: reading, writing, and a product's rows 2^25 apart."""
+    import neural_textures_b200 as nt
+    far = 1 << 31
+    pool = torch.empty(far + (1 << 26), dtype=torch.float16, device="cuda")
+    x = torch.as_strided(pool, (2, 200), (far, 1))
+    values = matrix(2, 200, torch.float16, 5)
+    x.copy_(values)
+    q, want = nt.mx4_quantize(x), nt.mx4_quantize(values.contiguous())
+    assert torch.equal(q.data, want.data) and torch.equal(q.scales, want.scales)
+    nt.mx4_dequantize(want, out=torch.as_strided(pool, (2, 200), (far, 1), 512))
+    assert torch.equal(torch.as_strided(pool, (2, 200), (far, 1), 512), nt.mx4_dequantize(want))
+    small, gamma, beta, _ = norm_case((2, 5, 6, 16), torch.float16, 4)
+    apart = torch.as_strided(pool, (2, 5, 6, 16), (far, 96, 16, 1), 4096)
+    apart.copy_(small)
+    y, *_ = nt.group_norm(apart, 4, gamma, beta, activation="silu")
+    w, *_ = nt.group_norm(small, 4, gamma, beta, activation="silu")
+    assert float((y.float() - w.float()).abs().max()) <= 2.0 ** -10 * float(w.float().abs().max())
+    out = torch.as_strided(pool, (2, 5, 6, 16), (far, 96, 16, 1), 8192)
+    nt.group_norm(small, 4, gamma, beta, activation="silu", out=out)
+    assert torch.equal(out, w)
+    a, b = nt.mx4_quantize(torch.randn((65, 128), device="cuda")), nt.mx4_quantize(torch.randn((96, 128), device="cuda"))
+    rows = torch.as_strided(pool, (65, 96), (1 << 25, 1), 1 << 14)
+    nt.mx4_product(a, b, out=rows)
+    assert torch.equal(rows, nt.mx4_product(a, b))
