@@ -69,6 +69,39 @@ struct Shared {
     Control ctl;
 };
 
+// A launch parameter in a register: the loops branch on these, and a chain of branches each behind a load from
+// the constant bank cost the epilogue of a tile 500 cycles, the issuing warps 200 a stage.
+__device__ __forceinline__ int held(int v)
+{
+    asm volatile("" : "+r"(v));
+    return v;
+}
+__device__ __forceinline__ float held(float v)
+{
+    asm volatile("" : "+f"(v));
+    return v;
+}
+template <class T>
+__device__ __forceinline__ T *held(T *v)
+{
+    asm volatile("" : "+l"(v));
+    return v;
+}
+
+// What the epilogue reads of the launch.
+struct Output {
+    int bn, l_rows, c_rows, dtype, tma_store;
+    float alpha;
+    const float *bias;
+    void *d;
+    int64_t row_stride;
+    __device__ __forceinline__ explicit Output(const ProductLaunch &p)
+        : bn(held(p.bn)), l_rows(held(p.l_rows)), c_rows(held(p.c_rows)), dtype(held(p.dtype)), tma_store(held(p.tma_store)),
+          alpha(held(p.alpha)), bias(held(p.bias)), d(held(p.d)), row_stride(p.row_stride)
+    {
+    }
+};
+
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar)
@@ -165,21 +198,21 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity)
     return false;
 }
 
-__device__ __forceinline__ void cluster_sync()
-{
-    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ float peer_f32(uint32_t addr, uint32_t rank)
+__device__ __forceinline__ uint32_t peer_address(uint32_t addr, uint32_t rank)
 {
     uint32_t remote;
-    float v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
-    return v;
+    return remote;
+}
+__device__ __forceinline__ void peer_store(uint32_t remote, uint32_t v)
+{
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote), "r"(v) : "memory");
 }
 
-__device__ __forceinline__ void store_one(const ProductLaunch &p, int64_t at, float v)
+__device__ __forceinline__ void store_one(const Output &p, int64_t at, float v)
 {
     if (p.dtype == NT_DTYPE_F32) static_cast<float *>(p.d)[at] = v;
     else if (p.dtype == NT_DTYPE_F16) static_cast<__half *>(p.d)[at] = __float2half_rn(v);
@@ -199,7 +232,7 @@ __device__ __forceinline__ uint32_t pack2(int dtype, float lo, float hi)
 // Lanes are b's rows: lane = column of d, accumulator columns = rows of d; a warp's store is contiguous.  The two
 // warps of a quarter take every other 32 columns (`half`).
 template <int ACT>
-__device__ __forceinline__ void epilogue_swapped(const ProductLaunch &p, uint32_t tmem, int lane0, int col0, int half)
+__device__ __forceinline__ void epilogue_swapped(const Output &p, uint32_t tmem, int lane0, int col0, int half)
 {
     const int64_t n = lane0 + (threadIdx.x & 127);
     const float bias = p.bias && n < p.l_rows ? __ldg(p.bias + n) : 0.f;
@@ -223,7 +256,7 @@ __device__ __forceinline__ void epilogue_swapped(const ProductLaunch &p, uint32_
 // `i0` is its first column range and `di` the distance to its next; of 256 columns, those from `first` on come
 // first, and `part` is told when they have been read.  `bias_at`: the columns that `bias` holds.
 template <int ACT>
-__device__ __forceinline__ void epilogue_rows(const ProductLaunch &p, const CUtensorMap *d_map, uint32_t tmem, int lane0, int col0, int i0,
+__device__ __forceinline__ void epilogue_rows(const Output &p, const CUtensorMap *d_map, uint32_t tmem, int lane0, int col0, int i0,
                                               int di, int first, uint32_t part, uint8_t *mine, float *bias, int &bias_at)
 {
     const int lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) & 3;
@@ -312,8 +345,8 @@ struct Tiles {
     __device__ __forceinline__ Tiles(const ProductLaunch &p)
     {
         const unsigned first = blockIdx.x / p.split, step = gridDim.x / p.split;
-        l_tiles = p.l_tiles;
-        c_tiles = p.c_tiles;
+        l_tiles = held(p.l_tiles);
+        c_tiles = held(p.c_tiles);
         l = (int)(first % (unsigned)l_tiles), c = (int)(first / (unsigned)l_tiles);
         dl = (int)(step % (unsigned)l_tiles), dc = (int)(step / (unsigned)l_tiles);
     }
@@ -326,6 +359,69 @@ struct Tiles {
     }
 };
 
+struct EpilogueArgs {
+    const CUtensorMap *d_map;
+    uint32_t acc_full, acc_empty, acc_part, accs;  // accs: the accumulators' lanes of this warp
+    uint8_t *staging;
+    float *bias;
+    int turns, swapped;
+};
+
+// All tiles of the block, for one epilogue warp.
+template <int ACT>
+__device__ __forceinline__ void epilogue(const Output &out, const ProductLaunch &p, const EpilogueArgs &e)
+{
+    const int lane = threadIdx.x & 31, half = (threadIdx.x - 128) >> 7, width = out.dtype == NT_DTYPE_F32 ? 32 : 64;
+    const int i0 = e.turns ? 0 : half * width, di = e.turns ? width : 2 * width;
+    int buf = 0, bias_at = -1;
+    uint32_t phase = 0;
+    e.bias[lane] = e.bias[lane + 32] = 0.f;
+    __syncwarp();
+    for (Tiles t(p); t.valid(); t.next()) {
+        if (!e.turns || buf == half) {
+            const uint32_t acc = e.accs + buf * kAccStep;
+            if (!__all_sync(0xffffffffu, wait(e.acc_full + 8 * buf, phase))) break;
+            umma::fence_after();
+            if (e.swapped)
+                epilogue_swapped<ACT>(out, acc, t.l * 128, t.c * out.bn, half);
+            else
+                epilogue_rows<ACT>(out, e.d_map, acc, t.l * 128, t.c * out.bn, i0, di, buf ? 0 : 128, e.acc_part + 8 * buf, e.staging,
+                                   e.bias, bias_at);
+            umma::fence_before();
+            __syncwarp();
+            if (lane == 0) umma::mbar_arrive(e.acc_empty + 8 * buf);
+        }
+        buf ^= 1;
+        if (buf == 0) phase ^= 1;
+    }
+    if (out.tma_store && elect_one()) store_wait();
+    __syncwarp();
+}
+
+// A block's partial sums to the blocks of the cluster that own their columns: there, `sums` holds
+// [block][own column][lane].
+constexpr int kPartialPitch = 129;  // lanes of a column and a bank more: columns are read across too
+
+__device__ __forceinline__ void send_partials(const Output &out, int split, int rank, uint32_t acc_full, uint32_t acc, uint32_t sums, int half)
+{
+    const bool ok = __all_sync(0xffffffffu, wait(acc_full, 0));
+    umma::fence_after();
+    cluster_wait();  // the peers run
+    if (!ok) return;
+    const int lane = threadIdx.x & 127, cols = out.bn / split, log = __ffs(cols) - 1;  // powers of two
+    for (int c0 = 32 * half; c0 < out.bn; c0 += 64) {
+        uint32_t v[32];
+        ld32(acc + c0, v);
+        umma::wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const int c = c0 + i;
+            if (c >= out.bn) break;
+            peer_store(peer_address(sums + ((rank * cols + (c & (cols - 1))) * kPartialPitch + lane) * 4, c >> log), v[i]);
+        }
+    }
+}
+
 template <int BLOCK>
 __global__ void __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap l_map, const __grid_constant__ CUtensorMap c_map,
@@ -336,17 +432,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ Shared sh;
     Control &ctl = sh.ctl;
     uint8_t *stages = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5;
     const uint32_t base = smem_u32(stages), full = smem_u32(ctl.full), empty = smem_u32(ctl.empty),
                    acc_full = smem_u32(ctl.acc_full), acc_empty = smem_u32(ctl.acc_empty), acc_part = smem_u32(ctl.acc_part);
-    const int c_off = 128 * p.row_bytes, ls_off = c_off + p.bn * p.row_bytes, cs_off = ls_off + kTiles * kTileBytes;
-    const int c_scales = p.bn > 128 ? 2 : 1;  // row tiles of the column operand's scales
-    const int k_steps = (p.k + 63) / 64, stage_steps = p.row_bytes / 32, k_stages = (k_steps + stage_steps - 1) / stage_steps;
-    const int rank = p.split > 1 ? blockIdx.x % p.split : 0;
-    const int k_lo = (int)((int64_t)k_stages * rank / p.split), k_hi = (int)((int64_t)k_stages * (rank + 1) / p.split);
+    const int bn = held(p.bn), row_bytes = held(p.row_bytes), num_stages = held(p.stages), stage_bytes = held(p.stage_bytes),
+              split = held(p.split);
+    const int c_off = 128 * row_bytes, ls_off = c_off + bn * row_bytes, cs_off = ls_off + kTiles * kTileBytes;
+    const int c_scales = bn > 128 ? 2 : 1;  // row tiles of the column operand's scales
+    const int k_steps = held((p.k + 63) / 64), stage_steps = row_bytes / 32, k_stages = (k_steps + stage_steps - 1) / stage_steps;
+    const int rank = split > 1 ? blockIdx.x % split : 0;
+    const int k_lo = split > 1 ? (int)((int64_t)k_stages * rank / split) : 0,
+              k_hi = split > 1 ? (int)((int64_t)k_stages * (rank + 1) / split) : k_stages;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < p.stages; ++i) {
+        for (int i = 0; i < num_stages; ++i) {
             umma::mbar_init(full + 8 * i, 1);
             umma::mbar_init(empty + 8 * i, 1);
         }
@@ -362,52 +461,57 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     umma::fence_after();
     const uint32_t tmem = ctl.tmem;
+    if (split > 1) cluster_arrive();  // peers write into this block's shared memory: only once it runs
     after_previous();
 
     if (warp == 0) {
         int s = 0;
         uint32_t phase = 0;
         bool ok = true;
+        const int scale_tiles = held(p.scale_tiles), c_rows = held(p.c_rows);
+        const uint8_t *const l_scales = held(p.l_scales), *const c_scale_data = held(p.c_scales);
         for (Tiles t(p); ok && t.valid(); t.next()) {
-            const int lt = t.l, c0 = t.c * p.bn;
+            const int lt = t.l, c0 = t.c * bn, cs = min(c_scales, (c_rows - c0 + 127) >> 7);
+            const uint8_t *const ls = l_scales + (int64_t)lt * scale_tiles * kTileBytes;
+            const uint8_t *const sc = c_scale_data + (int64_t)(c0 >> 7) * scale_tiles * kTileBytes;
             for (int ks = k_lo; ks < k_hi; ++ks) {
                 if (!(ok = __all_sync(0xffffffffu, wait(empty + 8 * s, phase ^ 1)))) break;
-                const uint32_t at = base + s * p.stage_bytes, bar = full + 8 * s;
-                const int st = min(kTiles, p.scale_tiles - ks * kTiles);
-                const int cs = min(c_scales, (p.c_rows - c0 + 127) >> 7);
+                const uint32_t at = base + s * stage_bytes, bar = full + 8 * s;
+                const int st = min(kTiles, scale_tiles - ks * kTiles), from = ks * kTiles * kTileBytes;
                 if (elect_one()) {
                     expect_tx(bar, ls_off + (1 + cs) * st * kTileBytes);
-                    tma_2d(at, &l_map, ks * p.row_bytes, lt * 128, bar);
-                    tma_2d(at + c_off, &c_map, ks * p.row_bytes, c0, bar);
-                    bulk_copy(at + ls_off, p.l_scales + ((int64_t)lt * p.scale_tiles + ks * kTiles) * kTileBytes, st * kTileBytes, bar);
-                    for (int j = 0; j < cs; ++j)
-                        bulk_copy(at + cs_off + j * kTiles * kTileBytes,
-                                  p.c_scales + ((int64_t)((c0 >> 7) + j) * p.scale_tiles + ks * kTiles) * kTileBytes, st * kTileBytes,
-                                  bar);
+                    tma_2d(at, &l_map, ks * row_bytes, lt * 128, bar);
+                    tma_2d(at + c_off, &c_map, ks * row_bytes, c0, bar);
+                    bulk_copy(at + ls_off, ls + from, st * kTileBytes, bar);
+                    bulk_copy(at + cs_off, sc + from, st * kTileBytes, bar);
+                    if (cs == 2)
+                        bulk_copy(at + cs_off + kTiles * kTileBytes, sc + (int64_t)scale_tiles * kTileBytes + from, st * kTileBytes, bar);
                 }
                 __syncwarp();
-                if (++s == p.stages) s = 0, phase ^= 1;
+                if (++s == num_stages) s = 0, phase ^= 1;
             }
         }
-        if (!ok)  // the products have stopped: wait for the copies that nobody will wait for
-            for (int i = 0; i < p.stages; ++i) umma::mbar_wait(full + 8 * i, i < s ? phase : phase ^ 1, 1u << 16);
+        // no copy is in flight when the block ends, whether or not the products took them all
+        for (int i = 0; i < num_stages; ++i) umma::mbar_wait(full + 8 * i, i < s ? phase : phase ^ 1, 1u << 16);
     } else if (warp == 1) {
         int s = 0, buf = 0, sbuf = 0;
         uint32_t phase = 0, acc_phase = 0, part_phase = 0;
         bool ok = true, first = true;
+        const uint64_t da0 = codes_desc(base, p.layout), db0 = codes_desc(base + c_off, p.layout);
+        const uint32_t id0 = idesc<BLOCK>(bn, 0), id1 = BLOCK == 16 ? id0 : idesc<BLOCK>(bn, 2);
         for (Tiles t(p); ok && t.valid(); t.next()) {
             if (!(ok = __all_sync(0xffffffffu, wait(acc_empty + 8 * buf, acc_phase ^ 1)))) break;
-            if (p.bn > kAccStep && !first && !(ok = __all_sync(0xffffffffu, wait(acc_part + 8 * (buf ^ 1), part_phase)))) break;
+            if (bn > kAccStep && !first && !(ok = __all_sync(0xffffffffu, wait(acc_part + 8 * (buf ^ 1), part_phase)))) break;
             if (buf == 0) part_phase ^= !first;
             first = false;
             umma::fence_after();
             const uint32_t acc = tmem + buf * kAccStep;
             for (int ks = k_lo; ks < k_hi; ++ks) {
+                const uint32_t at = base + s * stage_bytes, sl = tmem + kScaleCol + sbuf * kScaleCols, sc = sl + 16;
+                const int steps = min(stage_steps, k_steps - ks * stage_steps);
+                const uint64_t step = (uint64_t)((uint32_t)(s * stage_bytes) >> 4), da = da0 + step, db = db0 + step;
                 if (!(ok = __all_sync(0xffffffffu, wait(full + 8 * s, phase)))) break;
                 umma::fence_after();
-                const uint32_t at = base + s * p.stage_bytes, sl = tmem + kScaleCol + sbuf * kScaleCols, sc = sl + 16;
-                const int steps = min(stage_steps, k_steps - ks * stage_steps);
-                const uint64_t da = codes_desc(at, p.layout), db = codes_desc(at + c_off, p.layout);
                 if (elect_one()) {
 #pragma unroll
                     for (int i = 0; i < kTiles; ++i)
@@ -420,87 +524,55 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int i = 0; i < 4; ++i)
                         if (i < steps) {
                             const int tile = BLOCK == 16 ? i : i >> 1;
-                            mma<BLOCK>(acc, da + 2 * i, db + 2 * i, idesc<BLOCK>(p.bn, BLOCK == 16 ? 0 : (i & 1) * 2), sl + 4 * tile,
-                                       sc + 4 * tile * c_scales, ks > k_lo || i > 0);
+                            mma<BLOCK>(acc, da + 2 * i, db + 2 * i, i & 1 ? id1 : id0, sl + 4 * tile, sc + 4 * tile * c_scales,
+                                       ks > k_lo || i > 0);
                         }
                     umma::commit(empty + 8 * s);
                     if (ks + 1 == k_hi) umma::commit(acc_full + 8 * buf);
                 }
                 __syncwarp();
-                if (++s == p.stages) s = 0, phase ^= 1;
+                if (++s == num_stages) s = 0, phase ^= 1;
                 sbuf ^= 1;
             }
             buf ^= 1;
             if (buf == 0) acc_phase ^= 1;
         }
     } else if (warp >= 4) {
-        int buf = 0, bias_at = -1;
-        const int half = (warp - 4) >> 2, width = p.dtype == NT_DTYPE_F32 ? 32 : 64;
-        const int i0 = p.turns ? 0 : half * width, di = p.turns ? width : 2 * width;
-        uint8_t *const mine = sh.staging[warp - 4];
-        float *const bias = sh.bias[warp - 4];
-        bias[lane] = bias[lane + 32] = 0.f;
-        __syncwarp();
-        uint32_t acc_phase = 0;
-        for (Tiles t(p); t.valid(); t.next()) {
-            const uint32_t acc = tmem + buf * kAccStep + ((uint32_t)(warp & 3) << 21), part = acc_part + 8 * buf;
-            const int lane0 = t.l * 128, col0 = t.c * p.bn, first = buf ? 0 : 128;
-            if (!p.turns || buf == half) {
-                if (!__all_sync(0xffffffffu, wait(acc_full + 8 * buf, acc_phase))) break;
-                umma::fence_after();
-                if (p.split > 1) {  // partial sums [column][lane], a lane a bank
-                    float *dump = reinterpret_cast<float *>(stages) + (threadIdx.x & 127);
-                    for (int c0 = 32 * half; c0 < p.bn; c0 += 64) {
-                        uint32_t v[32];
-                        ld32(acc + c0, v);
-                        umma::wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (c0 + i < p.bn) dump[(c0 + i) * 129] = __uint_as_float(v[i]);
-                    }
-                } else if (p.swapped) {
-                    switch (p.activation) {
-                    case NT_ACT_RELU: epilogue_swapped<NT_ACT_RELU>(p, acc, lane0, col0, half); break;
-                    case NT_ACT_SILU: epilogue_swapped<NT_ACT_SILU>(p, acc, lane0, col0, half); break;
-                    case NT_ACT_GELU: epilogue_swapped<NT_ACT_GELU>(p, acc, lane0, col0, half); break;
-                    default: epilogue_swapped<NT_ACT_NONE>(p, acc, lane0, col0, half); break;
-                    }
-                } else {
-                    switch (p.activation) {
-                    case NT_ACT_RELU: epilogue_rows<NT_ACT_RELU>(p, &d_map, acc, lane0, col0, i0, di, first, part, mine, bias, bias_at); break;
-                    case NT_ACT_SILU: epilogue_rows<NT_ACT_SILU>(p, &d_map, acc, lane0, col0, i0, di, first, part, mine, bias, bias_at); break;
-                    case NT_ACT_GELU: epilogue_rows<NT_ACT_GELU>(p, &d_map, acc, lane0, col0, i0, di, first, part, mine, bias, bias_at); break;
-                    default: epilogue_rows<NT_ACT_NONE>(p, &d_map, acc, lane0, col0, i0, di, first, part, mine, bias, bias_at); break;
-                    }
-                }
-                umma::fence_before();
-                __syncwarp();
-                if (lane == 0) umma::mbar_arrive(acc_empty + 8 * buf);
+        const Output out(p);
+        const uint32_t accs = tmem + ((uint32_t)(warp & 3) << 21);
+        if (split > 1) {
+            send_partials(out, split, rank, acc_full, accs, base + num_stages * stage_bytes, (warp - 4) >> 2);
+        } else {
+            const EpilogueArgs e = {&d_map, acc_full, acc_empty, acc_part, accs, sh.staging[warp - 4], sh.bias[warp - 4], held(p.turns),
+                                    held(p.swapped)};
+            switch (p.activation) {
+            case NT_ACT_RELU: epilogue<NT_ACT_RELU>(out, p, e); break;
+            case NT_ACT_SILU: epilogue<NT_ACT_SILU>(out, p, e); break;
+            case NT_ACT_GELU: epilogue<NT_ACT_GELU>(out, p, e); break;
+            default: epilogue<NT_ACT_NONE>(out, p, e); break;
             }
-            buf ^= 1;
-            if (buf == 0) acc_phase ^= 1;
         }
-        if (p.tma_store && elect_one()) store_wait();
-        __syncwarp();
     }
-    __syncwarp();  // the single lanes of warps 0 and 1 rejoin the others
-    if (p.split > 1) {
+    __syncwarp();
+    if (split > 1) {
+        if (warp < 4) cluster_wait();  // of the arrival at the start; the others waited before they sent
         __syncthreads();
-        cluster_sync();
+        cluster_arrive();
+        cluster_wait();  // every block's partial sums have arrived
+        const Output out(p);
         const Tiles t(p);
-        const int lane0 = t.l * 128, col0 = t.c * p.bn;
-        const int lo = p.bn * rank / p.split, cols = p.bn * (rank + 1) / p.split - lo;
+        const int lane0 = t.l * 128, col0 = t.c * bn;
+        const int cols = bn / split, lo = cols * rank;
+        const float *sums = reinterpret_cast<const float *>(stages + num_stages * stage_bytes);
         for (int i = threadIdx.x; i < cols * 128; i += kThreads) {
             // consecutive threads along d's rows
-            const int l = p.swapped ? i & 127 : i / cols, c = lo + (p.swapped ? i >> 7 : i % cols);
+            const int l = p.swapped ? i & 127 : i / cols, c = p.swapped ? i >> 7 : i % cols;
             float sum = 0.f;
-            for (int r = 0; r < p.split; ++r) sum += peer_f32(base + (c * 129 + l) * 4, r);
-            const int64_t row = p.swapped ? col0 + c : lane0 + l, col = p.swapped ? lane0 + l : col0 + c;
-            if (lane0 + l < p.l_rows && col0 + c < p.c_rows)
-                store_one(p, row * p.row_stride + col,
-                          activate1(fmaf(p.alpha, sum, p.bias ? __ldg(p.bias + col) : 0.f), p.activation));
+            for (int r = 0; r < split; ++r) sum += sums[(r * cols + c) * kPartialPitch + l];
+            const int64_t row = p.swapped ? col0 + lo + c : lane0 + l, col = p.swapped ? lane0 + l : col0 + lo + c;
+            if (lane0 + l < out.l_rows && col0 + lo + c < out.c_rows)
+                store_one(out, row * out.row_stride + col, activate1(fmaf(out.alpha, sum, out.bias ? __ldg(out.bias + col) : 0.f), p.activation));
         }
-        cluster_sync();  // a block's sums stay until its peers have read them
     }
     umma::fence_before();
     __syncthreads();
@@ -592,9 +664,10 @@ nt_status launch_product(const NtMx4Matrix *a, const NtMx4Matrix *b, ProductLaun
     while (p.split < 8 && p.bn <= 128 && tiles * p.split * 2 <= sms && k_stages >= p.split * 4) p.split *= 2;
     p.turns = !p.swapped && p.split == 1 && p.bn <= 64;
     p.stage_bytes = (int32_t)ceil_div((128 + p.bn) * p.row_bytes + (p.bn > 128 ? 3 : 2) * kTiles * kTileBytes, 1024) * 1024;
-    const int room = 227 * 1024 - 1024 - (int)sizeof(Shared);
+    const size_t partials = p.split > 1 ? (size_t)p.bn * kPartialPitch * 4 : 0;
+    const int room = 227 * 1024 - 1024 - (int)sizeof(Shared) - (int)partials;
     p.stages = std::min(kMaxStages, room / p.stage_bytes);
-    const size_t smem = 1024 + std::max((size_t)p.stages * p.stage_bytes, p.split > 1 ? (size_t)p.bn * 129 * 4 : 0);
+    const size_t smem = 1024 + (size_t)p.stages * p.stage_bytes + partials;
     const int64_t grid = p.split > 1 ? tiles * p.split : std::min<int64_t>(tiles, sms);
     CUtensorMap l_map, c_map, d_map = {};
     if (!encode_codes(&l_map, l, 128, p.row_bytes) || !encode_codes(&c_map, c, p.bn, p.row_bytes))
