@@ -9,9 +9,9 @@
 //   warps 4-11  epilogue: accumulator -> scale, bias, activation, rounding -> shared -> rows of d by TMA.  Two
 //               warps for each quarter of the lanes: they halve a tile's columns, or, of tiles of 64 columns
 //               and less, take every other tile
-// There are two accumulators in tensor memory, so that the epilogue of a tile runs under the products of the
-// next; blocks take tiles gridDim apart.  Two of 256 columns and the scales do not fit: they share 96
-// columns, which the epilogue reads first.
+// There are two accumulators in tensor memory, four of 64 columns and less, so that the epilogue of a tile runs
+// under the products of the next; blocks take tiles gridDim apart.  Two of 256 columns and the scales do
+// not fit: they share 96 columns, which the epilogue reads first.
 //
 // Few rows (m <= 64): the weights' rows go to the lanes, and bn is m rounded up, so that a token costs no
 // empty columns.  Few tiles: a cluster of up to 8 blocks splits K, leaves its partial sums in shared
@@ -51,14 +51,15 @@ struct ProductLaunch {
 
 constexpr int kThreads = 384, kEpilogueWarps = 8;
 constexpr int kMaxStages = 8;
-constexpr int kAccStep = 160;  // columns between the two accumulators
+constexpr int kMaxAcc = 4;
+constexpr int kAccStep = 160, kNarrowAccStep = 64;  // columns between two accumulators
 constexpr int kStaging = 32 * 128;  // epilogue staging of a warp: 32 rows of 128 bytes, swizzled as TMA expects
 constexpr uint32_t kTmemCols = 512, kScaleCol = 416, kScaleCols = 48;
 
 struct Control {
     alignas(8) uint64_t full[kMaxStages];
     uint64_t empty[kMaxStages];
-    uint64_t acc_full[2], acc_empty[2];
+    uint64_t acc_full[kMaxAcc], acc_empty[kMaxAcc];
     uint64_t acc_part[2];  // the columns that the other accumulator shares are free
     uint32_t tmem;
 };
@@ -373,13 +374,14 @@ __device__ __forceinline__ void epilogue(const Output &out, const ProductLaunch 
 {
     const int lane = threadIdx.x & 31, half = (threadIdx.x - 128) >> 7, width = out.dtype == NT_DTYPE_F32 ? 32 : 64;
     const int i0 = e.turns ? 0 : half * width, di = e.turns ? width : 2 * width;
+    const int num_acc = e.turns ? 4 : 2, acc_step = e.turns ? kNarrowAccStep : kAccStep;
     int buf = 0, bias_at = -1;
     uint32_t phase = 0;
     e.bias[lane] = e.bias[lane + 32] = 0.f;
     __syncwarp();
     for (Tiles t(p); t.valid(); t.next()) {
-        if (!e.turns || buf == half) {
-            const uint32_t acc = e.accs + buf * kAccStep;
+        if (!e.turns || (buf & 1) == half) {
+            const uint32_t acc = e.accs + buf * acc_step;
             if (!__all_sync(0xffffffffu, wait(e.acc_full + 8 * buf, phase))) break;
             umma::fence_after();
             if (e.swapped)
@@ -391,8 +393,7 @@ __device__ __forceinline__ void epilogue(const Output &out, const ProductLaunch 
             __syncwarp();
             if (lane == 0) umma::mbar_arrive(e.acc_empty + 8 * buf);
         }
-        buf ^= 1;
-        if (buf == 0) phase ^= 1;
+        if (++buf == num_acc) buf = 0, phase ^= 1;
     }
     if (out.tma_store && elect_one()) store_wait();
     __syncwarp();
@@ -449,11 +450,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             umma::mbar_init(full + 8 * i, 1);
             umma::mbar_init(empty + 8 * i, 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kMaxAcc; ++i) {
             umma::mbar_init(acc_full + 8 * i, 1);
             umma::mbar_init(acc_empty + 8 * i, p.turns ? kEpilogueWarps / 2 : kEpilogueWarps);
-            umma::mbar_init(acc_part + 8 * i, kEpilogueWarps);
         }
+        for (int i = 0; i < 2; ++i) umma::mbar_init(acc_part + 8 * i, kEpilogueWarps);
         umma::mbar_fence_init();
     }
     if (warp == 2) umma::alloc(smem_u32(&ctl.tmem), kTmemCols);
@@ -497,6 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int s = 0, buf = 0, sbuf = 0;
         uint32_t phase = 0, acc_phase = 0, part_phase = 0;
         bool ok = true, first = true;
+        const int num_acc = p.turns ? 4 : 2, acc_step = p.turns ? kNarrowAccStep : kAccStep;
         const uint64_t da0 = codes_desc(base, p.layout), db0 = codes_desc(base + c_off, p.layout);
         const uint32_t id0 = idesc<BLOCK>(bn, 0), id1 = BLOCK == 16 ? id0 : idesc<BLOCK>(bn, 2);
         for (Tiles t(p); ok && t.valid(); t.next()) {
@@ -505,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (buf == 0) part_phase ^= !first;
             first = false;
             umma::fence_after();
-            const uint32_t acc = tmem + buf * kAccStep;
+            const uint32_t acc = tmem + buf * acc_step;
             for (int ks = k_lo; ks < k_hi; ++ks) {
                 const uint32_t at = base + s * stage_bytes, sl = tmem + kScaleCol + sbuf * kScaleCols, sc = sl + 16;
                 const int steps = min(stage_steps, k_steps - ks * stage_steps);
@@ -534,8 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (++s == num_stages) s = 0, phase ^= 1;
                 sbuf ^= 1;
             }
-            buf ^= 1;
-            if (buf == 0) acc_phase ^= 1;
+            if (++buf == num_acc) buf = 0, acc_phase ^= 1;
         }
     } else if (warp >= 4) {
         const Output out(p);
