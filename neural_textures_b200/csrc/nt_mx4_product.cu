@@ -4,7 +4,9 @@
 // One operand's rows are the accumulator's 128 lanes (the lane operand), the other's its bn columns
 // (the column operand).  A thread block computes 128 x bn tiles, 256 values of K a stage:
 //   warp 0      copies: TMA tiles of codes (rows of 128 bytes, or 32 or 64 where K is no longer, swizzled;
-//               zeros past the matrix) and the scale tiles, which lie in memory as tensor memory wants them
+//               zeros past the matrix) and the scale tiles, which lie in memory as tensor memory wants them.  A
+//               column operand of one tile and one stage, the weights of a narrow layer, comes once: copies
+//               of short rows are bound by their number, which the SMs of a GPC share
 //   warp 1      per stage: scale tiles shared -> tensor memory, four products of K = 64, commit
 //   warps 4-11  epilogue: accumulator -> scale, bias, activation, rounding -> shared -> rows of d by TMA.  Two
 //               warps for each quarter of the lanes: they halve a tile's columns, or, of tiles of 64 columns
@@ -36,6 +38,7 @@ struct ProductLaunch {
     int32_t bn, l_tiles, c_tiles;
     int32_t scale_tiles;       // scale tiles of 128 rows of either operand
     int32_t stages, stage_bytes;
+    int32_t resident;          // the column operand is one tile of one stage: loaded once, behind the stages
     int32_t row_bytes;         // codes of a row in a stage: 32, 64 or 128 bytes
     uint64_t layout;           // their swizzle and group stride, as descriptor bits
     int32_t split;             // thread blocks of a cluster, each with a share of K
@@ -438,7 +441,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                    acc_full = smem_u32(ctl.acc_full), acc_empty = smem_u32(ctl.acc_empty), acc_part = smem_u32(ctl.acc_part);
     const int bn = held(p.bn), row_bytes = held(p.row_bytes), num_stages = held(p.stages), stage_bytes = held(p.stage_bytes),
               split = held(p.split);
-    const int c_off = 128 * row_bytes, ls_off = c_off + bn * row_bytes, cs_off = ls_off + kTiles * kTileBytes;
+    // of a stage: the lane operand, its scales, the column operand, its scales; the latter two behind all stages
+    // where they are resident
+    const bool resident = held(p.resident);
+    const int ls_off = 128 * row_bytes, lane_bytes = ls_off + kTiles * kTileBytes,
+              c_off = resident ? num_stages * stage_bytes : (lane_bytes + 1023) & ~1023, cs_off = c_off + bn * row_bytes;
     const int c_scales = bn > 128 ? 2 : 1;  // row tiles of the column operand's scales
     const int k_steps = held((p.k + 63) / 64), stage_steps = row_bytes / 32, k_stages = (k_steps + stage_steps - 1) / stage_steps;
     const int rank = split > 1 ? blockIdx.x % split : 0;
@@ -471,6 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         const int scale_tiles = held(p.scale_tiles), c_rows = held(p.c_rows);
         const uint8_t *const l_scales = held(p.l_scales), *const c_scale_data = held(p.c_scales);
+        bool columns = true;  // to be loaded
         for (Tiles t(p); ok && t.valid(); t.next()) {
             const int lt = t.l, c0 = t.c * bn, cs = min(c_scales, (c_rows - c0 + 127) >> 7);
             const uint8_t *const ls = l_scales + (int64_t)lt * scale_tiles * kTileBytes;
@@ -479,15 +487,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!(ok = __all_sync(0xffffffffu, wait(empty + 8 * s, phase ^ 1)))) break;
                 const uint32_t at = base + s * stage_bytes, bar = full + 8 * s;
                 const int st = min(kTiles, scale_tiles - ks * kTiles), from = ks * kTiles * kTileBytes;
+                const uint32_t ct = resident ? base : at;
                 if (elect_one()) {
-                    expect_tx(bar, ls_off + (1 + cs) * st * kTileBytes);
+                    expect_tx(bar, ls_off + st * kTileBytes + (columns ? bn * row_bytes + cs * st * kTileBytes : 0));
                     tma_2d(at, &l_map, ks * row_bytes, lt * 128, bar);
-                    tma_2d(at + c_off, &c_map, ks * row_bytes, c0, bar);
                     bulk_copy(at + ls_off, ls + from, st * kTileBytes, bar);
-                    bulk_copy(at + cs_off, sc + from, st * kTileBytes, bar);
-                    if (cs == 2)
-                        bulk_copy(at + cs_off + kTiles * kTileBytes, sc + (int64_t)scale_tiles * kTileBytes + from, st * kTileBytes, bar);
+                    if (columns) {
+                        tma_2d(ct + c_off, &c_map, ks * row_bytes, c0, bar);
+                        bulk_copy(ct + cs_off, sc + from, st * kTileBytes, bar);
+                        if (cs == 2)
+                            bulk_copy(ct + cs_off + kTiles * kTileBytes, sc + (int64_t)scale_tiles * kTileBytes + from, st * kTileBytes, bar);
+                    }
                 }
+                columns = !resident;
                 __syncwarp();
                 if (++s == num_stages) s = 0, phase ^= 1;
             }
@@ -497,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 1) {
         int s = 0, buf = 0, sbuf = 0;
         uint32_t phase = 0, acc_phase = 0, part_phase = 0;
-        bool ok = true, first = true;
+        bool ok = true, first = true, columns = true;  // columns: their scales are to be copied
         const int num_acc = p.turns ? 4 : 2, acc_step = p.turns ? kNarrowAccStep : kAccStep;
         const uint64_t da0 = codes_desc(base, p.layout), db0 = codes_desc(base + c_off, p.layout);
         const uint32_t id0 = idesc<BLOCK>(bn, 0), id1 = BLOCK == 16 ? id0 : idesc<BLOCK>(bn, 2);
@@ -509,9 +521,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             umma::fence_after();
             const uint32_t acc = tmem + buf * acc_step;
             for (int ks = k_lo; ks < k_hi; ++ks) {
-                const uint32_t at = base + s * stage_bytes, sl = tmem + kScaleCol + sbuf * kScaleCols, sc = sl + 16;
+                const uint32_t at = base + s * stage_bytes, sl = tmem + kScaleCol + sbuf * kScaleCols,
+                               sc = resident ? tmem + kScaleCol + 16 : sl + 16;
                 const int steps = min(stage_steps, k_steps - ks * stage_steps);
-                const uint64_t step = (uint64_t)((uint32_t)(s * stage_bytes) >> 4), da = da0 + step, db = db0 + step;
+                const uint64_t step = (uint64_t)((uint32_t)(s * stage_bytes) >> 4), da = da0 + step, db = resident ? db0 : db0 + step;
                 if (!(ok = __all_sync(0xffffffffu, wait(full + 8 * s, phase)))) break;
                 umma::fence_after();
                 if (elect_one()) {
@@ -519,8 +532,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int i = 0; i < kTiles; ++i)
                         if (i * (4 / kTiles) < steps) {
                             copy_scale_tile(sl + 4 * i, at + ls_off + i * kTileBytes);
-                            copy_scale_tile(sc + 4 * i * c_scales, at + cs_off + i * kTileBytes);
-                            if (c_scales == 2) copy_scale_tile(sc + 8 * i + 4, at + cs_off + (kTiles + i) * kTileBytes);
+                            if (columns) {
+                                const uint32_t from = (resident ? base : at) + cs_off;
+                                copy_scale_tile(sc + 4 * i * c_scales, from + i * kTileBytes);
+                                if (c_scales == 2) copy_scale_tile(sc + 8 * i + 4, from + (kTiles + i) * kTileBytes);
+                            }
                         }
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -533,6 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (ks + 1 == k_hi) umma::commit(acc_full + 8 * buf);
                 }
                 __syncwarp();
+                columns = !resident;
                 if (++s == num_stages) s = 0, phase ^= 1;
                 sbuf ^= 1;
             }
@@ -664,11 +681,15 @@ nt_status launch_product(const NtMx4Matrix *a, const NtMx4Matrix *b, ProductLaun
     p.split = 1;
     while (p.split < 8 && p.bn <= 128 && tiles * p.split * 2 <= sms && k_stages >= p.split * 4) p.split *= 2;
     p.turns = !p.swapped && p.split == 1 && p.bn <= 64;
-    p.stage_bytes = (int32_t)ceil_div((128 + p.bn) * p.row_bytes + (p.bn > 128 ? 3 : 2) * kTiles * kTileBytes, 1024) * 1024;
+    p.resident = p.split == 1 && p.c_tiles == 1 && k_stages == 1 && tiles > sms;
+    const int64_t lane_bytes = 128 * p.row_bytes + kTiles * kTileBytes,
+                  column_bytes = ceil_div(p.bn * p.row_bytes + (p.bn > 128 ? 2 : 1) * kTiles * kTileBytes, 1024) * 1024;
+    p.stage_bytes = (int32_t)(ceil_div(lane_bytes, 1024) * 1024 + (p.resident ? 0 : column_bytes));
     const size_t partials = p.split > 1 ? (size_t)p.bn * kPartialPitch * 4 : 0;
-    const int room = 227 * 1024 - 1024 - (int)sizeof(Shared) - (int)partials;
+    const size_t behind = p.resident ? (size_t)column_bytes : partials;
+    const int room = 227 * 1024 - 1024 - (int)sizeof(Shared) - (int)behind;
     p.stages = std::min(kMaxStages, room / p.stage_bytes);
-    const size_t smem = 1024 + (size_t)p.stages * p.stage_bytes + partials;
+    const size_t smem = 1024 + (size_t)p.stages * p.stage_bytes + behind;
     const int64_t grid = p.split > 1 ? tiles * p.split : std::min<int64_t>(tiles, sms);
     CUtensorMap l_map, c_map, d_map = {};
     if (!encode_codes(&l_map, l, 128, p.row_bytes) || !encode_codes(&c_map, c, p.bn, p.row_bytes))
