@@ -107,9 +107,8 @@ cudaError_t launch_train_tc(const TrainLaunch &p, int channels, cudaStream_t str
 cudaError_t launch_decode_tc(const DecodeLaunch &p, int channels, cudaStream_t stream);
 // Status word of the decode kernel's bounded waits (host read, optionally cleared).
 cudaError_t read_decode_status(uint32_t *status, bool clear);
-// The same of the 4-bit product and group-norm kernels.
+// The same of the 4-bit product kernel.
 cudaError_t read_product_status(uint32_t *status, bool clear);
-cudaError_t read_norm_status(uint32_t *status, bool clear);
 cudaError_t launch_adam(const AdamLaunch &p, cudaStream_t stream);
 int sm_count();
 // Raise the dynamic shared-memory limit of `kernel` once per device.

@@ -18,20 +18,21 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_channels_kernel(const No
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Thread blocks of an image, and how they meet.  A function of the sizes alone, so that the caller's
-// workspace does not depend on addresses.
+// Thread blocks of an image.  A function of the sizes alone, so that the caller's workspace does not depend on
+// addresses.
 struct Plan {
-    int splits;
-    bool cluster;
-    int per_sm;  // blocks that share an SM's shared memory
+    bool cluster;  // one launch
+    int splits;    // blocks of an image, in the launch that makes the sums
+    int applies;   // and in the one that makes the result
+    int per_sm;    // blocks that share an SM's shared memory
 };
 
-// A cluster costs about 1 us over a single block; the grid's barrier, with the clearing of its counter and the cooperative
-// launch, about 6 us more, but then every SM computes.  A turn of a block (a vector for each of its threads, both
-// passes) takes about 0.35 us forward and 0.6 us backward.  So an image is split until a block has four turns,
-// and goes to the grid where the largest cluster would leave it more than kTurns.  128 x 128 x 64 fp16, forward:
-// 21.1 us on a cluster of 8, 13.6 us on one of 16, 12.6 us on the grid; 64 x 64 x 64: 8.8, 7.8, 12 us.
-constexpr int kForwardTurns = 20, kBackwardTurns = 10;
+// A cluster costs about 1 us over a single block, a second launch about 3 us more, but then every SM computes.  A
+// turn of a block (a vector for each of its threads, both passes) takes about 0.35 us forward and 0.6 us backward.
+// So an image is split until a block has four turns, and takes two launches where the largest cluster would
+// leave it more than kTurns.
+constexpr int kForwardTurns = 8, kBackwardTurns = 4;
+constexpr int kApplyTurns = 16;  // of a block of the second launch: enough of them that fast SMs take more
 
 Plan plan(const NtGroupNorm *p, bool backward)
 {
@@ -46,25 +47,23 @@ Plan plan(const NtGroupNorm *p, bool backward)
     int64_t splits = 1;
     while (splits < largest && splits * 2 <= most && turns > 4 * splits && splits * p->images <= sms) splits *= 2;
     const int64_t resident = (int64_t)per_sm * sms / p->images;
-    if (turns <= (backward ? kBackwardTurns : kForwardTurns) * splits || resident <= splits) {
-        const int64_t all = splits * p->images;
-        return {(int)splits, true, all <= sms ? 1 : per_sm};
-    }
-    return {(int)std::min({ceil_div(turns, 4), resident, most}), false, per_sm};
+    if (turns <= (backward ? kBackwardTurns : kForwardTurns) * splits || resident <= splits)
+        return {true, (int)splits, (int)splits, splits * p->images <= sms ? 1 : per_sm};
+    splits = std::min({ceil_div(turns, 4), resident, most});
+    return {false, (int)splits, (int)std::min(std::max(splits, ceil_div(turns, kApplyTurns)), texels), per_sm};
 }
 
 size_t align16(size_t n) { return (n + 15) / 16 * 16; }
 
-// Workspace: the barrier, group partials, channel partials.
+// Workspace: group partials, channel partials.
 struct Layout {
-    size_t groups_at, channels_at, total;
+    size_t channels_at, total;
 };
 
 Layout layout(const NtGroupNorm *p, const Plan &pl, bool backward)
 {
     Layout l;
-    l.groups_at = pl.cluster ? 0 : 16;
-    l.channels_at = l.groups_at + (pl.cluster ? 0 : align16((size_t)p->images * p->groups * pl.splits * sizeof(float2)));
+    l.channels_at = pl.cluster ? 0 : align16((size_t)p->images * p->groups * pl.splits * sizeof(float2));
     l.total = l.channels_at + (backward ? (size_t)p->images * pl.splits * p->channels * sizeof(float2) : 0);
     return l;
 }
@@ -97,15 +96,13 @@ cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
     L.p = *p;
     const int threads = backward ? kBackwardThreads : kForwardThreads, ring = backward ? kBackwardRing : kForwardRing;
     L.per = p->channels / p->groups;
-    L.splits = pl.splits;
-    L.cluster = pl.cluster;
+    L.parts = pl.splits;
     const bool even = flat(p->x, p, size) && flat(backward ? p->dy : p->y, p, size) && flat(backward ? p->dx : p->y, p, size);
     L.texels = p->height * p->width;
-    L.share = L.texels / L.splits;
-    L.extra = L.texels % L.splits;
+    L.part_share = L.texels / L.parts;
+    L.part_extra = L.texels % L.parts;
     L.inv_count = 1.f / ((float)L.texels * (float)L.per);
-    L.barrier = reinterpret_cast<unsigned int *>(ws);
-    L.groups_part = reinterpret_cast<float2 *>(ws + at.groups_at);
+    L.groups_part = reinterpret_cast<float2 *>(ws);
     L.channels_part = reinterpret_cast<float2 *>(ws + at.channels_at);
     const size_t most = 227 * 1024 / pl.per_sm - 1024;
     size_t smem = 0;
@@ -125,44 +122,36 @@ cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
         L.scratch = (int32_t)align16((2 * (size_t)p->groups + entries) * sizeof(float2));
         const size_t slot = (size_t)threads * v * size * (backward ? 2 : 1);
         const int64_t room = (int64_t)((most - L.scratch) / slot);
-        const int64_t slots = ceil_div(ceil_div(L.texels, L.splits), L.ty) * ceil_div(L.vectors, L.tx);
-        L.keep = (int32_t)(slots <= room ? slots : std::max<int64_t>(room - ring, 0));
-        smem = L.scratch + (slots <= room ? slots : L.keep + ring) * slot;
+        const int64_t slots = pl.cluster ? ceil_div(ceil_div(L.texels, pl.splits), L.ty) * ceil_div(L.vectors, L.tx) : ring + 1;
+        L.keep = !pl.cluster ? 0 : (int32_t)(slots <= room ? slots : std::max<int64_t>(room - ring, 0));
+        smem = L.scratch + (pl.cluster && slots <= room ? slots : L.keep + ring) * slot;
         if (smem <= most || v == 1) break;
     }
-
-    L.turns = L.share / L.ty;
-    L.left = L.share % L.ty;
     L.by_tx = (uint32_t)ceil_div(1 << 18, L.tx);
     const int units = whole ? L.per / v : L.per;
     L.by_group = units == 1 ? 0 : (uint32_t)ceil_div((int64_t)1 << 32, units);
 
-    const NormKernel kernel = backward ? backward_kernel(p->dtype, v, whole, even) : forward_kernel(p->dtype, v, whole, even);
-    cudaError_t e = set_smem_limit(reinterpret_cast<const void *>(kernel), 227 * 1024 - 1024);
-    if (e != cudaSuccess) return e;
+    // launches `kernel` with `splits` blocks an image
+    auto run = [&](NormKernel kernel, int splits, int cluster) {
+        L.splits = splits;
+        L.share = L.texels / splits;
+        L.extra = L.texels % splits;
+        L.turns = L.share / L.ty;
+        L.left = L.share % L.ty;
+        cudaError_t e = set_smem_limit(reinterpret_cast<const void *>(kernel), 227 * 1024 - 1024);
+        if (e == cudaSuccess && cluster > 8)
+            e = cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        return e == cudaSuccess ? launch_next(kernel, dim3((unsigned)splits, (unsigned)p->images), threads, smem, st, (unsigned)cluster, L) : e;
+    };
+    cudaError_t e;
     if (pl.cluster) {
-        if (pl.splits > 8) e = cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return e;
-        e = launch_next(kernel, dim3((unsigned)pl.splits, (unsigned)p->images), threads, smem, st, (unsigned)pl.splits, L);
+        e = run((backward ? backward_kernel : forward_kernel)(p->dtype, v, whole, even), pl.splits, pl.splits);
         if (e == cudaSuccess && backward && p->images > 1 && (p->dgamma || p->dbeta))
             e = launch_next(join_channels_kernel, dim3((unsigned)ceil_div(p->channels, kJoinWarps)), 32 * kJoinWarps, 0, st, 1, L);
         return e;
     }
-    // the blocks wait for one another: a cooperative launch, with its counter cleared in front of it
-    if ((e = cudaMemsetAsync(ws, 0, 16, st)) != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)pl.splits, (unsigned)p->images);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeCooperative;
-    attr[0].val.cooperative = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, L);
-    if (e == cudaSuccess) count_launch();
-    return e;
+    e = run((backward ? backward_sums_kernel : forward_sums_kernel)(p->dtype, v, whole, even), pl.splits, 1);
+    return e == cudaSuccess ? run((backward ? backward_apply_kernel : forward_apply_kernel)(p->dtype, v, whole, even), pl.applies, 1) : e;
 }
 
 nt_status check_map(const NtFeatureMap &f, const char *name, const NtGroupNorm *p, int size, bool written)
@@ -237,15 +226,6 @@ nt_status run(const NtGroupNorm *p, bool backward, nt_stream_t stream)
 }
 
 }  // namespace norm
-
-cudaError_t read_norm_status(uint32_t *status, bool clear)
-{
-    uint32_t a = 0, b = 0;
-    cudaError_t e = norm::read_forward_status(&a, clear);
-    if (e == cudaSuccess) e = norm::read_backward_status(&b, clear);
-    *status = a | b;
-    return e;
-}
 
 }  // namespace nt
 

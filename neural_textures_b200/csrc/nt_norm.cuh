@@ -2,18 +2,21 @@
 // nt_group_norm_backward); nt_norm_forward.cu and nt_norm_backward.cu instantiate it, nt_norm.cu
 // checks arguments and plans the launch.
 //
-// One launch makes two passes over a map, with a barrier between them:
+// Two passes over a map:
 //   1. sums.  `splits` thread blocks share an image; a thread keeps one vector of V channels and
 //      strides over texels.  Forward: count, mean and centred squares, each thread about its own
-//      first value and joined pairwise after that, so that a common offset costs no digits.
+//      first value and joined about common means after that, so that a common offset costs no digits.
 //      Backward: per channel sums of e = dy act'(z) and e h.
 //   2. the result, from the image's joined sums.
+// An image that a cluster of up to 16 blocks gets through quickly takes one launch: the blocks read each
+// other's sums from shared memory, and keep there what the first pass read as far as it goes.  Larger
+// ones take a launch for each pass, with the blocks' sums in the workspace; the second is set up under the
+// first, and starts with the texels read last, which are still in L2.  (One cooperative launch for both
+// passes, the blocks meeting at a barrier of the grid with 30 MB kept on chip, was slower: SMs of
+// different GPCs differ by half in bandwidth, so that at the barrier and at the end all waited for the
+// slowest: 79 us against 60 us for 1024 x 1024 x 64 fp16, 12 against 10 us where neither is long.)
 // A thread's vectors arrive by asynchronous copies in its own slots of shared memory, so that loads stay in
-// flight while it computes and no barrier is needed.  The slots hold a ring of a few vectors and, as far as
-// they go, the texels read first, for the second pass; that one begins with the texels read last, which
-// are still in L2.
-// Blocks of an image meet in a cluster (up to 16), where they read each other's sums from shared memory, or,
-// for large maps, at a barrier of the whole cooperative grid, with the sums in the workspace.
+// flight while it computes and no barrier is needed: a ring of a few vectors, and behind it what is kept.
 // All sums are joined in a fixed order.
 #pragma once
 
@@ -27,15 +30,15 @@ constexpr int kForwardRing = 4, kBackwardRing = 4;  // 64 and 96 KB in flight on
 constexpr int kBackwardThreads = 384;  // 84 registers a thread with two blocks on an SM: 64 spill
 constexpr int kMaxCluster = 16;
 constexpr int kMaxSplits = 320;  // thread blocks of an image
-constexpr uint32_t kSpinLimit = 1u << 24;
 
-static __device__ unsigned int g_norm_status;  // bit 0: the wait at the grid's barrier gave up
+// Both passes in one launch by a cluster, or a launch for each.
+enum Phase { kBoth, kSums, kApply };
 
 struct NormLaunch {
     NtGroupNorm p;
     int32_t per;        // channels of a group
-    int32_t splits;     // thread blocks of an image
-    int32_t cluster;    // 1: they form a cluster; 0: the grid meets at *barrier
+    int32_t splits;     // thread blocks of an image, in this launch
+    int32_t parts, part_share, part_extra;  // blocks of an image that made the sums, and their texels
     int32_t texels, vectors;  // vectors of V channels in a texel
     int32_t tx, ty;     // threads along channels and texels
     int32_t share, extra;   // texels of a block: share, the first `extra` blocks one more
@@ -45,9 +48,8 @@ struct NormLaunch {
     int32_t keep;       // vectors of a thread (of x, and of dy) that stay in shared memory, in front of its ring
     int32_t scratch;    // bytes of shared memory in front of them
     float inv_count;    // 1 / values of a group
-    float2 *groups_part;    // [image][group][split]
-    float2 *channels_part;  // [channel][image * split], backward
-    unsigned int *barrier;
+    float2 *groups_part;    // [image][group][part]
+    float2 *channels_part;  // [channel][image * part], backward
 };
 
 // V consecutive channels.
@@ -189,28 +191,10 @@ __device__ __forceinline__ float2 peer_f2(const float2 *mine, uint32_t rank)
 
 __device__ __forceinline__ void prefetch(const void *p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
 
-// All blocks of a cooperative launch; *counter is zero before it.
-__device__ __forceinline__ void grid_sync(unsigned int *counter, unsigned int *status)
-{
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        __threadfence();
-        atomicAdd(counter, 1u);
-        uint32_t seen = 0;
-        const uint32_t blocks = gridDim.x * gridDim.y;
-        for (uint32_t i = 0; i < kSpinLimit; ++i) {
-            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(counter) : "memory");
-            if (seen >= blocks) break;
-        }
-        if (seen < blocks) atomicOr(status, 1u);
-    }
-    __syncthreads();
-}
-
 // dgamma, dbeta of one channel from the blocks' sums: a warp.
 __device__ __forceinline__ void join_channel(const NormLaunch &L, int c)
 {
-    const int lane = threadIdx.x & 31, parts = L.p.images * L.splits;
+    const int lane = threadIdx.x & 31, parts = L.p.images * L.parts;
     float2 s = make_float2(0.f, 0.f);
     for (int i = lane; i < parts; i += 32) {
         const float2 v = __ldcg(L.channels_part + (int64_t)c * parts + i);
@@ -499,7 +483,7 @@ struct Threads {
 };
 
 // WHOLE: a vector lies in one group.  FLAT: the texels of every map are evenly spaced.
-template <class T, int V, bool WHOLE, bool FLAT, bool BACKWARD>
+template <class T, int V, bool WHOLE, bool FLAT, bool BACKWARD, Phase PHASE>
 __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads), WHOLE ? 2 : 1)
     norm_kernel(const __grid_constant__ NormLaunch L)
 {
@@ -508,7 +492,7 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
     const NtGroupNorm &p = L.p;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t n = blockIdx.y;
-    const int split = blockIdx.x;
+    const int split = PHASE == kApply ? L.splits - 1 - blockIdx.x : blockIdx.x;  // the texels read last first
     const int share = L.share, extra = L.extra;
     const int lo = split * share + min(split, extra), hi = lo + share + (split < extra);
     // shared memory: group results [groups], group partials [groups], scratch, kept vectors
@@ -523,11 +507,11 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
                                                (uint32_t)__cvta_generic_to_shared(smem + L.scratch) + tid * (uint32_t)sizeof(Vec<T, V>)};
     after_previous();
     int slot0 = 0;
-    for (int v0 = 0; v0 < L.vectors; v0 += L.tx, slot0 += most) {
+    for (int v0 = 0; PHASE != kApply && v0 < L.vectors; v0 += L.tx, slot0 += most) {
         const int vec = v0 + col;
         if (vec >= L.vectors || row >= L.ty) continue;
         const int near = min(max(L.keep - slot0, 0), mine);
-        if (!BACKWARD) {  // the second pass wants them soon
+        if (!BACKWARD && PHASE == kBoth) {  // the second pass wants them soon
             if (p.gamma) prefetch(p.gamma + vec * V);
             if (p.beta) prefetch(p.beta + vec * V);
         }
@@ -549,75 +533,75 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
             if (p.rstd) p.rstd[n * p.groups + g] = rstd;
         }
     };
-    float2 *const shared_out = L.cluster ? part : nullptr;
-    const int parts = p.images * L.splits;
-    if constexpr (!BACKWARD) {
-        const int step = WHOLE ? V : 1, entries = L.per / step, width = p.channels / step;
-        for (int g = warp; g < p.groups; g += kWarps) {
-            // two passes over the group's entries: the mean, from differences to one of them; the squares about it
-            const float2 *const of = scratch + g * entries;
-            const float origin = of[0].x;
-            float shift = 0.f, sum = 0.f;
-            for (int e = lane; e < L.ty * entries; e += 32) {
-                const int r = entries == 1 ? e : e / entries;
-                shift = fmaf((float)(turn + (r < left)) * step, of[r * (width - entries) + e].x - origin, shift);
+    const int blocks = p.images * L.splits;
+    if constexpr (PHASE != kApply) {
+        if constexpr (!BACKWARD) {
+            const int step = WHOLE ? V : 1, entries = L.per / step, width = p.channels / step;
+            for (int g = warp; g < p.groups; g += kWarps) {
+                // two passes over the group's entries: the mean, from differences to one of them; the squares about it
+                const float2 *const of = scratch + g * entries;
+                const float origin = of[0].x;
+                float shift = 0.f, sum = 0.f;
+                for (int e = lane; e < L.ty * entries; e += 32) {
+                    const int r = entries == 1 ? e : e / entries;
+                    shift = fmaf((float)(turn + (r < left)) * step, of[r * (width - entries) + e].x - origin, shift);
+                }
+                const float mean = origin + __fdividef(warp_sum_all(shift), (float)(hi - lo) * L.per);
+                for (int e = lane; e < L.ty * entries; e += 32) {
+                    const int r = entries == 1 ? e : e / entries;
+                    const float2 v = of[r * (width - entries) + e];
+                    sum += fmaf((float)(turn + (r < left)) * step * (v.x - mean), v.x - mean, v.y);
+                }
+                sum = warp_sum_all(sum);
+                if (lane == 0) {
+                    if (PHASE == kBoth && L.splits == 1) finish(g, mean, sum);
+                    else if (PHASE == kBoth) part[g] = make_float2(mean, sum);
+                    else L.groups_part[(n * p.groups + g) * L.splits + split] = make_float2(mean, sum);
+                }
             }
-            const float mean = origin + __fdividef(warp_sum_all(shift), (float)(hi - lo) * L.per);
-            for (int e = lane; e < L.ty * entries; e += 32) {
-                const int r = entries == 1 ? e : e / entries;
-                const float2 v = of[r * (width - entries) + e];
-                sum += fmaf((float)(turn + (r < left)) * step * (v.x - mean), v.x - mean, v.y);
+        } else {
+            // the rows of each channel, folded in halves
+            for (int rows = L.ty; rows > 1; rows = (rows + 1) >> 1) {
+                const int half = (rows + 1) >> 1;
+                for (int i = tid; i < (rows - half) * p.channels; i += NT) {
+                    const float2 v = scratch[half * p.channels + i];
+                    scratch[i].x += v.x;
+                    scratch[i].y += v.y;
+                }
+                __syncthreads();
             }
-            sum = warp_sum_all(sum);
-            if (lane == 0) {
-                if (L.splits == 1) finish(g, mean, sum);
-                else if (shared_out) shared_out[g] = make_float2(mean, sum);
-                else L.groups_part[(n * p.groups + g) * L.splits + split] = make_float2(mean, sum);
-            }
-        }
-    } else {
-        // the rows of each channel, folded in halves
-        for (int rows = L.ty; rows > 1; rows = (rows + 1) >> 1) {
-            const int half = (rows + 1) >> 1;
-            for (int i = tid; i < (rows - half) * p.channels; i += NT) {
-                const float2 v = scratch[half * p.channels + i];
-                scratch[i].x += v.x;
-                scratch[i].y += v.y;
-            }
-            __syncthreads();
-        }
-        if ((p.dgamma || p.dbeta) && (p.images > 1 || !L.cluster))
-            for (int c = tid; c < p.channels; c += NT) L.channels_part[(int64_t)c * parts + blockIdx.y * L.splits + blockIdx.x] = scratch[c];
-        for (int g = warp; g < p.groups; g += kWarps) {
-            float2 s = make_float2(0.f, 0.f);
-            for (int e = lane; e < L.per; e += 32) {
-                const int c = g * L.per + e;
-                const float w = p.gamma ? __ldg(p.gamma + c) : 1.f;
-                s.x = fmaf(w, scratch[c].x, s.x);
-                s.y = fmaf(w, scratch[c].y, s.y);
-            }
-            s = warp_sum(s);
-            if (lane == 0) {
-                if (L.splits == 1) stat[g] = s;
-                else if (shared_out) shared_out[g] = s;
-                else L.groups_part[(n * p.groups + g) * L.splits + split] = s;
+            if ((p.dgamma || p.dbeta) && (p.images > 1 || PHASE == kSums))
+                for (int c = tid; c < p.channels; c += NT) L.channels_part[(int64_t)c * blocks + blockIdx.y * L.splits + blockIdx.x] = scratch[c];
+            for (int g = warp; g < p.groups; g += kWarps) {
+                float2 s = make_float2(0.f, 0.f);
+                for (int e = lane; e < L.per; e += 32) {
+                    const int c = g * L.per + e;
+                    const float w = p.gamma ? __ldg(p.gamma + c) : 1.f;
+                    s.x = fmaf(w, scratch[c].x, s.x);
+                    s.y = fmaf(w, scratch[c].y, s.y);
+                }
+                s = warp_sum(s);
+                if (lane == 0) {
+                    if (PHASE == kBoth && L.splits == 1) stat[g] = s;
+                    else if (PHASE == kBoth) part[g] = s;
+                    else L.groups_part[(n * p.groups + g) * L.splits + split] = s;
+                }
             }
         }
     }
-    if (!L.cluster) grid_sync(L.barrier, &g_norm_status);
-    else if (L.splits > 1) cluster_sync();
-    else __syncthreads();
+    if constexpr (PHASE == kSums) return;
+    if (PHASE == kBoth && L.splits > 1) cluster_sync();
+    else if (PHASE == kBoth) __syncthreads();
 
     // ---- the image's sums ----
-    for (int g = warp; g < p.groups && L.splits > 1; g += kWarps) {
+    const int parts = L.parts;
+    for (int g = warp; g < p.groups && (PHASE == kApply || parts > 1); g += kWarps) {
         float2 v[kMaxSplits / 32];
 #pragma unroll
         for (int k = 0; k < kMaxSplits / 32; ++k) {
             const int i = lane + 32 * k;
             v[k] = make_float2(0.f, 0.f);
-            if (i < L.splits)
-                v[k] = L.cluster ? peer_f2(part + g, i)
-                                 : __ldcg(L.groups_part + (n * p.groups + g) * L.splits + i);
+            if (i < parts) v[k] = PHASE == kBoth ? peer_f2(part + g, i) : __ldcg(L.groups_part + (n * p.groups + g) * parts + i);
         }
         float a = 0.f, b = 0.f;
         if (BACKWARD) {
@@ -630,17 +614,17 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
             const float origin = __shfl_sync(0xffffffffu, v[0].x, 0);
 #pragma unroll
             for (int k = 0; k < kMaxSplits / 32; ++k)
-                if (lane + 32 * k < L.splits) a = fmaf((float)(share + (lane + 32 * k < extra)), v[k].x - origin, a);
+                if (lane + 32 * k < parts) a = fmaf((float)(L.part_share + (lane + 32 * k < L.part_extra)), v[k].x - origin, a);
             const float mean = origin + __fdividef(warp_sum_all(a), (float)L.texels);
 #pragma unroll
             for (int k = 0; k < kMaxSplits / 32; ++k)
-                if (lane + 32 * k < L.splits)
-                    b += fmaf((float)(share + (lane + 32 * k < extra)) * L.per * (v[k].x - mean), v[k].x - mean, v[k].y);
+                if (lane + 32 * k < parts)
+                    b += fmaf((float)(L.part_share + (lane + 32 * k < L.part_extra)) * L.per * (v[k].x - mean), v[k].x - mean, v[k].y);
             b = warp_sum_all(b);
             if (lane == 0) finish(g, mean, b);
         }
     }
-    if (BACKWARD && L.cluster && p.images == 1 && (p.dgamma || p.dbeta))
+    if (BACKWARD && PHASE == kBoth && p.images == 1 && (p.dgamma || p.dbeta))
         for (int c = split * NT + tid; c < p.channels; c += L.splits * NT) {
             float2 s = scratch[c];
             if (L.splits > 1) {
@@ -654,17 +638,17 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
             if (p.dbeta) p.dbeta[c] = s.x;
             if (p.dgamma) p.dgamma[c] = s.y;
         }
-    if (L.cluster && L.splits > 1) cluster_sync();  // a block's sums stay until its peers have read them
-    else if (L.splits > 1) __syncthreads();
-    if (BACKWARD && !L.cluster && (p.dgamma || p.dbeta))
-        for (int c = warp * parts + blockIdx.y * L.splits + blockIdx.x; c < p.channels; c += kWarps * parts) join_channel(L, c);
+    if (PHASE == kBoth && L.splits > 1) cluster_sync();  // a block's sums stay until its peers have read them
+    else if (PHASE == kApply) __syncthreads();
+    if (BACKWARD && PHASE == kApply && (p.dgamma || p.dbeta))
+        for (int c = warp * blocks + blockIdx.y * L.splits + blockIdx.x; c < p.channels; c += kWarps * blocks) join_channel(L, c);
 
     for (int v0 = (L.vectors - 1) / L.tx * L.tx; v0 >= 0; v0 -= L.tx) {
-        slot0 -= most;
+        if (PHASE == kBoth) slot0 -= most;
         const int vec = v0 + col;
         if (vec >= L.vectors || mine == 0) continue;
         const int near = min(max(L.keep - slot0, 0), mine);
-        const bool fresh = v0 + L.tx < L.vectors;  // the ring holds the last columns of pass 1
+        const bool fresh = PHASE == kApply || v0 + L.tx < L.vectors;  // else the ring holds the last columns of pass 1
         switch (p.activation) {
         case NT_ACT_RELU: th.template second<NT_ACT_RELU>(vec * V, mine, near, slot0, fresh); break;
         case NT_ACT_SILU: th.template second<NT_ACT_SILU>(vec * V, mine, near, slot0, fresh); break;
@@ -676,45 +660,39 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
 
 using NormKernel = void (*)(NormLaunch);
 
-template <class T, int V, bool BACKWARD>
+template <class T, int V, bool BACKWARD, Phase PHASE>
 NormKernel pick_whole(bool whole, bool flat)
 {
     if constexpr (V > 1)
-        if (!whole) return flat ? norm_kernel<T, V, false, true, BACKWARD> : norm_kernel<T, V, false, false, BACKWARD>;
-    return flat ? norm_kernel<T, V, true, true, BACKWARD> : norm_kernel<T, V, true, false, BACKWARD>;
+        if (!whole) return flat ? norm_kernel<T, V, false, true, BACKWARD, PHASE> : norm_kernel<T, V, false, false, BACKWARD, PHASE>;
+    return flat ? norm_kernel<T, V, true, true, BACKWARD, PHASE> : norm_kernel<T, V, true, false, BACKWARD, PHASE>;
 }
 
-template <class T, bool BACKWARD>
+template <class T, bool BACKWARD, Phase PHASE>
 NormKernel pick_width(int v, bool whole, bool flat)
 {
     if constexpr (sizeof(T) == 2)
-        if (v == 8) return pick_whole<T, 8, BACKWARD>(whole, flat);
-    return v == 4   ? pick_whole<T, 4, BACKWARD>(whole, flat)
-           : v == 2 ? pick_whole<T, 2, BACKWARD>(whole, flat)
-                    : pick_whole<T, 1, BACKWARD>(whole, flat);
+        if (v == 8) return pick_whole<T, 8, BACKWARD, PHASE>(whole, flat);
+    return v == 4   ? pick_whole<T, 4, BACKWARD, PHASE>(whole, flat)
+           : v == 2 ? pick_whole<T, 2, BACKWARD, PHASE>(whole, flat)
+                    : pick_whole<T, 1, BACKWARD, PHASE>(whole, flat);
 }
 
-template <bool BACKWARD>
+template <bool BACKWARD, Phase PHASE>
 NormKernel pick_kernel(int32_t dtype, int v, bool whole, bool flat)
 {
-    return dtype == NT_DTYPE_F16    ? pick_width<__half, BACKWARD>(v, whole, flat)
-           : dtype == NT_DTYPE_BF16 ? pick_width<__nv_bfloat16, BACKWARD>(v, whole, flat)
-                                    : pick_width<float, BACKWARD>(v, whole, flat);
+    return dtype == NT_DTYPE_F16    ? pick_width<__half, BACKWARD, PHASE>(v, whole, flat)
+           : dtype == NT_DTYPE_BF16 ? pick_width<__nv_bfloat16, BACKWARD, PHASE>(v, whole, flat)
+                                    : pick_width<float, BACKWARD, PHASE>(v, whole, flat);
 }
 
+// One per file that instantiates kernels: [forward, backward] x [both passes, sums, result].
 NormKernel forward_kernel(int32_t dtype, int v, bool whole, bool flat);
+NormKernel forward_sums_kernel(int32_t dtype, int v, bool whole, bool flat);
+NormKernel forward_apply_kernel(int32_t dtype, int v, bool whole, bool flat);
 NormKernel backward_kernel(int32_t dtype, int v, bool whole, bool flat);
-
-// This file's status word, read and cleared on request.
-static inline cudaError_t read_status(uint32_t *status, bool clear)
-{
-    cudaError_t e = cudaMemcpyFromSymbol(status, g_norm_status, sizeof(uint32_t));
-    if (e != cudaSuccess || !clear) return e;
-    const uint32_t zero = 0;
-    return cudaMemcpyToSymbol(g_norm_status, &zero, sizeof(uint32_t));
-}
-cudaError_t read_forward_status(uint32_t *status, bool clear);
-cudaError_t read_backward_status(uint32_t *status, bool clear);
+NormKernel backward_sums_kernel(int32_t dtype, int v, bool whole, bool flat);
+NormKernel backward_apply_kernel(int32_t dtype, int v, bool whole, bool flat);
 
 }  // namespace norm
 }  // namespace nt

@@ -1,0 +1,8 @@
+// nt_norm_backward_apply.cu -- the backward group-norm kernels: the result.
+#include "nt_norm.cuh"
+
+namespace nt {
+namespace norm {
+NormKernel backward_apply_kernel(int32_t dtype, int v, bool whole, bool flat) { return pick_kernel<true, kApply>(dtype, v, whole, flat); }
+}  // namespace norm
+}  // namespace nt

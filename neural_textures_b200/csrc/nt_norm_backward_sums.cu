@@ -1,0 +1,8 @@
+// nt_norm_backward_sums.cu -- the backward group-norm kernels: the sums.
+#include "nt_norm.cuh"
+
+namespace nt {
+namespace norm {
+NormKernel backward_sums_kernel(int32_t dtype, int v, bool whole, bool flat) { return pick_kernel<true, kSums>(dtype, v, whole, flat); }
+}  // namespace norm
+}  // namespace nt

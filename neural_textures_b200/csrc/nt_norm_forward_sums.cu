@@ -1,0 +1,8 @@
+// nt_norm_forward_sums.cu -- the forward group-norm kernels: the sums.
+#include "nt_norm.cuh"
+
+namespace nt {
+namespace norm {
+NormKernel forward_sums_kernel(int32_t dtype, int v, bool whole, bool flat) { return pick_kernel<false, kSums>(dtype, v, whole, flat); }
+}  // namespace norm
+}  // namespace nt

@@ -972,15 +972,14 @@ extern "C" nt_status nt_wait_timeout_selftest(uint32_t tries)
 extern "C" nt_status nt_read_device_status(uint32_t *status, int32_t clear)
 {
     if (!status) return NT_ERR_INVALID_ARG;
-    uint32_t train = 0, decode = 0, product = 0, norm = 0;
+    uint32_t train = 0, decode = 0, product = 0;
     if (cudaMemcpyFromSymbol(&train, nt::g_device_status, sizeof(uint32_t)) != cudaSuccess) return NT_ERR_CUDA;
     if (nt::read_decode_status(&decode, clear != 0) != cudaSuccess) return NT_ERR_CUDA;
     if (nt::read_product_status(&product, clear != 0) != cudaSuccess) return NT_ERR_CUDA;
-    if (nt::read_norm_status(&norm, clear != 0) != cudaSuccess) return NT_ERR_CUDA;
     if (clear) {
         const uint32_t zero = 0;
         if (cudaMemcpyToSymbol(nt::g_device_status, &zero, sizeof(uint32_t)) != cudaSuccess) return NT_ERR_CUDA;
     }
-    *status = train | decode | product | norm;
+    *status = train | decode | product;
     return NT_OK;
 }
