@@ -12,9 +12,9 @@
 // other's sums from shared memory, and keep there what the first pass read as far as it goes.  Larger
 // ones take a launch for each pass, with the blocks' sums in the workspace; the second is set up under the
 // first, and starts with the texels read last, which are still in L2.  (One cooperative launch for both
-// passes, the blocks meeting at a barrier of the grid with 30 MB kept on chip, was slower: SMs of
-// different GPCs differ by half in bandwidth, so that at the barrier and at the end all waited for the
-// slowest: 79 us against 60 us for 1024 x 1024 x 64 fp16, 12 against 10 us where neither is long.)
+// passes, the blocks meeting at a barrier of the grid with 24 MB kept on chip, was slower: SMs of
+// different GPCs differ by half in bandwidth, and all waited for the slowest twice: 73 us against 68 us for
+// 1024 x 1024 x 64 fp16, 17.6 against 9.8 us for 256 x 256 x 64.)
 // A thread's vectors arrive by asynchronous copies in its own slots of shared memory, so that loads stay in
 // flight while it computes and no barrier is needed: a ring of a few vectors, and behind it what is kept.
 // All sums are joined in a fixed order.
@@ -26,7 +26,8 @@ namespace nt {
 namespace norm {
 
 constexpr int kForwardThreads = 512;
-constexpr int kForwardRing = 4, kBackwardRing = 4;  // 64 and 96 KB in flight on an SM cover the latency of HBM
+// Vectors in flight for each thread, 64 and 72 KB on an SM; 8 and 6 of them for the sums changed nothing.
+constexpr int kForwardRing = 4, kBackwardRing = 4;
 constexpr int kBackwardThreads = 384;  // 84 registers a thread with two blocks on an SM: 64 spill
 constexpr int kMaxCluster = 16;
 constexpr int kMaxSplits = 320;  // thread blocks of an image
@@ -209,7 +210,7 @@ __device__ __forceinline__ void join_channel(const NormLaunch &L, int c)
 }
 
 // What a thread's passes share.
-template <class T, int V, bool WHOLE, bool FLAT, bool BACKWARD>
+template <class T, int V, bool WHOLE, bool FLAT, bool BACKWARD, Phase PHASE>
 struct Threads {
     static constexpr int P = (V + 1) / 2;
     static constexpr int NT = BACKWARD ? kBackwardThreads : kForwardThreads;
@@ -276,7 +277,7 @@ struct Threads {
         }
     };
 
-    // use(slot) for texels 0 .. count - 1.  Afterwards the last kDepth of them are still in the ring, texel i in
+    // use(slot, i) for texels 0 .. count - 1.  Afterwards the last kDepth of them are still in the ring, texel i in
     // slot (i - near) % kDepth.
     template <class Use>
     __device__ __forceinline__ void each_forth(int c, int count, int near, int slot0, Use use) const
@@ -293,12 +294,12 @@ struct Threads {
         }
         fetch_wait<kDepth>();
 #pragma unroll 2
-        for (int i = 0; i < near; ++i) use(keep + i * kSlot);
+        for (int i = 0; i < near; ++i) use(keep + i * kSlot, i);
 #pragma unroll 2
         for (int i = near; i < count; ++i) {
             const uint32_t slot = ring + ((i - near) & (kDepth - 1)) * kSlot;
             fetch_wait<kDepth - 1>();
-            use(slot);
+            use(slot, i);
             if (i + kDepth < count) src.get(slot, i + kDepth, again);
             fetch_commit();
         }
@@ -331,12 +332,60 @@ struct Threads {
         for (int i = near - 1; i >= 0; --i) use(keep + i * kSlot, i);
     }
 
+    // use(slot, i) for every texel, nothing kept: texels 0 .. count - 1, or backwards.  The ring's slots are constants of an
+    // unrolled loop.
+    template <bool REVERSED, class Use>
+    __device__ __forceinline__ void each_fresh(int c, int count, Use use) const
+    {
+        const Source src(*this, c);
+        const uint64_t policy = REVERSED ? policy_once() : policy_again();
+        auto texel = [&](int i) { return REVERSED ? count - 1 - i : i; };
+#pragma unroll
+        for (int u = 0; u < kDepth; ++u) {
+            if (u < count) src.get(kept + u * kSlot, texel(u), policy);
+            fetch_commit();
+        }
+        int i = 0;
+        for (; i + 2 * kDepth <= count; i += kDepth) {
+#pragma unroll
+            for (int u = 0; u < kDepth; ++u) {
+                fetch_wait<kDepth - 1>();
+                use(kept + u * kSlot, texel(i + u));
+                src.get(kept + u * kSlot, texel(i + u + kDepth), policy);
+                fetch_commit();
+            }
+        }
+#pragma unroll 1
+        for (; i < count; i += kDepth) {
+#pragma unroll
+            for (int u = 0; u < kDepth; ++u) {
+                fetch_wait<kDepth - 1>();
+                if (i + u < count) use(kept + u * kSlot, texel(i + u));
+                if (i + u + kDepth < count) src.get(kept + u * kSlot, texel(i + u + kDepth), policy);
+                fetch_commit();
+            }
+        }
+    }
+
+    template <class Use>
+    __device__ __forceinline__ void every_forth(int c, int count, int near, int slot0, Use use) const
+    {
+        if constexpr (PHASE == kSums) each_fresh<false>(c, count, use);
+        else each_forth(c, count, near, slot0, use);
+    }
+    template <class Use>
+    __device__ __forceinline__ void every_back(int c, int count, int near, int slot0, bool fresh, Use use) const
+    {
+        if constexpr (PHASE == kApply) each_fresh<true>(c, count, use);
+        else each_back(c, count, near, slot0, fresh, use);
+    }
+
     // ---- pass 1 ----
     __device__ __forceinline__ void forward_sums(int c, int count, int near, int slot0) const
     {
         float2 pivot[P] = {}, s1[P] = {}, s2[P] = {};
         bool begun = false;
-        each_forth(c, count, near, slot0, [&](uint32_t slot) {
+        every_forth(c, count, near, slot0, [&](uint32_t slot, int) {
             float2 f[P];
             unpack<T, V>(read_slot<T, V>(slot), f);
             if (!begun) {
@@ -396,7 +445,7 @@ struct Threads {
         statistics(c, shift, rstd);
         channels(L.p.gamma, 1.f, c, gamma);
         channels(L.p.beta, 0.f, c, beta);
-        each_forth(c, count, near, slot0, [&](uint32_t slot) {
+        every_forth(c, count, near, slot0, [&](uint32_t slot, int) {
             float2 fa[P], fb[P];
             unpack<T, V>(read_slot<T, V>(slot), fa);
             unpack<T, V>(read_slot<T, V>(slot + kNext), fb);
@@ -428,7 +477,7 @@ struct Threads {
             scale[j] = __fmul2_rn(scale[j], make_float2(a.y, b.y));
         }
         const Path out(*this, L.p.y, c);
-        each_back(c, count, near, slot0, fresh, [&](uint32_t slot, int i) {
+        every_back(c, count, near, slot0, fresh, [&](uint32_t slot, int i) {
             float2 f[P];
             unpack<T, V>(read_slot<T, V>(slot), f);
 #pragma unroll
@@ -453,7 +502,7 @@ struct Threads {
             k2[j] = make_float2(-a.y * L.inv_count, -b.y * L.inv_count);
         }
         const Path out(*this, L.p.dx, c);
-        each_back(c, count, near, slot0, fresh, [&](uint32_t slot, int i) {
+        every_back(c, count, near, slot0, fresh, [&](uint32_t slot, int i) {
             float2 fa[P], fb[P];
             unpack<T, V>(read_slot<T, V>(slot), fa);
             unpack<T, V>(read_slot<T, V>(slot + kNext), fb);
@@ -502,7 +551,7 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
     if (left == L.ty) ++turn, left = 0;
     const int mine = row < L.ty ? turn + (row < left) : 0;  // texels of this thread
     const int most = turn + (left > 0);                     // and of any
-    const Threads<T, V, WHOLE, FLAT, BACKWARD> th = {L,    n,       lo, row, col, mine,
+    const Threads<T, V, WHOLE, FLAT, BACKWARD, PHASE> th = {L,    n,       lo, row, col, mine,
                                                stat, scratch,
                                                (uint32_t)__cvta_generic_to_shared(smem + L.scratch) + tid * (uint32_t)sizeof(Vec<T, V>)};
     after_previous();
