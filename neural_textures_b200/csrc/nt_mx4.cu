@@ -145,8 +145,10 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QuantizeL
 
 // Columns along the memory (a transposed matrix): lanes along the rows, so that a warp's load of one column is
 // contiguous; a thread quantises 32 columns of its row, 16 bytes of codes, without any exchange.  PAIRS: of two
-// neighbouring rows of a 16-bit matrix, for loads of 4 bytes.
-constexpr int kColumnsGroup = 64;  // columns of a thread block, twice that for pairs
+// neighbouring rows of a 16-bit matrix, for loads of 4 bytes.  The warps of a block lie along the rows: 1 KB of every
+// column rather than 256 bytes of four times the columns (8190 x 8192 fp16: 61.3 -> 59.5 us).
+constexpr int kColumnsGroup = 32;  // columns of a thread block
+constexpr int kColumnsTiles = 2;   // row tiles of a thread block, twice that for pairs
 
 template <class T, int BLOCK>
 __device__ __forceinline__ void quantize_column_run(const QuantizeLaunch &p, const T (&v)[32], int64_t row, int64_t c0)
@@ -166,7 +168,7 @@ __device__ __forceinline__ void quantize_column_run(const QuantizeLaunch &p, con
     if (row < p.rows && c0 < row_pitch(p.cols) * 2)
         *reinterpret_cast<uint4 *>(p.data + row * p.pitch + (c0 >> 1)) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
     const int k = (int)(c0 / BLOCK);  // first block
-    if ((k >> 2) < p.tiles) {  // rows past the matrix too: their scales are 0
+    if ((k >> 2) < p.tiles && (row & ~127) < p.rows) {  // rows past the matrix too: their scales are 0
         uint8_t *at = p.scales + ((row >> 7) * p.tiles + (k >> 2)) * kTileBytes + (row & 31) * 16 + (row >> 5 & 3) * 4 + (k & 3);
         if (BLOCK == 16) *reinterpret_cast<uint16_t *>(at) = (uint16_t)bytes;
         else *at = (uint8_t)bytes;
@@ -178,11 +180,9 @@ __global__ void __launch_bounds__(kThreads) quantize_columns_kernel(const Quanti
 {
     after_previous();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t tile = blockIdx.x / p.groups;
-    const int group = blockIdx.x % p.groups;
+    const int64_t band = blockIdx.x / p.groups, c0 = (int64_t)(blockIdx.x % p.groups) * kColumnsGroup;
     if constexpr (PAIRS) {
-        const int64_t row = tile * kTileRows + (warp & 1) * 64 + 2 * lane;
-        const int64_t c0 = (int64_t)group * 2 * kColumnsGroup + (warp >> 1) * 32;
+        const int64_t row = band * 2 * kColumnsTiles * kTileRows + warp * 64 + 2 * lane;
         const T *src = static_cast<const T *>(p.src) + row;
         uint32_t w[32];
 #pragma unroll
@@ -201,8 +201,7 @@ __global__ void __launch_bounds__(kThreads) quantize_columns_kernel(const Quanti
             quantize_column_run<T, BLOCK>(p, v, row + h, c0);
         }
     } else {
-        const int64_t row = tile * kTileRows + (warp & 3) * 32 + lane;
-        const int64_t c0 = (int64_t)group * kColumnsGroup + (warp >> 2) * 32;
+        const int64_t row = band * kColumnsTiles * kTileRows + warp * 32 + lane;
         const T *src = static_cast<const T *>(p.src) + row;
         alignas(4) T v[32];
 #pragma unroll
@@ -218,9 +217,9 @@ cudaError_t launch_quantize(QuantizeLaunch p, cudaStream_t st)
     const bool unit = p.col_stride == 1 || p.cols == 1, columns = !unit && p.row_stride == 1;
     // a scale tile's padding is written too: whole tiles of 4 blocks
     const bool pairs = sizeof(T) == 2 && is_aligned(p.src, 4) && p.col_stride % 2 == 0;
-    const int64_t width = columns ? (pairs ? 2 : 1) * kColumnsGroup : kGroupCols;
+    const int64_t width = columns ? kColumnsGroup : kGroupCols, height = columns ? (pairs ? 2 : 1) * kColumnsTiles * kTileRows : kTileRows;
     p.groups = (int32_t)(((int64_t)p.tiles * 4 * BLOCK + width - 1) / width);
-    int64_t blocks = ((int64_t)p.rows + kTileRows - 1) / kTileRows * p.groups;
+    int64_t blocks = (p.rows + height - 1) / height * p.groups;
     if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
     const bool vec = unit && is_aligned(p.src, 16) && (p.rows == 1 || p.row_stride * sizeof(T) % 16 == 0);
     void (*kernel)(QuantizeLaunch) = quantize_rows_kernel<T, BLOCK, kStrided, false>;
