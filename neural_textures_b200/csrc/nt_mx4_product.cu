@@ -321,23 +321,28 @@ __device__ __forceinline__ void epilogue_rows(const Output &p, const CUtensorMap
             continue;
         }
         __syncwarp();
-        const int rows = (int)min((int64_t)32, p.l_rows - m0), cols = min(min(width, p.bn - c0), p.c_rows - n0);
-        for (int r0 = 0; r0 < rows; r0 += 4)
-            for (int c = lane; c < cols; c += 32) {
-                uint32_t v[4];
+        // rows of d that no tensor map takes: a row at a time, 4 bytes a lane where its address allows it, eight in flight
+        const int rows = (int)min((int64_t)32, p.l_rows - m0), bytes = min(min(width, p.bn - c0), p.c_rows - n0) * size;
+        uint8_t *const dst = static_cast<uint8_t *>(p.d) + (m0 * p.row_stride + n0) * size;
+        const int64_t pitch = p.row_stride * size;
+        const bool words = ((reinterpret_cast<uintptr_t>(p.d) | (uintptr_t)pitch) & 3) == 0;
+        for (int r0 = 0; r0 < rows; r0 += 8) {
+            uint32_t v[8];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint8_t *from = mine + (r0 + r) * 128 + (((c * size >> 4) ^ (r0 + r & 7)) << 4) + (c * size & 15);
-                    v[r] = size == 4 ? *reinterpret_cast<const uint32_t *>(from) : *reinterpret_cast<const uint16_t *>(from);
-                }
+            for (int r = 0; r < 8; ++r)
+                v[r] = *reinterpret_cast<const uint32_t *>(mine + (r0 + r) * 128 + (((lane >> 2) ^ r) << 4) + (lane & 3) * 4);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (r0 + r >= rows) break;
-                    const int64_t at = (m0 + r0 + r) * p.row_stride + n0 + c;
-                    if (size == 4) static_cast<uint32_t *>(p.d)[at] = v[r];
-                    else static_cast<uint16_t *>(p.d)[at] = (uint16_t)v[r];
+            for (int r = 0; r < 8; ++r) {
+                uint8_t *const at = dst + (r0 + r) * pitch + 4 * lane;
+                if (r0 + r >= rows || 4 * lane >= bytes) continue;
+                if (words && 4 * lane + 4 <= bytes) {
+                    *reinterpret_cast<uint32_t *>(at) = v[r];
+                } else {  // 16-bit values
+                    *reinterpret_cast<uint16_t *>(at) = (uint16_t)v[r];
+                    if (4 * lane + 4 <= bytes) *reinterpret_cast<uint16_t *>(at + 2) = (uint16_t)(v[r] >> 16);
                 }
             }
+        }
         __syncwarp();
     }
 }

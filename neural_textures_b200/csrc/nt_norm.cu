@@ -38,9 +38,9 @@ Plan plan(const NtGroupNorm *p, bool backward)
 {
     const int sms = sm_count(), threads = backward ? kBackwardThreads : kForwardThreads;
     int v = 16 / layer_dtype_size(p->dtype);
-    const bool whole = p->channels / p->groups % v == 0;
-    const int per_sm = whole && p->channels <= 2048 ? 2 : 1;
     while (p->channels % v) v /= 2;
+    const bool light = p->channels / p->groups % v == 0 || v <= 4;  // kernels that two blocks of fit an SM's registers
+    const int per_sm = light && p->channels <= 2048 ? 2 : 1;
     const int64_t texels = (int64_t)p->height * p->width, turns = ceil_div(texels * (p->channels / v), threads);
     const int64_t most = std::min<int64_t>(texels, kMaxSplits);
     const int largest = (int64_t)p->images * kMaxCluster <= sms * 7 / 8 ? kMaxCluster : 8;  // of 16: one in most of the GPCs
@@ -68,16 +68,10 @@ Layout layout(const NtGroupNorm *p, const Plan &pl, bool backward)
     return l;
 }
 
-// Widest vector that every map's addresses allow.
-int vector_width(const NtGroupNorm *p, int size, bool backward)
+// Whether vectors of v channels are aligned in a map.
+bool vectors_aligned(const NtFeatureMap &f, int v, int size)
 {
-    for (int v = 16 / size; v > 1; v /= 2) {
-        bool ok = p->channels % v == 0;
-        for (const NtFeatureMap *f : {&p->x, backward ? &p->dy : &p->y, backward ? &p->dx : &p->y})
-            ok = ok && is_aligned(f->data, v * size) && f->image_stride % v == 0 && f->row_stride % v == 0 && f->texel_stride % v == 0;
-        if (ok) return v;
-    }
-    return 1;
+    return is_aligned(f.data, v * size) && f.image_stride % v == 0 && f.row_stride % v == 0 && f.texel_stride % v == 0;
 }
 
 // Whether a map's texels are evenly spaced, `ty` of them by less than 2^31 bytes.
@@ -106,7 +100,8 @@ cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
     L.channels_part = reinterpret_cast<float2 *>(ws + at.channels_at);
     const size_t most = 227 * 1024 / pl.per_sm - 1024;
     size_t smem = 0;
-    int v = vector_width(p, size, backward);
+    int v = 16 / size;
+    while (p->channels % v) v /= 2;
     bool whole = true;
     for (;; v /= 2) {  // narrower vectors where the sums of very many groups leave no room for the ring
         whole = L.per % v == 0;
@@ -127,6 +122,9 @@ cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
         smem = L.scratch + (pl.cluster && slots <= room ? slots : L.keep + ring) * slot;
         if (smem <= most || v == 1) break;
     }
+    L.aligned = (vectors_aligned(p->x, v, size) ? kXAligned : 0) | (!backward || vectors_aligned(p->dy, v, size) ? kDyAligned : 0) |
+                (vectors_aligned(backward ? p->dx : p->y, v, size) ? kOutAligned : 0);
+    const bool regular = even && L.aligned == (kXAligned | kDyAligned | kOutAligned);
     L.by_tx = (uint32_t)ceil_div(1 << 18, L.tx);
     const int units = whole ? L.per / v : L.per;
     L.by_group = units == 1 ? 0 : (uint32_t)ceil_div((int64_t)1 << 32, units);
@@ -145,13 +143,13 @@ cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
     };
     cudaError_t e;
     if (pl.cluster) {
-        e = run((backward ? backward_kernel : forward_kernel)(p->dtype, v, whole, even), pl.splits, pl.splits);
+        e = run((backward ? backward_kernel : forward_kernel)(p->dtype, v, whole, regular), pl.splits, pl.splits);
         if (e == cudaSuccess && backward && p->images > 1 && (p->dgamma || p->dbeta))
             e = launch_next(join_channels_kernel, dim3((unsigned)ceil_div(p->channels, kJoinWarps)), 32 * kJoinWarps, 0, st, 1, L);
         return e;
     }
-    e = run((backward ? backward_sums_kernel : forward_sums_kernel)(p->dtype, v, whole, even), pl.splits, 1);
-    return e == cudaSuccess ? run((backward ? backward_apply_kernel : forward_apply_kernel)(p->dtype, v, whole, even), pl.applies, 1) : e;
+    e = run((backward ? backward_sums_kernel : forward_sums_kernel)(p->dtype, v, whole, regular), pl.splits, 1);
+    return e == cudaSuccess ? run((backward ? backward_apply_kernel : forward_apply_kernel)(p->dtype, v, whole, regular), pl.applies, 1) : e;
 }
 
 nt_status check_map(const NtFeatureMap &f, const char *name, const NtGroupNorm *p, int size, bool written)

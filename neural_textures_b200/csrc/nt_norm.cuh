@@ -32,6 +32,8 @@ constexpr int kBackwardThreads = 384;  // 84 registers a thread with two blocks 
 constexpr int kMaxCluster = 16;
 constexpr int kMaxSplits = 320;  // thread blocks of an image
 
+enum { kXAligned = 1, kDyAligned = 2, kOutAligned = 4 };  // NormLaunch.aligned
+
 // Both passes in one launch by a cluster, or a launch for each.
 enum Phase { kBoth, kSums, kApply };
 
@@ -40,6 +42,7 @@ struct NormLaunch {
     int32_t per;        // channels of a group
     int32_t splits;     // thread blocks of an image, in this launch
     int32_t parts, part_share, part_extra;  // blocks of an image that made the sums, and their texels
+    int32_t aligned;    // maps whose vectors are aligned
     int32_t texels, vectors;  // vectors of V channels in a texel
     int32_t tx, ty;     // threads along channels and texels
     int32_t share, extra;   // texels of a block: share, the first `extra` blocks one more
@@ -85,6 +88,22 @@ __device__ __forceinline__ void fetch(uint32_t to, const char *p, uint64_t polic
         asm volatile("cp.async.ca.shared.global.L2::cache_hint [%0], [%1], %2, %3;" ::"r"(to), "l"(p), "n"(bytes), "l"(policy) : "memory");
     else
         asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(*reinterpret_cast<const uint16_t *>(p)) : "memory");
+}
+
+// The same of a vector that is aligned to its elements only.
+template <class T, int V>
+__device__ __forceinline__ void fetch_each(uint32_t to, const char *p, uint64_t policy)
+{
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) fetch<T, 1>(to + 4 * i, p + 4 * i, policy);
+    } else {
+        uint16_t v[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = reinterpret_cast<const uint16_t *>(p)[i];
+#pragma unroll
+        for (int i = 0; i < V; ++i) asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + 2 * i), "h"(v[i]) : "memory");
+    }
 }
 
 template <class T, int V>
@@ -210,7 +229,7 @@ __device__ __forceinline__ void join_channel(const NormLaunch &L, int c)
 }
 
 // What a thread's passes share.
-template <class T, int V, bool WHOLE, bool FLAT, bool BACKWARD, Phase PHASE>
+template <class T, int V, bool WHOLE, bool REGULAR, bool BACKWARD, Phase PHASE>
 struct Threads {
     static constexpr int P = (V + 1) / 2;
     static constexpr int NT = BACKWARD ? kBackwardThreads : kForwardThreads;
@@ -230,12 +249,12 @@ struct Threads {
         __device__ __forceinline__ Path(const Threads &t, const NtFeatureMap &f, int c) : t(t), f(f)
         {
             at = static_cast<char *>(f.data) + (t.n * f.image_stride + c) * (int64_t)sizeof(T);
-            if (FLAT) at += (t.lo + t.row) * f.texel_stride * (int64_t)sizeof(T);
+            if (REGULAR) at += (t.lo + t.row) * f.texel_stride * (int64_t)sizeof(T);
             step = (int)(t.L.ty * f.texel_stride * (int64_t)sizeof(T));
         }
         __device__ __forceinline__ char *operator()(int i) const
         {
-            if (FLAT) return at + (int64_t)i * step;
+            if (REGULAR) return at + (int64_t)i * step;
             const int k = t.lo + t.row + i * t.L.ty, y = k / t.L.p.width, x = k - y * t.L.p.width;
             return at + (y * f.row_stride + x * f.texel_stride) * (int64_t)sizeof(T);
         }
@@ -272,8 +291,13 @@ struct Threads {
         __device__ __forceinline__ Source(const Threads &t, int c) : x(t, t.L.p.x, c), dy(t, t.L.p.dy, c) {}
         __device__ __forceinline__ void get(uint32_t slot, int i, uint64_t policy) const
         {
-            fetch<T, V>(slot, x(i), policy);
-            if (BACKWARD) fetch<T, V>(slot + kNext, dy(i), policy);
+            one(slot, x(i), policy, kXAligned);
+            if (BACKWARD) one(slot + kNext, dy(i), policy, kDyAligned);
+        }
+        __device__ __forceinline__ void one(uint32_t slot, const char *p, uint64_t policy, int bit) const
+        {
+            if (REGULAR || V == 1 || (x.t.L.aligned & bit)) fetch<T, V>(slot, p, policy);
+            else fetch_each<T, V>(slot, p, policy);
         }
     };
 
@@ -464,6 +488,17 @@ struct Threads {
     }
 
     // ---- pass 2, the texels read last first ----
+    __device__ __forceinline__ void put(char *at, const Vec<T, V> &v) const
+    {
+        T *p = reinterpret_cast<T *>(at);
+        if (REGULAR || V == 1 || (L.aligned & kOutAligned)) {
+            store_vec<T, V>(p, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) p[i] = v.v[i];
+        }
+    }
+
     template <int ACT>
     __device__ __forceinline__ void forward_apply(int c, int count, int near, int slot0, bool fresh) const
     {
@@ -483,7 +518,7 @@ struct Threads {
 #pragma unroll
             for (int j = 0; j < P; ++j)
                 f[j] = activate2<ACT>(__ffma2_rn(__fadd2_rn(f[j], shift[WHOLE ? 0 : j]), scale[j], beta[j]));
-            store_vec<T, V>(reinterpret_cast<T *>(out(i)), norm::pack<T, V>(f));
+            put(out(i), norm::pack<T, V>(f));
         });
     }
 
@@ -513,7 +548,7 @@ struct Threads {
                 terms<ACT>(fa[j], fb[j], shift[s], rstd[s], gamma[j], beta[j], h, e);
                 fa[j] = __fmul2_rn(rstd[s], __ffma2_rn(gamma[j], e, __ffma2_rn(h, k2[s], k1[s])));
             }
-            store_vec<T, V>(reinterpret_cast<T *>(out(i)), norm::pack<T, V>(fa));
+            put(out(i), norm::pack<T, V>(fa));
         });
     }
 
@@ -531,9 +566,10 @@ struct Threads {
     }
 };
 
-// WHOLE: a vector lies in one group.  FLAT: the texels of every map are evenly spaced.
-template <class T, int V, bool WHOLE, bool FLAT, bool BACKWARD, Phase PHASE>
-__global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads), WHOLE ? 2 : 1)
+// WHOLE: a vector lies in one group.  REGULAR: the texels of every map are evenly spaced and its
+// vectors aligned.
+template <class T, int V, bool WHOLE, bool REGULAR, bool BACKWARD, Phase PHASE>
+__global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads), WHOLE || V <= 4 ? 2 : 1)
     norm_kernel(const __grid_constant__ NormLaunch L)
 {
     constexpr int NT = BACKWARD ? kBackwardThreads : kForwardThreads, kWarps = NT / 32;
@@ -551,7 +587,7 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
     if (left == L.ty) ++turn, left = 0;
     const int mine = row < L.ty ? turn + (row < left) : 0;  // texels of this thread
     const int most = turn + (left > 0);                     // and of any
-    const Threads<T, V, WHOLE, FLAT, BACKWARD, PHASE> th = {L,    n,       lo, row, col, mine,
+    const Threads<T, V, WHOLE, REGULAR, BACKWARD, PHASE> th = {L,    n,       lo, row, col, mine,
                                                stat, scratch,
                                                (uint32_t)__cvta_generic_to_shared(smem + L.scratch) + tid * (uint32_t)sizeof(Vec<T, V>)};
     after_previous();
@@ -710,38 +746,38 @@ __global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads
 using NormKernel = void (*)(NormLaunch);
 
 template <class T, int V, bool BACKWARD, Phase PHASE>
-NormKernel pick_whole(bool whole, bool flat)
+NormKernel pick_whole(bool whole, bool regular)
 {
     if constexpr (V > 1)
-        if (!whole) return flat ? norm_kernel<T, V, false, true, BACKWARD, PHASE> : norm_kernel<T, V, false, false, BACKWARD, PHASE>;
-    return flat ? norm_kernel<T, V, true, true, BACKWARD, PHASE> : norm_kernel<T, V, true, false, BACKWARD, PHASE>;
+        if (!whole) return regular ? norm_kernel<T, V, false, true, BACKWARD, PHASE> : norm_kernel<T, V, false, false, BACKWARD, PHASE>;
+    return regular ? norm_kernel<T, V, true, true, BACKWARD, PHASE> : norm_kernel<T, V, true, false, BACKWARD, PHASE>;
 }
 
 template <class T, bool BACKWARD, Phase PHASE>
-NormKernel pick_width(int v, bool whole, bool flat)
+NormKernel pick_width(int v, bool whole, bool regular)
 {
     if constexpr (sizeof(T) == 2)
-        if (v == 8) return pick_whole<T, 8, BACKWARD, PHASE>(whole, flat);
-    return v == 4   ? pick_whole<T, 4, BACKWARD, PHASE>(whole, flat)
-           : v == 2 ? pick_whole<T, 2, BACKWARD, PHASE>(whole, flat)
-                    : pick_whole<T, 1, BACKWARD, PHASE>(whole, flat);
+        if (v == 8) return pick_whole<T, 8, BACKWARD, PHASE>(whole, regular);
+    return v == 4   ? pick_whole<T, 4, BACKWARD, PHASE>(whole, regular)
+           : v == 2 ? pick_whole<T, 2, BACKWARD, PHASE>(whole, regular)
+                    : pick_whole<T, 1, BACKWARD, PHASE>(whole, regular);
 }
 
 template <bool BACKWARD, Phase PHASE>
-NormKernel pick_kernel(int32_t dtype, int v, bool whole, bool flat)
+NormKernel pick_kernel(int32_t dtype, int v, bool whole, bool regular)
 {
-    return dtype == NT_DTYPE_F16    ? pick_width<__half, BACKWARD, PHASE>(v, whole, flat)
-           : dtype == NT_DTYPE_BF16 ? pick_width<__nv_bfloat16, BACKWARD, PHASE>(v, whole, flat)
-                                    : pick_width<float, BACKWARD, PHASE>(v, whole, flat);
+    return dtype == NT_DTYPE_F16    ? pick_width<__half, BACKWARD, PHASE>(v, whole, regular)
+           : dtype == NT_DTYPE_BF16 ? pick_width<__nv_bfloat16, BACKWARD, PHASE>(v, whole, regular)
+                                    : pick_width<float, BACKWARD, PHASE>(v, whole, regular);
 }
 
 // One per file that instantiates kernels: [forward, backward] x [both passes, sums, result].
-NormKernel forward_kernel(int32_t dtype, int v, bool whole, bool flat);
-NormKernel forward_sums_kernel(int32_t dtype, int v, bool whole, bool flat);
-NormKernel forward_apply_kernel(int32_t dtype, int v, bool whole, bool flat);
-NormKernel backward_kernel(int32_t dtype, int v, bool whole, bool flat);
-NormKernel backward_sums_kernel(int32_t dtype, int v, bool whole, bool flat);
-NormKernel backward_apply_kernel(int32_t dtype, int v, bool whole, bool flat);
+NormKernel forward_kernel(int32_t dtype, int v, bool whole, bool regular);
+NormKernel forward_sums_kernel(int32_t dtype, int v, bool whole, bool regular);
+NormKernel forward_apply_kernel(int32_t dtype, int v, bool whole, bool regular);
+NormKernel backward_kernel(int32_t dtype, int v, bool whole, bool regular);
+NormKernel backward_sums_kernel(int32_t dtype, int v, bool whole, bool regular);
+NormKernel backward_apply_kernel(int32_t dtype, int v, bool whole, bool regular);
 
 }  // namespace norm
 }  // namespace nt

@@ -3,6 +3,6 @@
 
 namespace nt {
 namespace norm {
-NormKernel backward_kernel(int32_t dtype, int v, bool whole, bool flat) { return pick_kernel<true, kBoth>(dtype, v, whole, flat); }
+NormKernel backward_kernel(int32_t dtype, int v, bool whole, bool regular) { return pick_kernel<true, kBoth>(dtype, v, whole, regular); }
 }  // namespace norm
 }  // namespace nt

@@ -3,6 +3,6 @@
 
 namespace nt {
 namespace norm {
-NormKernel backward_apply_kernel(int32_t dtype, int v, bool whole, bool flat) { return pick_kernel<true, kApply>(dtype, v, whole, flat); }
+NormKernel backward_apply_kernel(int32_t dtype, int v, bool whole, bool regular) { return pick_kernel<true, kApply>(dtype, v, whole, regular); }
 }  // namespace norm
 }  // namespace nt

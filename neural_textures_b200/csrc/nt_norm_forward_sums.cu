@@ -3,6 +3,6 @@
 
 namespace nt {
 namespace norm {
-NormKernel forward_sums_kernel(int32_t dtype, int v, bool whole, bool flat) { return pick_kernel<false, kSums>(dtype, v, whole, flat); }
+NormKernel forward_sums_kernel(int32_t dtype, int v, bool whole, bool regular) { return pick_kernel<false, kSums>(dtype, v, whole, regular); }
 }  // namespace norm
 }  // namespace nt
