@@ -256,45 +256,61 @@ struct DequantizeLaunch {
 
 constexpr int kDequantRows = 4;  // rows of one lane
 
-// A lane takes 8 codes (one word) of a row and writes 16 or 32 bytes.
-template <class T, int BLOCK>
+template <class T>
+__device__ __forceinline__ uint32_t pack_pair(float2 f)
+{
+    if constexpr (sizeof(T) == 4) {
+        return 0;
+    } else {
+        const auto h = f32_pair<T>(f);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+
+// A lane takes 8 codes (one word) of a row and writes 16 or 32 bytes.  WIDE: a warp to a row and 32 rows to a block, whose
+// codes, scales and results then lie at constant distances.
+template <class T, int BLOCK, bool WIDE>
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const DequantizeLaunch p)
 {
     after_previous();
-    const int lanes = 1 << p.lanes_log2;
+    const int lanes_log2 = WIDE ? 5 : p.lanes_log2, lanes = 1 << lanes_log2;
     const int sub = threadIdx.x & (lanes - 1);
-    const int rows_per_pass = kThreads >> p.lanes_log2;
-    const int64_t row0 =
-        (int64_t)(blockIdx.x / p.col_blocks) * rows_per_pass * kDequantRows + (threadIdx.x >> p.lanes_log2);
+    const int rows_per_pass = kThreads >> lanes_log2;
+    const int64_t row0 = (int64_t)(blockIdx.x / p.col_blocks) * rows_per_pass * kDequantRows + (threadIdx.x >> lanes_log2);
     const int64_t c = ((int64_t)(blockIdx.x % p.col_blocks) * lanes + sub) * 8;
-    __shared__ alignas(16) T turn[kThreads / 32][256];
+    __shared__ alignas(16) T turn[WIDE ? kThreads / 32 : 1][256];
     const bool in = c < p.cols;  // every lane of a warp stays for its exchange
+    const uint8_t *const data = p.data + row0 * p.pitch + (c >> 1);
+    const uint8_t *const scales = p.scales + (WIDE ? scale_at(row0, (int)(c / BLOCK), p.tiles) : 0);
     uint32_t codes[kDequantRows], bytes[kDequantRows];
 #pragma unroll
     for (int j = 0; j < kDequantRows; ++j) {
         const int64_t row = row0 + (int64_t)j * rows_per_pass;
-        if (row >= p.rows) break;
         codes[j] = bytes[j] = 0;
-        if (!in) continue;
-        codes[j] = __ldg(reinterpret_cast<const uint32_t *>(p.data + row * p.pitch + (c >> 1)));
-        bytes[j] = __ldg(p.scales + scale_at(row, (int)(c / BLOCK), p.tiles));
+        if (row >= p.rows || !in) continue;
+        codes[j] = __ldg(reinterpret_cast<const uint32_t *>(data + (int64_t)j * rows_per_pass * p.pitch));
+        // WIDE: 8 rows on, 16 bytes each, in the same quarter of the tile
+        bytes[j] = __ldg(WIDE ? scales + 128 * j : p.scales + scale_at(row, (int)(c / BLOCK), p.tiles));
     }
+    T *dst = static_cast<T *>(p.dst) + row0 * p.row_stride + c;
 #pragma unroll
-    for (int j = 0; j < kDequantRows; ++j) {
-        const int64_t row = row0 + (int64_t)j * rows_per_pass;
-        if (row >= p.rows) break;
+    for (int j = 0; j < kDequantRows; ++j, dst += rows_per_pass * p.row_stride) {
+        if (row0 + (int64_t)j * rows_per_pass >= p.rows) break;
         const float s = scale_value<BLOCK>(bytes[j]);
         uint32_t h2[4];
         values8(codes[j], h2);
         alignas(16) T out[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h2[i]));
-            out[2 * i] = from_f32<T>(f.x * s);
-            out[2 * i + 1] = from_f32<T>(f.y * s);
+            const float2 f = __fmul2_rn(__half22float2(*reinterpret_cast<const __half2 *>(&h2[i])), f2(s));
+            if constexpr (sizeof(T) == 2) {
+                reinterpret_cast<uint32_t *>(out)[i] = pack_pair<T>(f);
+            } else {
+                out[2 * i] = f.x;
+                out[2 * i + 1] = f.y;
+            }
         }
-        T *dst = static_cast<T *>(p.dst) + row * p.row_stride + c;
-        if (!p.vec && lanes == 32) {  // unaligned rows: a warp's 256 values through shared memory, 32 consecutive ones at a time
+        if (WIDE && !p.vec) {  // unaligned rows: a warp's 256 values through shared memory, 32 consecutive ones at a time
             T *const mine = turn[threadIdx.x >> 5];
             __syncwarp();
 #pragma unroll
@@ -306,7 +322,7 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const DequantizeLa
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (32 * i + sub < left) first[32 * i + sub] = mine[32 * i + sub];
-        } else if (sizeof(T) == 4 && lanes == 32 && c - 8 * sub + 256 <= p.cols) {  // the same for whole aligned rows, 512 bytes at a time
+        } else if (WIDE && sizeof(T) == 4 && c - 8 * sub + 256 <= p.cols) {  // the same for whole aligned rows, 512 bytes at a time
             T *const mine = turn[threadIdx.x >> 5];
             __syncwarp();
 #pragma unroll
@@ -339,7 +355,8 @@ cudaError_t launch_dequantize(DequantizeLaunch p, cudaStream_t st)
     const int64_t rows_per_block = (int64_t)(kThreads >> p.lanes_log2) * kDequantRows;
     const int64_t grid = ((int64_t)p.rows + rows_per_block - 1) / rows_per_block * p.col_blocks;
     if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    return launch_next(dequantize_kernel<T, BLOCK>, dim3((unsigned)grid), kThreads, 0, st, 1, p);
+    return launch_next(p.lanes_log2 == 5 ? dequantize_kernel<T, BLOCK, true> : dequantize_kernel<T, BLOCK, false>, dim3((unsigned)grid),
+                       kThreads, 0, st, 1, p);
 }
 
 // Shared checks of a matrix argument.

@@ -60,21 +60,6 @@ struct NormLaunch {
 };
 
 // V consecutive channels.
-template <class T>
-struct Pair;
-template <>
-struct Pair<__half> { using type = __half2; };
-template <>
-struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
-__device__ __forceinline__ float2 pair_f32(__half2 v) { return __half22float2(v); }
-__device__ __forceinline__ float2 pair_f32(__nv_bfloat162 v) { return __bfloat1622float2(v); }
-template <class T>
-__device__ __forceinline__ typename Pair<T>::type f32_pair(float2 v);
-template <>
-__device__ __forceinline__ __half2 f32_pair<__half>(float2 v) { return __float22half2_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat162 f32_pair<__nv_bfloat16>(float2 v) { return __float22bfloat162_rn(v); }
-
 template <class T, int V>
 struct alignas(V * sizeof(T) > 16 ? 16 : V * sizeof(T)) Vec {
     T v[V];
