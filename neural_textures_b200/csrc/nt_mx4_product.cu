@@ -283,36 +283,43 @@ __device__ __forceinline__ void epilogue_rows(const Output &p, const CUtensorMap
             __syncwarp();
         }
         uint8_t *const row = mine + lane * 128;
-        for (int s = 0; s < width && c0 + s < p.bn; s += 32) {
-            uint32_t v[32];
-            ld32(tmem + c0 + s, v);
-            umma::wait_ld();
+        // both halves of 64 columns are on their way before the first is waited for
+        const bool two = size == 2 && c0 + 32 < p.bn;
+        uint32_t v[2][32];
+        ld32(tmem + c0, v[0]);
+        if (two) ld32(tmem + c0 + 32, v[1]);
+        umma::wait_ld();
+        if (p.tma_store && elect_one()) store_wait_read();  // the last store has read the staging
+        __syncwarp();
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            if (s && !two) break;
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
-                const float4 b = *reinterpret_cast<const float4 *>(bias + s + i);
-                float2 y = activate2<ACT>(__ffma2_rn(f2(p.alpha), make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), make_float2(b.x, b.y)));
-                v[i] = __float_as_uint(y.x);
-                v[i + 1] = __float_as_uint(y.y);
-                y = activate2<ACT>(__ffma2_rn(f2(p.alpha), make_float2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), make_float2(b.z, b.w)));
-                v[i + 2] = __float_as_uint(y.x);
-                v[i + 3] = __float_as_uint(y.y);
-            }
-            if (s == 0) {  // the last store has read this buffer
-                if (p.tma_store && elect_one()) store_wait_read();
-                __syncwarp();
+                const float4 b = *reinterpret_cast<const float4 *>(bias + 32 * s + i);
+                uint32_t(&w)[32] = v[s];
+                const float2 y0 = activate2<ACT>(
+                    __ffma2_rn(f2(p.alpha), make_float2(__uint_as_float(w[i]), __uint_as_float(w[i + 1])), make_float2(b.x, b.y)));
+                const float2 y1 = activate2<ACT>(
+                    __ffma2_rn(f2(p.alpha), make_float2(__uint_as_float(w[i + 2]), __uint_as_float(w[i + 3])), make_float2(b.z, b.w)));
+                w[i] = __float_as_uint(y0.x);
+                w[i + 1] = __float_as_uint(y0.y);
+                w[i + 2] = __float_as_uint(y1.x);
+                w[i + 3] = __float_as_uint(y1.y);
             }
             if (size == 4) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    *reinterpret_cast<uint4 *>(row + ((i ^ (lane & 7)) << 4)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                    *reinterpret_cast<uint4 *>(row + ((i ^ (lane & 7)) << 4)) =
+                        make_uint4(v[s][4 * i], v[s][4 * i + 1], v[s][4 * i + 2], v[s][4 * i + 3]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     uint32_t h[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        h[e] = pack2(p.dtype, __uint_as_float(v[8 * i + 2 * e]), __uint_as_float(v[8 * i + 2 * e + 1]));
-                    *reinterpret_cast<uint4 *>(row + (((s >> 3) + i ^ (lane & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+                        h[e] = pack2(p.dtype, __uint_as_float(v[s][8 * i + 2 * e]), __uint_as_float(v[s][8 * i + 2 * e + 1]));
+                    *reinterpret_cast<uint4 *>(row + ((4 * s + i ^ (lane & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
                 }
             }
         }

@@ -1,6 +1,9 @@
 // nt_norm.cu -- channels-last group normalisation with an activation: argument checks and launch
 // plan of nt_group_norm_forward and nt_group_norm_backward (the kernel is in nt_norm.cuh).
 #include <algorithm>
+#include <mutex>
+#include <set>
+#include <utility>
 
 #include "nt_norm.cuh"
 
@@ -81,6 +84,20 @@ bool flat(const NtFeatureMap &f, const NtGroupNorm *p, int size)
     return (p->height == 1 || f.row_stride == p->width * f.texel_stride) && f.texel_stride < ((int64_t)1 << 31) / (512 * size);
 }
 
+// Once per kernel and device.
+cudaError_t allow_large_clusters(const void *kernel)
+{
+    static std::mutex mu;
+    static std::set<std::pair<const void *, int>> done;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::lock_guard<std::mutex> lock(mu);
+    if (done.count({kernel, dev})) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) done.insert({kernel, dev});
+    return e;
+}
+
 cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
 {
     const int size = layer_dtype_size(p->dtype);
@@ -138,8 +155,7 @@ cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
         L.turns = L.share / L.ty;
         L.left = L.share % L.ty;
         cudaError_t e = set_smem_limit(reinterpret_cast<const void *>(kernel), 227 * 1024 - 1024);
-        if (e == cudaSuccess && cluster > 8)
-            e = cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e == cudaSuccess && cluster > 8) e = allow_large_clusters(reinterpret_cast<const void *>(kernel));
         return e == cudaSuccess ? launch_next(kernel, dim3((unsigned)splits, (unsigned)p->images), threads, smem, st, (unsigned)cluster, L) : e;
     };
     cudaError_t e;
