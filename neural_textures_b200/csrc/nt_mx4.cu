@@ -1,8 +1,8 @@
 // nt_mx4.cu -- 4-bit microscaled matrices: quantisation from fp16 / bf16 / fp32 and back
 // (nt_mx4_quantize, nt_mx4_dequantize).
 //
-// Bound by HBM where a matrix is large and its rows lie along the memory: 16384 x 8192 bf16 in blocks of 16 takes 60 us each way
-// (5.7 TB/s), 8192 x 8192 fp32 52 and 48 us.  Transposed (8192 x 8192 fp32 85 us) and unaligned rows (16384 x 8191
+// Bound by HBM where a matrix is large and its rows lie along the memory: 16384 x 8192 bf16 in blocks of 16 takes 60 us
+// (5.7 TB/s) and 54 us back (6.4 TB/s), 8192 x 8192 fp32 52 and 48 us.  Transposed (8192 x 8192 fp32 85 us) and unaligned rows (16384 x 8191
 // bf16 118 us) are bound by their narrower loads.
 #include "nt_mx4.cuh"
 
