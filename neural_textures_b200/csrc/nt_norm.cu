@@ -27,7 +27,7 @@ struct Plan {
     bool cluster;  // one launch
     int splits;    // blocks of an image, in the launch that makes the sums
     int applies;   // and in the one that makes the result
-    int per_sm;    // blocks that share an SM's shared memory
+    int per_sm;    // blocks that share an SM's shared memory: one where the sums of a texel need the room
 };
 
 // A cluster costs about 1 us over a single block; two launches let every SM compute, but take the host 3 us more.  A
@@ -38,13 +38,19 @@ struct Plan {
 constexpr int kForwardTurns = 8, kBackwardTurns = 4;
 constexpr int kApplyTurns = 16;  // of a block of the second launch: enough of them that fast SMs take more
 
-Plan plan(const NtGroupNorm *p, bool backward)
+// Channels of a vector: up to 16 bytes of them, and up to 4 where vectors cross groups, whose per-channel values take
+// the registers of a second block on the SM otherwise (3x83x138x48 fp16 of 8 groups: 14.2 us in vectors of 8, 9.2 in 4).
+int vector_width(const NtGroupNorm *p)
 {
-    const int sms = sm_count(), threads = backward ? kBackwardThreads : kForwardThreads;
     int v = 16 / layer_dtype_size(p->dtype);
     while (p->channels % v) v /= 2;
-    const bool light = p->channels / p->groups % v == 0 || v <= 4;  // kernels that two blocks of fit an SM's registers
-    const int per_sm = light && p->channels <= 2048 ? 2 : 1;
+    return v == 8 && p->channels / p->groups % 8 ? 4 : v;
+}
+
+Plan plan(const NtGroupNorm *p, bool backward)
+{
+    const int sms = sm_count(), threads = backward ? kBackwardThreads : kForwardThreads, v = vector_width(p);
+    const int per_sm = p->channels <= 2048 ? 2 : 1;
     const int64_t texels = (int64_t)p->height * p->width, turns = ceil_div(texels * (p->channels / v), threads);
     const int64_t most = std::min<int64_t>(texels, kMaxSplits);
     const int largest = (int64_t)p->images * kMaxCluster <= sms * 7 / 8 ? kMaxCluster : 8;  // of 16: one in most of the GPCs
@@ -118,8 +124,13 @@ cudaError_t launch(const NtGroupNorm *p, bool backward, cudaStream_t st)
     L.channels_part = reinterpret_cast<float2 *>(ws + at.channels_at);
     const size_t most = 227 * 1024 / pl.per_sm - 1024;
     size_t smem = 0;
-    int v = 16 / size;
-    while (p->channels % v) v /= 2;
+    // vectors that are not aligned are put together from their elements, unless half of one is aligned
+    int v = vector_width(p);
+    auto all_aligned = [&](int w) {
+        return vectors_aligned(p->x, w, size) && vectors_aligned(backward ? p->dy : p->y, w, size) &&
+               vectors_aligned(backward ? p->dx : p->y, w, size);
+    };
+    if (v * size == 16 && !all_aligned(v) && all_aligned(v / 2)) v /= 2;
     bool whole = true;
     for (;; v /= 2) {  // narrower vectors where the sums of very many groups leave no room for the ring
         whole = L.per % v == 0;

@@ -557,7 +557,7 @@ struct Threads {
 // WHOLE: a vector lies in one group.  REGULAR: the texels of every map are evenly spaced and its
 // vectors aligned.
 template <class T, int V, bool WHOLE, bool REGULAR, bool BACKWARD, Phase PHASE>
-__global__ void __launch_bounds__((BACKWARD ? kBackwardThreads : kForwardThreads), WHOLE || V <= 4 ? 2 : 1)
+__global__ void __launch_bounds__(BACKWARD ? kBackwardThreads : kForwardThreads, 2)
     norm_kernel(const __grid_constant__ NormLaunch L)
 {
     constexpr int NT = BACKWARD ? kBackwardThreads : kForwardThreads, kWarps = NT / 32;
@@ -736,7 +736,7 @@ using NormKernel = void (*)(NormLaunch);
 template <class T, int V, bool BACKWARD, Phase PHASE>
 NormKernel pick_whole(bool whole, bool regular)
 {
-    if constexpr (V > 1)
+    if constexpr (V > 1 && V < 8)
         if (!whole) return regular ? norm_kernel<T, V, false, true, BACKWARD, PHASE> : norm_kernel<T, V, false, false, BACKWARD, PHASE>;
     return regular ? norm_kernel<T, V, true, true, BACKWARD, PHASE> : norm_kernel<T, V, true, false, BACKWARD, PHASE>;
 }
