@@ -1,6 +1,6 @@
 // nt_norm.cuh -- the group-norm kernel, forward and backward (nt_group_norm_forward,
-// nt_group_norm_backward); nt_norm_forward.cu and nt_norm_backward.cu instantiate it, nt_norm.cu
-// checks arguments and plans the launch.
+// nt_group_norm_backward); nt_norm_{forward,backward}{,_sums,_apply}.cu instantiate it, nt_norm.cu
+// checks arguments and plans the launches.
 //
 // Two passes over a map:
 //   1. sums.  `splits` thread blocks share an image; a thread keeps one vector of V channels and
@@ -16,7 +16,7 @@
 // different GPCs differ by half in bandwidth, and all waited for the slowest twice: 73 us against 68 us for
 // 1024 x 1024 x 64 fp16, 17.6 against 9.8 us for 256 x 256 x 64.)
 // A thread's vectors arrive by asynchronous copies in its own slots of shared memory, so that loads stay in
-// flight while it computes and no barrier is needed: a ring of a few vectors, and behind it what is kept.
+// flight while it computes and no barrier is needed: a ring of a few vectors, and in front of it what is kept.
 // All sums are joined in a fixed order.
 //
 // Bound by HBM (2 to 3 readings of a map in all) and, in the second pass, by issue slots and the special-function unit.
