@@ -40,16 +40,19 @@ class LatentEncoder:
     @_on_device
     def train_step(self, features) -> None:
         """One step: latents from the features, the texture's training pass, gradients back through the layers,
-        Adam on them and on the texture's network.  The loss is added to tex.loss_accum."""
+        Adam on them and on the texture's network.  The loss is added to tex.loss_accum.  Everything is queued on
+        torch's current stream."""
+        import torch
         tex = self.tex
+        stream = torch.cuda.current_stream(self.device).cuda_stream
         self.encode(features, keep=True)
         p = tex.params()
-        InvokeTraining(p)
+        InvokeTraining(p, stream=stream)
         d = tex.ggrads[self.grid]
         for layer in reversed(self.layers):
             d = layer.backward(d)
         self._optimize()
-        InvokeOptimizeNetwork(p)
+        InvokeOptimizeNetwork(p, stream=stream)
         for g in tex.ggrads:
             g.zero_()
         tex.step += 1
