@@ -4,8 +4,9 @@ them as one layer of a network over a feature map.
 
 Every call queues its kernels on `stream` (a torch.cuda.Stream or a raw handle; None: torch's
 current stream of the tensors' device) and returns without waiting.  Results are new tensors unless
-`out` is given.  Invalid arguments raise: TypeError / ValueError for what only the tensors show
-(device, dtype, shape), NtError for what the library rejects.
+`out` is given, from the memory pool of that stream; a caller that passes `stream` orders it behind what made the
+inputs, and keeps them until it is done.  Invalid arguments raise: TypeError / ValueError for what only the tensors
+show (device, dtype, shape), NtError for what the library rejects.
 """
 from __future__ import annotations
 
@@ -82,27 +83,42 @@ def _new(shape, dtype, device):
     return _torch.empty_like(t)
 
 
-def _launch(device, stream, made, fn, *args):
-    """fn(*args, stream) on `device`.  `made` are tensors of this call: they live in torch's pool of
-    the current stream, so when another stream uses them they are recorded on it."""
+def _launch(device, fn, *args):
+    """fn(*args, torch's current stream) on `device`."""
     torch = _torch
     if device.type != "cuda":
         raise ValueError(f"a CUDA tensor is needed, not one on {device}")
     index = device.index
-    current = torch._C._cuda_getCurrentRawStream(index)
-    handle = current if stream is None else stream if isinstance(stream, int) else int(stream.cuda_stream)
+    handle = torch._C._cuda_getCurrentRawStream(index)
     if torch._C._cuda_getDevice() == index:
         status = fn(*args, handle)
     else:
         with torch.cuda.device(index):
             status = fn(*args, handle)
-    if handle != current:
-        other = torch.cuda.ExternalStream(handle, device=device)
-        for t in made:
-            if t is not None:
-                t.record_stream(other)
     if status:
         check(status)
+
+
+def _on(stream, device, fn, *args, out=None):
+    """fn(*args, out=out) with `stream` as torch's current one.  Results and workspace come from its pool then:
+    memory of the caller's current stream may have been freed with work pending there, which nothing orders before
+    `stream`.  New results are recorded on the caller's stream, so that it may use them too."""
+    torch = _torch
+    if device.type != "cuda":
+        raise ValueError(f"a CUDA tensor is needed, not one on {device}")
+    if getattr(stream, "device", device) != device:
+        raise ValueError(f"the stream is on {stream.device}, not on {device}")
+    current = torch.cuda.current_stream(device)
+    if not isinstance(stream, torch.cuda.Stream):
+        handle = stream if isinstance(stream, int) else int(stream.cuda_stream)
+        stream = current if handle == current.cuda_stream else torch.cuda.ExternalStream(handle, device=device)
+    with torch.cuda.stream(stream):
+        result = fn(*args, out=out)
+    if stream != current:
+        parts = (result.data, result.scales) if isinstance(result, Mx4Tensor) else result if isinstance(result, tuple) else (result,)
+        for t in parts if out is None else parts[1:] if isinstance(result, tuple) else ():
+            t.record_stream(current)
+    return result
 
 
 # ---------------------------------------------------------------------------------------
@@ -161,7 +177,9 @@ def group_norm(x, groups: int, gamma=None, beta=None, activation: str = "none", 
     (y, mean, rstd) with float32 statistics [N][groups], which group_norm_backward takes.  `out`
     receives y and may be x."""
     torch = _torch or _lazy_torch()
-    if out is None and stream is None:
+    if stream is not None:
+        return _on(stream, x.device, group_norm, x, groups, gamma, beta, activation, eps, out=out)
+    if out is None:
         made = _fast.group_norm(x, groups, gamma, beta, ACTIVATIONS.get(activation), eps)
         if made is not None:
             return made
@@ -178,7 +196,7 @@ def group_norm(x, groups: int, gamma=None, beta=None, activation: str = "none", 
         yp, y0, y1, y2 = _strides(y, "y")
     mean, rstd = _new((n, max(g, 0)), torch.float32, device), _new((n, max(g, 0)), torch.float32, device)
     ws, wp, size = _norm_workspace(L, sizes, dtype, device, 0)
-    _launch(device, stream, (None if out is not None else y, mean, rstd, ws), L.nt_group_norm_forward,
+    _launch(device, L.nt_group_norm_forward,
             _GROUP_NORM.pack(n, h, w, c, g, dtype, act, eps, xp, x0, x1, x2, ga, be, mean.data_ptr(), rstd.data_ptr(),
                              yp, y0, y1, y2, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, wp, size))
     return y, mean, rstd
@@ -189,7 +207,9 @@ def group_norm_backward(dy, x, mean, rstd, groups: int, gamma=None, beta=None, a
     dbeta).  dx has x's type; dgamma and dbeta are float32 [C], summed over images and texels.
     `out` receives dx and may be dy or x."""
     torch = _torch or _lazy_torch()
-    if out is None and stream is None:
+    if stream is not None:
+        return _on(stream, x.device, group_norm_backward, dy, x, mean, rstd, groups, gamma, beta, activation, out=out)
+    if out is None:
         made = _fast.group_norm_backward(dy, x, mean, rstd, groups, gamma, beta, ACTIVATIONS.get(activation))
         if made is not None:
             return made
@@ -208,7 +228,7 @@ def group_norm_backward(dy, x, mean, rstd, groups: int, gamma=None, beta=None, a
         dp, d0, d1, d2 = _strides(dx, "dx")
     dgamma, dbeta = _new((c,), torch.float32, device), _new((c,), torch.float32, device)
     ws, wp, size = _norm_workspace(L, sizes, dtype, device, 1)
-    _launch(device, stream, (None if out is not None else dx, dgamma, dbeta, ws), L.nt_group_norm_backward,
+    _launch(device, L.nt_group_norm_backward,
             _GROUP_NORM.pack(n, h, w, c, g, dtype, act, 1.0, xp, x0, x1, x2, ga, be, mp, rp, 0, 0, 0, 0, gp, g0, g1, g2,
                              dp, d0, d1, d2, dgamma.data_ptr(), dbeta.data_ptr(), wp, size))
     return dx, dgamma, dbeta
@@ -272,7 +292,9 @@ def mx4_quantize(x, block: int = 32, out: Mx4Tensor | None = None, stream=None) 
     """The float16, bfloat16 or float32 matrix x (2-D, any strides: x.t() is read in place) in 4-bit
     microscaled form, blocks along its columns (nt_mx4_quantize)."""
     _torch or _lazy_torch()
-    if out is None and stream is None:
+    if stream is not None:
+        return _on(stream, x.device, mx4_quantize, x, block, out=out)
+    if out is None:
         made = _fast.mx4_quantize(x, block)
         if made is not None:
             out = Mx4Tensor.__new__(Mx4Tensor)
@@ -282,14 +304,12 @@ def mx4_quantize(x, block: int = 32, out: Mx4Tensor | None = None, stream=None) 
     dtype = _dtype(x, "x")
     if x.dim() != 2:
         raise ValueError(f"x must be a matrix, not {tuple(x.shape)}")
-    made = out is None
-    if made:
+    if out is None:
         out = Mx4Tensor.empty(x.shape[0], x.shape[1], block, x.device)
     elif out.shape != tuple(x.shape) or out.block != block or out.device != x.device:
         raise ValueError(f"out must be {tuple(x.shape)} in blocks of {block} on {x.device}")
     rs, cs = x.stride()
-    _launch(x.device, stream, (out.data, out.scales) if made else (), load().nt_mx4_quantize, x.data_ptr(), dtype, rs, cs,
-            out._packed)
+    _launch(x.device, load().nt_mx4_quantize, x.data_ptr(), dtype, rs, cs, out._packed)
     return out
 
 
@@ -307,12 +327,14 @@ def mx4_dequantize(q: Mx4Tensor, dtype=None, out=None, stream=None):
     torch = _torch or _lazy_torch()
     dtype = dtype or (out.dtype if out is not None else torch.float16)
     code = _dtype(dtype, "dtype")
-    if out is None and stream is None:
+    if stream is not None:
+        return _on(stream, q.device, mx4_dequantize, q, dtype, out=out)
+    if out is None:
         y = _fast.mx4_dequantize(q._packed, q.data, code)
         if y is not None:
             return y
     y, stride = _output(out, q.rows, q.cols, dtype, q.device)
-    _launch(q.device, stream, (y if out is None else None,), load().nt_mx4_dequantize, q._packed, y.data_ptr(), code, stride)
+    _launch(q.device, load().nt_mx4_dequantize, q._packed, y.data_ptr(), code, stride)
     return y
 
 
@@ -323,7 +345,9 @@ def mx4_product(a: Mx4Tensor, b: Mx4Tensor, bias=None, activation: str = "none",
     torch = _torch or _lazy_torch()
     dtype = dtype or (out.dtype if out is not None else torch.float16)
     code, act = _dtype(dtype, "dtype"), _activation(activation)
-    if out is None and stream is None:
+    if stream is not None:
+        return _on(stream, a.device, mx4_product, a, b, bias, activation, alpha, dtype, out=out)
+    if out is None:
         y = _fast.mx4_product(a._packed, a.data, b._packed, b.data, bias, act, alpha, code)
         if y is not None:
             return y
@@ -331,7 +355,7 @@ def mx4_product(a: Mx4Tensor, b: Mx4Tensor, bias=None, activation: str = "none",
     if b.data.device != device:
         raise ValueError(f"b is on {b.device}, not on {device}")
     y, stride = _output(out, a.rows, b.rows, dtype, device)
-    _launch(device, stream, (y if out is None else None,), load().nt_mx4_product, a._packed, b._packed,
+    _launch(device, load().nt_mx4_product, a._packed, b._packed,
             _vector(bias, b.rows, device, "bias"), act, alpha, y.data_ptr(), code, stride)
     return y
 
