@@ -181,12 +181,13 @@ PyObject *group_norm_backward(PyObject *, PyObject *const *a, Py_ssize_t n)
     END_HANDLE_TH_ERRORS
 }
 
-// A NtMx4Matrix packed as bytes (Mx4Tensor._packed) whose memory is on `device`.
-bool matrix_arg(PyObject *packed, PyObject *data, c10::DeviceIndex device, NtMx4Matrix &m)
+// A NtMx4Matrix packed as bytes (Mx4Tensor._packed), while it names the memory of its tensors, on `device`.
+bool matrix_arg(PyObject *packed, PyObject *data, PyObject *scales, c10::DeviceIndex device, NtMx4Matrix &m)
 {
-    if (!PyBytes_Check(packed) || PyBytes_GET_SIZE(packed) != (Py_ssize_t)sizeof m || !cuda_tensor(data, device)) return false;
+    const at::Tensor *d = cuda_tensor(data, device), *s = cuda_tensor(scales, device);
+    if (!d || !s || !PyBytes_Check(packed) || PyBytes_GET_SIZE(packed) != (Py_ssize_t)sizeof m) return false;
     std::memcpy(&m, PyBytes_AS_STRING(packed), sizeof m);
-    return true;
+    return m.data == d->data_ptr() && m.scales == s->data_ptr();
 }
 
 // (codes, scales, rows, cols, block) -> packed NtMx4Matrix
@@ -248,16 +249,16 @@ PyObject *mx4_quantize(PyObject *, PyObject *const *a, Py_ssize_t n)
 
 at::ScalarType scalar_type(int32_t dtype) { return dtype == NT_DTYPE_F32 ? at::kFloat : dtype == NT_DTYPE_F16 ? at::kHalf : at::kBFloat16; }
 
-// (packed, codes, dtype) -> values
+// (packed, codes, scales, dtype) -> values
 PyObject *mx4_dequantize(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
-    if (n != 3) Py_RETURN_NONE;
+    if (n != 4) Py_RETURN_NONE;
     const c10::DeviceIndex device = current_device_of(a[1]);
     if (device < 0) Py_RETURN_NONE;
     NtMx4Matrix m;
     int32_t dtype;
-    if (!matrix_arg(a[0], a[1], device, m) || !int_arg(a[2], 0, NT_DTYPE_BF16, dtype)) Py_RETURN_NONE;
+    if (!matrix_arg(a[0], a[1], a[2], device, m) || !int_arg(a[3], 0, NT_DTYPE_BF16, dtype)) Py_RETURN_NONE;
     at::Tensor y = make({m.rows, m.cols}, scalar_type(dtype), device);
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device);
     if (without_gil([&] { return nt_mx4_dequantize(&m, y.data_ptr(), dtype, m.cols, stream); }) != NT_OK) Py_RETURN_NONE;
@@ -265,21 +266,22 @@ PyObject *mx4_dequantize(PyObject *, PyObject *const *a, Py_ssize_t n)
     END_HANDLE_TH_ERRORS
 }
 
-// (a packed, a codes, b packed, b codes, bias, activation, alpha, dtype) -> d
+// (a packed, a codes, a scales, b packed, b codes, b scales, bias, activation, alpha, dtype) -> d
 PyObject *mx4_product(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
-    if (n != 8) Py_RETURN_NONE;
+    if (n != 10) Py_RETURN_NONE;
     const c10::DeviceIndex device = current_device_of(a[1]);
     if (device < 0) Py_RETURN_NONE;
     NtMx4Matrix l, r;
     int32_t act, dtype;
     float *bias;
-    if (!matrix_arg(a[0], a[1], device, l) || !matrix_arg(a[2], a[3], device, r) || !vector_arg(a[4], r.rows, device, bias) ||
-        !int_arg(a[5], 0, 3, act) || !PyFloat_Check(a[6]) || !int_arg(a[7], 0, NT_DTYPE_BF16, dtype))
+    if (!matrix_arg(a[0], a[1], a[2], device, l) || !matrix_arg(a[3], a[4], a[5], device, r) ||
+        !vector_arg(a[6], r.rows, device, bias) || !int_arg(a[7], 0, 3, act) || !PyFloat_Check(a[8]) ||
+        !int_arg(a[9], 0, NT_DTYPE_BF16, dtype))
         Py_RETURN_NONE;
     at::Tensor d = make({l.rows, r.rows}, scalar_type(dtype), device);
-    const float alpha = (float)PyFloat_AS_DOUBLE(a[6]);
+    const float alpha = (float)PyFloat_AS_DOUBLE(a[8]);
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device);
     if (without_gil([&] { return nt_mx4_product(&l, &r, bias, act, alpha, d.data_ptr(), dtype, r.rows, stream); }) != NT_OK) Py_RETURN_NONE;
     return THPVariable_Wrap(d);

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import importlib.util
+import operator
 import os
 import struct
 
@@ -237,31 +238,42 @@ def group_norm_backward(dy, x, mean, rstd, groups: int, gamma=None, beta=None, a
 # ---------------------------------------------------------------------------------------
 # 4-bit microscaled matrices
 
+def _matrix(q):
+    """The NtMx4Matrix of q's tensors as they are now, packed as bytes."""
+    torch = _torch or _lazy_torch()
+    data, scales, rows, cols, block = q._data, q._scales, q._rows, q._cols, q._block
+    q._packed = _fast.mx4_pack(data, scales, rows, cols, block)
+    if q._packed is not None:
+        return q._packed
+    # not a matrix: say why
+    if block not in (16, 32):
+        raise ValueError(f"block must be 16 or 32, not {block}")
+    if not 0 <= rows <= 0x7fffff00 or not 1 <= cols <= 0x7fffff00:
+        raise ValueError(f"{rows} x {cols} is not a matrix size")
+    pitch, size = -(-cols // 32) * 16, -(-rows // 128) * -(-cols // (4 * block)) * 512
+    if data.dtype is not torch.uint8 or data.dim() != 2 or data.shape[0] < rows or data.shape[1] < pitch or rows and data.stride(1) != 1:
+        raise ValueError(f"data must be uint8 [{rows}][{pitch}] or larger, the codes of a row contiguous")
+    if scales.dtype is not torch.uint8 or not scales.is_contiguous() or scales.numel() < size:
+        raise ValueError(f"scales must be contiguous uint8 of {size} bytes")
+    if scales.device != data.device:
+        raise ValueError(f"scales is on {scales.device}, not on {data.device}")
+    raise TypeError("data and scales must be torch tensors, rows, cols and block integers")
+
+
 class Mx4Tensor:
     """A rows x cols matrix in 4-bit microscaled form (NtMx4Matrix): `data`, the uint8 codes
     [rows][pitch], two to a byte, and `scales`, a byte per block of `block` columns (32: powers of
-    two, 16: E4M3) in tiles of 128 rows x 4 blocks.  Padding must be zero, as mx4_quantize leaves it."""
-    __slots__ = ("data", "scales", "rows", "cols", "block", "_packed")
+    two, 16: E4M3) in tiles of 128 rows x 4 blocks.  Padding must be zero, as mx4_quantize leaves it.  The fields
+    are read-only; copies, pickles and torch.save carry the tensors."""
+    __slots__ = ("_data", "_scales", "_rows", "_cols", "_block", "_packed")  # _packed: the NtMx4Matrix of a call
+    data, scales, rows, cols, block = (property(operator.attrgetter(f)) for f in __slots__[:5])
 
     def __init__(self, data, scales, rows: int, cols: int, block: int = 32):
-        torch = _torch or _lazy_torch()
-        self.data, self.scales, self.rows, self.cols, self.block = data, scales, rows, cols, block
-        self._packed = _fast.mx4_pack(data, scales, rows, cols, block)
-        if self._packed is not None:
-            return
-        # not a matrix: say why
-        if block not in (16, 32):
-            raise ValueError(f"block must be 16 or 32, not {block}")
-        if not 0 <= rows <= 0x7fffff00 or not 1 <= cols <= 0x7fffff00:
-            raise ValueError(f"{rows} x {cols} is not a matrix size")
-        pitch, size = -(-cols // 32) * 16, -(-rows // 128) * -(-cols // (4 * block)) * 512
-        if data.dtype is not torch.uint8 or data.dim() != 2 or data.shape[0] < rows or data.shape[1] < pitch or rows and data.stride(1) != 1:
-            raise ValueError(f"data must be uint8 [{rows}][{pitch}] or larger, the codes of a row contiguous")
-        if scales.dtype is not torch.uint8 or not scales.is_contiguous() or scales.numel() < size:
-            raise ValueError(f"scales must be contiguous uint8 of {size} bytes")
-        if scales.device != data.device:
-            raise ValueError(f"scales is on {scales.device}, not on {data.device}")
-        raise TypeError("data and scales must be torch tensors, rows, cols and block integers")
+        self._data, self._scales, self._rows, self._cols, self._block = data, scales, rows, cols, block
+        _matrix(self)
+
+    def __reduce__(self):  # copies and loaded matrices name the memory of their own tensors
+        return Mx4Tensor, (self._data, self._scales, self._rows, self._cols, self._block)
 
     @classmethod
     def empty(cls, rows: int, cols: int, block: int = 32, device="cuda"):
@@ -298,8 +310,8 @@ def mx4_quantize(x, block: int = 32, out: Mx4Tensor | None = None, stream=None) 
         made = _fast.mx4_quantize(x, block)
         if made is not None:
             out = Mx4Tensor.__new__(Mx4Tensor)
-            (out.rows, out.cols), out.block = x.shape, block
-            out.data, out.scales, out._packed = made
+            (out._rows, out._cols), out._block = x.shape, block
+            out._data, out._scales, out._packed = made
             return out
     dtype = _dtype(x, "x")
     if x.dim() != 2:
@@ -309,7 +321,7 @@ def mx4_quantize(x, block: int = 32, out: Mx4Tensor | None = None, stream=None) 
     elif out.shape != tuple(x.shape) or out.block != block or out.device != x.device:
         raise ValueError(f"out must be {tuple(x.shape)} in blocks of {block} on {x.device}")
     rs, cs = x.stride()
-    _launch(x.device, load().nt_mx4_quantize, x.data_ptr(), dtype, rs, cs, out._packed)
+    _launch(x.device, load().nt_mx4_quantize, x.data_ptr(), dtype, rs, cs, _matrix(out))
     return out
 
 
@@ -330,11 +342,11 @@ def mx4_dequantize(q: Mx4Tensor, dtype=None, out=None, stream=None):
     if stream is not None:
         return _on(stream, q.device, mx4_dequantize, q, dtype, out=out)
     if out is None:
-        y = _fast.mx4_dequantize(q._packed, q.data, code)
+        y = _fast.mx4_dequantize(q._packed, q._data, q._scales, code)
         if y is not None:
             return y
     y, stride = _output(out, q.rows, q.cols, dtype, q.device)
-    _launch(q.device, load().nt_mx4_dequantize, q._packed, y.data_ptr(), code, stride)
+    _launch(q.device, load().nt_mx4_dequantize, _matrix(q), y.data_ptr(), code, stride)
     return y
 
 
@@ -348,14 +360,14 @@ def mx4_product(a: Mx4Tensor, b: Mx4Tensor, bias=None, activation: str = "none",
     if stream is not None:
         return _on(stream, a.device, mx4_product, a, b, bias, activation, alpha, dtype, out=out)
     if out is None:
-        y = _fast.mx4_product(a._packed, a.data, b._packed, b.data, bias, act, alpha, code)
+        y = _fast.mx4_product(a._packed, a._data, a._scales, b._packed, b._data, b._scales, bias, act, alpha, code)
         if y is not None:
             return y
     device = a.device
     if b.data.device != device:
         raise ValueError(f"b is on {b.device}, not on {device}")
     y, stride = _output(out, a.rows, b.rows, dtype, device)
-    _launch(device, load().nt_mx4_product, a._packed, b._packed,
+    _launch(device, load().nt_mx4_product, _matrix(a), _matrix(b),
             _vector(bias, b.rows, device, "bias"), act, alpha, y.data_ptr(), code, stride)
     return y
 
