@@ -12,6 +12,10 @@ constexpr int kTileBytes = 512;  // 128 rows x 4 blocks
 __host__ __device__ constexpr int tiles_per_row(int cols, int block) { return (int)(((int64_t)cols + 4 * block - 1) / (4 * block)); }
 __host__ __device__ constexpr int64_t row_pitch(int cols) { return ((int64_t)cols + 31) / 32 * 16; }
 
+// Byte of scale tile `tile` of a row of tiles: a row of 2^31 columns has 16 GB of them.
+__host__ __device__ constexpr int64_t tile_offset(int tile) { return (int64_t)tile * kTileBytes; }
+static_assert(tile_offset(1 << 22) == (int64_t)1 << 31, "no 32-bit product");
+
 // Byte of the scale of row r, block k.
 __device__ __forceinline__ int64_t scale_at(int64_t r, int k, int tiles)
 {

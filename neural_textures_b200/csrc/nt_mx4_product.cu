@@ -502,7 +502,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int ks = k_lo; ks < k_hi; ++ks) {
                 if (!(ok = __all_sync(0xffffffffu, wait(empty + 8 * s, phase ^ 1)))) break;
                 const uint32_t at = base + s * stage_bytes, bar = full + 8 * s;
-                const int st = min(kTiles, scale_tiles - ks * kTiles), from = ks * kTiles * kTileBytes;
+                const int st = min(kTiles, scale_tiles - ks * kTiles);
+                const int64_t from = tile_offset(ks * kTiles);
                 const uint32_t ct = resident ? base : at;
                 if (elect_one()) {
                     expect_tx(bar, ls_off + st * kTileBytes + (columns ? bn * row_bytes + cs * st * kTileBytes : 0));

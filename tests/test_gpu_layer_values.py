@@ -32,3 +32,27 @@ def test_a_copied_layer_keeps_its_weights(cuda):
     for other in copies:
         assert torch.equal(other.forward(x), want)
     assert not torch.equal(layer.forward(x), want)
+
+
+@pytest.mark.parametrize("block,k", [(16, (1 << 28) + (1 << 20) + 40), (32, (1 << 29) + (1 << 21) + 72)])
+def test_product_of_rows_whose_scales_pass_32_bits(cuda, block, k):
+    """Rows that are zero but for 300 places, the last ones behind 2^31 bytes of scale tiles.  Zeros add nothing, so
+    the sum rounds 300 times at most."""
+    import neural_textures_b200 as nt
+    g = torch.Generator().manual_seed(block)
+    at = torch.cat((torch.randint(0, k, (280,), generator=g), k - 1 - torch.arange(0, 2000, 100))).unique().cuda()
+    value = torch.exp2(torch.randint(-3, 4, (2, at.numel()), generator=g).float()).cuda()
+    x = torch.zeros((1, k), dtype=torch.float16, device="cuda")
+    packed, values = [], []
+    for v in value:
+        x[0, at] = v.half()
+        packed.append(nt.mx4_quantize(x, block=block))
+        back = nt.mx4_dequantize(packed[-1], torch.float16)
+        values.append(f64(back[0, at]))
+        assert int(torch.count_nonzero(back)) == at.numel()
+        del back
+    got = float(nt.mx4_product(*packed, dtype=torch.float32))
+    want, size = float(values[0] @ values[1]), float(np.abs(values[0]) @ np.abs(values[1]))
+    far = (at >= k - 2001).cpu().numpy()
+    assert float(values[0][far] @ values[1][far]) > 1e-2 * size, "the far places count"
+    assert abs(got - want) <= 308 * U * size
