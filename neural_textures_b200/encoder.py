@@ -48,9 +48,14 @@ class LatentEncoder:
         self.encode(features, keep=True)
         p = tex.params()
         InvokeTraining(p, stream=stream)
-        d = tex.ggrads[self.grid]
+        # a latent's gradient is its error over the number of samples, or of latents where they are fewer: times that
+        # (a power of two) between the layers, where fp16 would lose it
+        w, h = tex.grid_sizes[self.grid]
+        d, scale = tex.ggrads[self.grid], 1.0
+        gain = 2.0 ** (min(p.num_samples, w * h).bit_length() - 1)
         for layer in reversed(self.layers):
-            d = layer.backward(d)
+            d = layer.backward(d, scale, gain)
+            scale, gain = scale * gain, 1.0
         self._optimize()
         InvokeOptimizeNetwork(p, stream=stream)
         for g in tex.ggrads:

@@ -384,7 +384,8 @@ class TexelLayer:
     gradient of the output and returns that of x; those of the parameters are in `grads`, in `parameters`' order.
     Its products run in 4 bits too, on matrices quantised along the other axis, in blocks of 32: their
     power-of-two scales hold gradients of any size, where E4M3 scales end at 2^-9.  The rounding to 4 bits is
-    passed straight through."""
+    passed straight through.  The gradient of x, and that of the norm's result before it, have x's type: in fp16 they
+    need the factors of backward where gradients are below 10^-4."""
 
     def __init__(self, channels_in: int, channels_out: int, groups: int, activation: str = "silu", block: int = 16,
                  device="cuda", seed: int = 0):
@@ -413,13 +414,21 @@ class TexelLayer:
             self._kept = (x, rows, mean, rstd)
         return out.view(*x.shape[:-1], out.shape[-1])
 
-    def backward(self, dout):
+    def backward(self, dout, scale: float = 1.0, gain: float = 1.0):
+        """`dout` holds `scale` times the gradient of the output, the result `scale * gain` times that of x, so that
+        fp16 holds it; powers of two cost no digits.  `grads` are the gradients themselves."""
         torch = _torch
+        if not 0 < scale < float("inf") or not 0 < gain < float("inf"):
+            raise ValueError(f"scale and gain must be positive, not {scale} and {gain}")
         x, rows, mean, rstd = self._kept
         d = dout.reshape(-1, dout.shape[-1])
-        dy = mx4_product(mx4_quantize(d), mx4_quantize(self.weight.t()), dtype=x.dtype)
-        dweight = mx4_product(mx4_quantize(d.t()), mx4_quantize(rows.t()), dtype=torch.float32)
+        dy = mx4_product(mx4_quantize(d), mx4_quantize(self.weight.t()), alpha=float(gain), dtype=x.dtype)
+        dweight = mx4_product(mx4_quantize(d.t()), mx4_quantize(rows.t()), alpha=1.0 / scale, dtype=torch.float32)
         dx, dgamma, dbeta = group_norm_backward(dy.view(x.shape), x, mean, rstd, self.groups, self.gamma, self.beta,
                                                 activation=self.activation)
-        self.grads = [dweight, d.float().sum(dim=0), dgamma, dbeta]
+        dbias = d.float().sum(dim=0)
+        for g, factor in ((dbias, scale), (dgamma, scale * gain), (dbeta, scale * gain)):
+            if factor != 1.0:
+                g.mul_(1.0 / factor)
+        self.grads = [dweight, dbias, dgamma, dbeta]
         return dx

@@ -56,3 +56,42 @@ def test_product_of_rows_whose_scales_pass_32_bits(cuda, block, k):
     far = (at >= k - 2001).cpu().numpy()
     assert float(values[0][far] @ values[1][far]) > 1e-2 * size, "the far places count"
     assert abs(got - want) <= 308 * U * size
+
+
+def test_encoder_gradients_of_many_samples(cuda, monkeypatch):
+    """The gradients of 262,144 samples that are off by about 0.01 are 10^-8 each, below fp16's smallest step: the
+    encoder's come out as those of 2^18 times larger ones, divided by 2^18, bit for bit."""
+    import neural_textures_b200 as nt
+    from neural_textures_b200 import encoder
+    from tests.model_utils import make_texture
+    tex = make_texture((512, 512), ((512, 512), (256, 256)), 8, 8, lattice=(512, 512), seed=3)
+    g = torch.Generator(device="cuda").manual_seed(8)
+    d = 1e-8 * torch.randn((512, 512, 8), generator=g, device="cuda")
+    features = torch.randn((512, 512, 32), generator=g, device="cuda").half()
+    monkeypatch.setattr(encoder, "InvokeTraining", lambda p, *a, stream=None: tex.ggrads[0].copy_(d))
+    enc = nt.LatentEncoder(tex, grid=0, features=32)
+    first, second = copy.deepcopy(enc.layers)
+    enc.train_step(features)
+    second.forward(first.forward(features, keep=True), keep=True)
+    first.backward(second.backward(d * 2.0 ** 18))
+    for layer, want in zip(enc.layers, (first, second)):
+        for got, large in zip(layer.grads, want.grads):
+            assert float(large.abs().max()) > 0
+            assert torch.equal(got, large * 2.0 ** -18)
+
+
+def test_layer_gradients_with_factors(cuda):
+    """A gain is that of the result alone, a scale is taken out of the parameters' gradients: bit for bit."""
+    import neural_textures_b200 as nt
+    layer = nt.TexelLayer(48, 24, groups=6, seed=5)
+    x, d = torch.randn((9, 13, 48), device="cuda").half(), torch.randn((9, 13, 24), device="cuda")
+    layer.forward(x, keep=True)
+    dx = layer.backward(d)
+    grads = layer.grads
+    tiny = layer.backward(d * 2.0 ** -30, gain=2.0 ** 30)
+    assert torch.equal(tiny, dx) and all(torch.equal(a, b * 2.0 ** -30) for a, b in zip(layer.grads, grads))
+    large = layer.backward(d * 2.0 ** 10, scale=2.0 ** 10, gain=2.0 ** -10)
+    assert torch.equal(large, dx) and all(torch.equal(a, b) for a, b in zip(layer.grads, grads))
+    for factors in ((0.0, 1.0), (1.0, -2.0), (float("nan"), 1.0), (1.0, float("inf"))):
+        with pytest.raises(ValueError, match="positive"):
+            layer.backward(d, *factors)
