@@ -108,12 +108,13 @@ __device__ __forceinline__ float2 rcp2(float2 a)
     return make_float2(a.y * r, a.x * r);
 }
 
-// 1 / (1 + exp(-z)).  Below -43 the true value is under 3e-19, where it is held.
+// 1 / (1 + exp(-z)) as e / (1 + e), e = exp(z): silu multiplies it by z, however far below 0, where e keeps its digits and
+// ends at 0.  Above 43 it is 1, where e is held.
 __device__ __forceinline__ float2 sigmoid2(float2 z)
 {
-    const float2 m = make_float2(fmaxf(z.x, -43.f), fmaxf(z.y, -43.f));
-    const float2 t = __fmul2_rn(m, f2(-1.44269504f));
-    return rcp2(__fadd2_rn(make_float2(ex2(t.x), ex2(t.y)), f2(1.f)));
+    const float2 t = __fmul2_rn(make_float2(fminf(z.x, 43.f), fminf(z.y, 43.f)), f2(1.44269504f));
+    const float2 e = make_float2(ex2(t.x), ex2(t.y));
+    return __fmul2_rn(e, rcp2(__fadd2_rn(e, f2(1.f))));
 }
 
 // The normal distribution's integral Phi(z), and exp(-z^2 / 2).  With x = |z| / sqrt 2, t = 1 / (1 + p x):

@@ -95,3 +95,57 @@ def test_layer_gradients_with_factors(cuda):
     for factors in ((0.0, 1.0), (1.0, -2.0), (float("nan"), 1.0), (1.0, float("inf"))):
         with pytest.raises(ValueError, match="positive"):
             layer.backward(d, *factors)
+
+
+# arguments of an activation, far ones among them
+FAR = [-3e38, -1e20, -1e4, -200.0, -104.0, -100.0, -88.5, -87.0, -60.0, -50.0, -43.5, -43.0, -42.5, -30.0, -12.0, -5.0, -1.0,
+       -1e-3, -1e-30, 0.0, 1e-30, 1e-3, 1.0, 5.0, 30.0, 60.0, 88.5, 200.0, 1e4, 1e20, 3e38]
+FLT_MIN = 2.0 ** -126
+
+
+def _far(act):
+    """(z, activation(z), its slope, both as fp32 holds them, their tolerances).  silu's exponential is rounded relative to its argument,
+    8 + |z| units; results below FLT_MIN may be 0.  gelu's integral of the normal distribution is good to 1.5e-7."""
+    z = np.array(FAR, np.float32).astype(np.float64)
+    with np.errstate(over="ignore"):
+        value, slope = (v.astype(np.float32).astype(np.float64) for v in (O.activate(z, act), O.slope(z, act)))
+    if act == "silu":
+        s = np.exp(-np.logaddexp(0, -z))
+        units = 2 * U * (8 + np.minimum(np.abs(z), 104))
+        return z, value, slope, units * np.abs(value) + 104 * FLT_MIN, units * s * (2 + np.minimum(np.abs(z), 104)) + 104 * FLT_MIN
+    bell = np.abs(z) * np.exp(-np.minimum(z * z, 2000) / 2)
+    tail = np.where(z < -16, 0.0, 1.5e-7)
+    return z, value, slope, tail * np.minimum(np.abs(z), 16) + 8 * U * np.abs(value), tail + 32 * U * (bell + 1) * (z > -16)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_activations_of_far_arguments(cuda, act):
+    """A map of zeros is normalised to zeros, so that z is beta and the gradient of beta the slope; zero codes leave
+    a product its bias."""
+    import neural_textures_b200 as nt
+    z, value, slope, value_tol, slope_tol = _far(act)
+    c = z.size
+    beta = torch.tensor(z, dtype=torch.float32, device="cuda")
+    x = torch.zeros((1, 1, 1, c), device="cuda")
+    y, mean, rstd = nt.group_norm(x, 1, None, beta, activation=act)
+    assert (np.abs(f64(y).ravel() - value) <= value_tol).all(), f64(y).ravel() - value
+    _, _, dbeta = nt.group_norm_backward(torch.ones_like(x), x, mean, rstd, 1, None, beta, activation=act)
+    assert (np.abs(f64(dbeta) - slope) <= slope_tol).all(), f64(dbeta) - slope
+    for m, k in ((1, 64), (1, 4096), (200, 64)):
+        a, b = nt.mx4_quantize(torch.zeros((m, k), device="cuda")), nt.mx4_quantize(torch.zeros((c, k), device="cuda"))
+        d = f64(nt.mx4_product(a, b, bias=beta, activation=act, dtype=torch.float32))
+        assert (np.abs(d - value) <= value_tol).all(), (m, k, d[0] - value)
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu"])
+def test_activations_of_infinities(cuda, act):
+    """+inf stays; -inf is 0 under relu and, as 0 x inf, NaN under silu and gelu; a NaN is one."""
+    import neural_textures_b200 as nt
+    inf = float("inf")
+    bias = torch.tensor([inf, -inf, float("nan"), 1.0], device="cuda")
+    q = nt.mx4_quantize(torch.zeros((4, 64), device="cuda"))
+    for m in (1, 200):
+        d = nt.mx4_product(nt.mx4_quantize(torch.zeros((m, 64), device="cuda")), q, bias=bias, activation=act, dtype=torch.float32)
+        assert (d[:, 0] == inf).all() and torch.isnan(d[:, 2]).all() and torch.isfinite(d[:, 3]).all()
+        low = d[:, 1]
+        assert {"none": (low == -inf).all(), "relu": (low == 0).all()}.get(act, torch.isnan(low).all())
