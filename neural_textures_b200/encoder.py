@@ -11,7 +11,7 @@ layers to their weights.  The other grid and the texture's network are optimised
 """
 from __future__ import annotations
 
-from .api import InvokeOptimizeNetwork, InvokeTraining, NeuralTexture, _on_device
+from .api import InvokeOptimizeAll, InvokeTraining, NeuralTexture, _on_device
 from .layers import TexelLayer
 
 
@@ -40,7 +40,7 @@ class LatentEncoder:
     @_on_device
     def train_step(self, features) -> None:
         """One step: latents from the features, the texture's training pass, gradients back through the layers,
-        Adam on them and on the texture's network.  The loss is added to tex.loss_accum.  Everything is queued on
+        Adam on them, on the texture's network and on its other grid.  The loss is added to tex.loss_accum.  Everything is queued on
         torch's current stream."""
         import torch
         tex = self.tex
@@ -57,9 +57,8 @@ class LatentEncoder:
             d = layer.backward(d, scale, gain)
             scale, gain = scale * gain, 1.0
         self._optimize()
-        InvokeOptimizeNetwork(p, stream=stream)
-        for g in tex.ggrads:
-            g.zero_()
+        tex.ggrads[self.grid].zero_()  # Adam leaves values without a gradient alone
+        InvokeOptimizeAll(p, stream=stream)
         tex.step += 1
 
     def _optimize(self):

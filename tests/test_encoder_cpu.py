@@ -66,3 +66,24 @@ def test_a_step_stays_on_the_current_stream(step):
     assert passes and all(stream == SIDE for _, stream in passes), passes
     order = [c[0] for c in calls]
     assert order.index("InvokeTraining") == 2 and order[3:5] == ["backward", "backward"]
+
+
+@pytest.mark.parametrize("grid", [0, 1])
+def test_a_step_optimises_the_other_grid(step, monkeypatch, grid):
+    """The texture's Adam sees the other grid's gradient and none of the encoded one, which it leaves alone then."""
+    from neural_textures_b200 import encoder
+    enc, calls = step
+    enc.grid = grid
+    enc.tex.grid_sizes, enc.tex.grids[grid] = [(4, 4), (4, 4)], torch.zeros(4, 4, 8)
+    enc.tex.ggrads = [torch.ones(4, 4, 8), torch.ones(4, 4, 8)]
+    seen = {}
+
+    def note(name):
+        return lambda p, *a, stream=None: seen.setdefault(name, [bool(g.any()) for g in enc.tex.ggrads])
+
+    for name in ("InvokeOptimizeNetwork", "InvokeOptimizeFeatures", "InvokeOptimizeAll"):
+        monkeypatch.setattr(encoder, name, note(name), raising=False)
+    enc.train_step(torch.ones(4, 4, 8))
+    features = [v for k, v in seen.items() if k in ("InvokeOptimizeFeatures", "InvokeOptimizeAll")]
+    assert features == [[g != grid for g in range(2)]]
+    assert enc.tex.step == 1 and not enc.tex.ggrads[grid].any()

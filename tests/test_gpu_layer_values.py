@@ -149,3 +149,22 @@ def test_activations_of_infinities(cuda, act):
         assert (d[:, 0] == inf).all() and torch.isnan(d[:, 2]).all() and torch.isfinite(d[:, 3]).all()
         low = d[:, 1]
         assert {"none": (low == -inf).all(), "relu": (low == 0).all()}.get(act, torch.isnan(low).all())
+
+
+def test_encoder_step_optimises_the_other_grid(cuda):
+    """Beside a plain texture that starts from the encoded latents: its step moves the other grid by as much.  The two
+    passes add in no fixed order, and a first step of Adam has a gradient's sign, so one value in 100 may differ."""
+    import neural_textures_b200 as nt
+    from tests.model_utils import make_texture
+    make = lambda: make_texture((64, 64), ((32, 32), (16, 16)), 8, 8, lattice=(32, 32), seed=7)
+    tex, plain = make(), make()
+    features = tex.target.view(32, 2, 32, 2, 8).permute(0, 2, 1, 3, 4).reshape(32, 32, 32).contiguous()
+    enc = nt.LatentEncoder(tex, grid=0, features=32)
+    before = tex.grids[1].clone()
+    plain.grids[0].copy_(enc.encode(features))
+    enc.train_step(features)
+    assert torch.equal(tex.grids[0], plain.grids[0])
+    plain.train_step()
+    assert float((plain.grids[1] != before).float().mean()) > 0.9
+    assert float((plain.grids[1] == tex.grids[1]).float().mean()) >= 0.99
+    assert not any(g.any() for g in tex.ggrads)
