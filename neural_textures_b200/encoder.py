@@ -7,10 +7,12 @@ NeuralTexture, trained through the texture's own training pass.
     enc.encode(features)             # tex.grids[0] holds the latents
 
 The training pass (InvokeTraining) leaves dL / dlatents in tex.ggrads; here it goes back through the
-layers to their weights.  The other grid and the texture's network are optimised as always.
+layers to their weights.  The other grid and the texture's network are optimised as always.  The encoded grid is
+one of fp16 values without mips.
 """
 from __future__ import annotations
 
+from . import _native as N
 from .api import InvokeOptimizeAll, InvokeTraining, NeuralTexture, _on_device
 from .layers import TexelLayer
 
@@ -20,14 +22,22 @@ class LatentEncoder:
                  lr: float = 2e-3, beta1: float = 0.9, beta2: float = 0.99, eps: float = 1e-8, seed: int = 0):
         import torch
         self.tex, self.grid, self.device = tex, grid, tex.device
+        self._check()
         self.layers = [TexelLayer(features, hidden, groups=1, activation="none", block=block, device=tex.device, seed=seed),
                        TexelLayer(hidden, tex.C, groups=groups, activation="silu", block=block, device=tex.device, seed=seed + 1)]
         self.adam, self.step = (lr, beta1, beta2, eps), 0
         self.moments = [[(torch.zeros_like(p), torch.zeros_like(p)) for p in l.parameters] for l in self.layers]
 
+    def _check(self):
+        if self.tex.latent_format != N.NT_LATENT_GRID_F16:
+            raise ValueError("a LatentEncoder fills fp16 grids, not block records")
+        if self.tex.num_mips[self.grid] > 1:
+            raise ValueError(f"a LatentEncoder fills grids of one level, not of {self.tex.num_mips[self.grid]}")
+
     @_on_device
     def encode(self, features, keep: bool = False):
         """Latents of `features` [h][w][F] (fp16), written into the texture's grid."""
+        self._check()
         x = features
         for layer in self.layers:
             x = layer.forward(x, keep)

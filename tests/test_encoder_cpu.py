@@ -87,3 +87,25 @@ def test_a_step_optimises_the_other_grid(step, monkeypatch, grid):
     features = [v for k, v in seen.items() if k in ("InvokeOptimizeFeatures", "InvokeOptimizeAll")]
     assert features == [[g != grid for g in range(2)]]
     assert enc.tex.step == 1 and not enc.tex.ggrads[grid].any()
+
+
+@pytest.mark.parametrize("change,needle", [(dict(num_mips=[3, 1]), "one level"), (dict(latent_format=1), "fp16 grids")])
+def test_encoder_refuses_textures_that_it_cannot_fill(step, change, needle):
+    """Of a chain of mips only the first level would be encoded; block records have no grid to write. Found when the
+    encoder is made and, since a texture can change its form, at every call; nothing is written or queued then."""
+    from neural_textures_b200 import encoder
+    enc, calls = step
+    with pytest.raises(ValueError, match=needle):
+        encoder.LatentEncoder(FakeTexture(**change))
+    enc.tex.__dict__.update(change)
+    for call in (enc.encode, enc.train_step):
+        with pytest.raises(ValueError, match=needle):
+            call(torch.ones(4, 4, 8))
+    assert not calls and not enc.tex.grids[0].any()
+
+
+def test_encoder_takes_a_texture_whose_other_grid_has_mips(step):
+    enc, calls = step
+    enc.tex.num_mips = [1, 2]
+    enc.train_step(torch.ones(4, 4, 8))
+    assert enc.tex.step == 1
