@@ -353,9 +353,11 @@ class NeuralTexture:
         self.lod = 0.0  # mip coordinate of every sample (NtKernelParams.lod)
         f16, f32 = torch.float16, torch.float32
         z = lambda shape, dt: torch.zeros(shape, dtype=dt, device=self.device)
-        # each grid is a mip chain (level 0 first); grids[g] views level 0 as [h][w][C]
-        self.grid_chains = [z(mip_chain_texels(w, h, n) * self.C, f16)
-                            for (w, h), n in zip(self.grid_sizes, self.num_mips)]
+        # each grid is a mip chain (level 0 first); grids[g] views level 0 as [h][w][C].  Memory in whole rows of 256
+        # (_mx4_rows), zero past the chain
+        lengths = [mip_chain_texels(w, h, n) * self.C for (w, h), n in zip(self.grid_sizes, self.num_mips)]
+        self._grid_rows = [z((-(-n // 256), 256), f16) for n in lengths]
+        self.grid_chains = [r.view(-1)[:n] for r, n in zip(self._grid_rows, lengths)]
         self.grids = [c[:w * h * self.C].view(h, w, self.C) for c, (w, h) in zip(self.grid_chains, self.grid_sizes)]
         shaped = lambda c, g: c.view(g.shape) if c.numel() == g.numel() else c
         self.ggrads = [shaped(z(c.numel(), f32), g) for c, g in zip(self.grid_chains, self.grids)]
@@ -451,7 +453,8 @@ class NeuralTexture:
     @_on_device
     def export_mx4(self, block: int = 16, stream=None):
         """The fp16 grids (all levels) in 4-bit microscaled form, one Mx4Tensor per grid of rows of one texel row's
-        values (level 0) or of 256 (chains): 4.5 bits a value in blocks of 16, 4.25 in blocks of 32."""
+        values (level 0 alone, 32 values and more) or of 256 (the last one filled up with zeros): 4.5 bits a value
+        in blocks of 16, 4.25 in blocks of 32, in whole tiles of 128 rows of scales.  `stream`: as in layers.py."""
         from .layers import mx4_quantize
         if self.latent_format != N.NT_LATENT_GRID_F16:
             raise RuntimeError("export_mx4 stores fp16 grids")
@@ -459,7 +462,7 @@ class NeuralTexture:
 
     @_on_device
     def from_mx4(self, packed, stream=None):
-        """Grids from export_mx4's tensors (of a texture of the same sizes)."""
+        """Grids from export_mx4's tensors (of a texture of the same sizes).  `stream`: as in layers.py."""
         from .layers import mx4_dequantize
         if self.latent_format != N.NT_LATENT_GRID_F16:
             raise RuntimeError("from_mx4 fills fp16 grids")
@@ -468,10 +471,11 @@ class NeuralTexture:
 
     def _mx4_rows(self, g: int):
         w, h = self.grid_sizes[g]
-        if self.num_mips[g] == 1:
+        if self.num_mips[g] == 1 and w * self.C >= 32:
             return self.grid_chains[g].view(h, w * self.C)
-        n = self.grid_chains[g].numel()
-        return self.grid_chains[g].view(-1, 256 if n % 256 == 0 else self.C)
+        if self._grid_rows[g].data_ptr() != self.grid_chains[g].data_ptr():
+            raise RuntimeError(f"grid_chains[{g}] was replaced: write into it instead")
+        return self._grid_rows[g]
 
     # -- initialisation -------------------------------------------------------------------
     @_on_device
