@@ -73,8 +73,8 @@ _shapes = {}
 
 
 def _new(shape, dtype, device):
-    """torch.empty(shape), at less than half its host time: empty_like of a one-element tensor
-    expanded to the shape, kept per shape."""
+    """torch.empty(shape) on a device with its index, at less than half its host time: empty_like of a one-element
+    tensor expanded to the shape, kept per shape."""
     key = (shape, dtype, device)
     t = _shapes.get(key)
     if t is None:
@@ -280,6 +280,9 @@ class Mx4Tensor:
         torch = _torch or _lazy_torch()
         if block not in (16, 32) or rows < 0 or cols < 1:
             raise ValueError(f"{rows} x {cols} in blocks of {block} is not a 4-bit matrix")
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
         pitch = -(-cols // 32) * 16
         return cls(_new((rows, pitch), torch.uint8, device),
                    _new((-(-rows // 128) * -(-cols // (4 * block)) * 512,), torch.uint8, device), rows, cols, block)
