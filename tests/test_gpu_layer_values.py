@@ -168,3 +168,30 @@ def test_encoder_step_optimises_the_other_grid(cuda):
     assert float((plain.grids[1] != before).float().mean()) > 0.9
     assert float((plain.grids[1] == tex.grids[1]).float().mean()) >= 0.99
     assert not any(g.any() for g in tex.ggrads)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("offset", [20.0, 1000.0])
+def test_group_norm_statistics_behind_a_black_border(cuda, offset, dtype):
+    """Every thread's first texels are 0 and the 8,000 after them `offset` deviations away: the variance must not
+    be a difference of sums about that 0. Rounding errors of n values add like sqrt(n) = 91 units; sums about a
+    pivot within the values so far are at most 4 times the centred ones: 364 of the 512 units of SUM. The mean is one
+    fp32 number of the offset's size."""
+    import neural_textures_b200 as nt
+    g = torch.Generator(device="cuda").manual_seed(5)
+    image = offset + torch.randn((512, 512, 64), generator=g, device="cuda")
+    image[0] = 0
+    image = image.to(dtype)
+    x = image.expand(150, 512, 512, 64)  # as many images as leave one block to each
+    y, mean, rstd = nt.group_norm(x, 64)
+    v = image.double().view(-1, 64)
+    want = v.mean(dim=0)
+    var = (v - want).square().mean(dim=0)
+    wrstd = (var + 1e-5).rsqrt()
+    assert torch.equal(mean[0].expand_as(mean), mean) and torch.equal(rstd[0].expand_as(rstd), rstd)
+    assert float((mean[0].double() - want).abs().max()) <= 16 * U * offset
+    assert float((rstd[0].double() / wrstd - 1).abs().max()) <= 512 * U, float((rstd[0].double() / wrstd - 1).abs().max())
+    z = (image.double() - want) * wrstd
+    tol = 512 * U * (1 + z.abs()) + 16 * U * offset * wrstd.max()
+    tol = tol + O.HALF_ULP[dtype] * (z.abs() + tol)
+    assert bool(((y[149].double() - z).abs() <= tol).all())
