@@ -195,3 +195,23 @@ def test_group_norm_statistics_behind_a_black_border(cuda, offset, dtype):
     tol = 512 * U * (1 + z.abs()) + 16 * U * offset * wrstd.max()
     tol = tol + O.HALF_ULP[dtype] * (z.abs() + tol)
     assert bool(((y[149].double() - z).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_group_norm_gradient_sums_of_equal_terms(cuda, act):
+    """A gradient of 0.1 everywhere, 11,000 texels a thread: adding equal terms one by one rounds one way.  The bound
+    is SUM of the magnitudes, 512 units, as for short sums."""
+    import neural_textures_b200 as nt
+    g = torch.Generator(device="cuda").manual_seed(6)
+    image = torch.randn((512, 512, 64), generator=g, device="cuda")
+    x = image.expand(150, 512, 512, 64)
+    dy = torch.full((64,), 0.1, device="cuda").expand(150, 512, 512, 64)
+    mean, rstd = torch.zeros((150, 8), device="cuda"), torch.ones((150, 8), device="cuda")
+    _, dgamma, dbeta = nt.group_norm_backward(dy, x, mean, rstd, 8, activation=act)
+    h = image.double().view(-1, 64)
+    s = torch.sigmoid(h)
+    slope = s * (1 + h * (1 - s)) if act == "silu" else torch.ones_like(h)
+    e = 150 * float(np.float32(0.1)) * slope
+    for got, terms in ((dbeta, e), (dgamma, e * h)):
+        err, size = (got.double() - terms.sum(dim=0)).abs(), terms.abs().sum(dim=0)
+        assert bool((err <= 512 * U * size).all()), float((err / size).max()) / U
