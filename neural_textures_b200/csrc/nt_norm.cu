@@ -185,13 +185,19 @@ nt_status check_map(const NtFeatureMap &f, const char *name, const NtGroupNorm *
     NT_LAYER_REQUIRE(f.data && is_aligned(f.data, size), "%s must be a non-null device pointer aligned to its element", name);
     NT_LAYER_REQUIRE(f.image_stride >= 0 && f.row_stride >= 0 && f.texel_stride >= 0, "%s: strides must be non-negative", name);
     if (written) {
-        // each axis steps over everything inside it
+        // each axis steps over everything inside it, whatever their order
+        struct Axis {
+            int64_t stride;
+            int32_t size;
+            const char *what;
+        } axes[3] = {{f.texel_stride, p->width, "texels"}, {f.row_stride, p->height, "rows"}, {f.image_stride, p->images, "images"}};
+        std::stable_sort(axes, axes + 3, [](const Axis &a, const Axis &b) { return a.stride < b.stride; });
         int64_t inner = p->channels;
-        NT_LAYER_REQUIRE(p->width == 1 || f.texel_stride >= inner, "%s: texels overlap", name);
-        if (p->width > 1) inner += (p->width - 1) * f.texel_stride;
-        NT_LAYER_REQUIRE(p->height == 1 || f.row_stride >= inner, "%s: rows overlap", name);
-        if (p->height > 1) inner += (p->height - 1) * f.row_stride;
-        NT_LAYER_REQUIRE(p->images <= 1 || f.image_stride >= inner, "%s: images overlap", name);
+        for (const Axis &a : axes) {
+            if (a.size <= 1) continue;
+            NT_LAYER_REQUIRE(a.stride >= inner, "%s: %s overlap", name, a.what);
+            inner += (a.size - 1) * a.stride;
+        }
     }
     return NT_OK;
 }

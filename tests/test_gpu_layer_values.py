@@ -215,3 +215,18 @@ def test_group_norm_gradient_sums_of_equal_terms(cuda, act):
     for got, terms in ((dbeta, e), (dgamma, e * h)):
         err, size = (got.double() - terms.sum(dim=0)).abs(), terms.abs().sum(dim=0)
         assert bool((err <= 512 * U * size).all()), float((err / size).max()) / U
+
+
+def test_group_norm_into_a_transposed_map(cuda):
+    import neural_textures_b200 as nt
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn((2, 9, 13, 24), generator=g, device="cuda").half()
+    want, mean, rstd = nt.group_norm(x, 3, activation="relu")
+    wdx, _, _ = nt.group_norm_backward(x, x, mean, rstd, 3, activation="silu")
+    for axes in ((0, 2, 1, 3), (1, 2, 0, 3), (2, 1, 0, 3)):
+        back = [axes.index(i) for i in range(4)]
+        y, dx = (torch.empty([x.shape[a] for a in axes], dtype=x.dtype, device="cuda").permute(back) for _ in range(2))
+        nt.group_norm(x, 3, activation="relu", out=y)
+        nt.group_norm_backward(x, x, mean, rstd, 3, activation="silu", out=dx)
+        assert float((y.float() - want.float()).abs().max()) <= 2.0 ** -10 * float(want.abs().max())
+        assert float((dx.float() - wdx.float()).abs().max()) <= 2.0 ** -10 * float(wdx.abs().max())
