@@ -448,7 +448,8 @@ struct Threads {
         for (int j = 0; j < V; ++j) {
             const float a = j & 1 ? s1[j / 2].y : s1[j / 2].x, b = j & 1 ? s2[j / 2].y + before[j / 2].y : s2[j / 2].x + before[j / 2].x;
             mean[j] = fmaf(a, inv, -(j & 1 ? pivot[j / 2].y : pivot[j / 2].x));
-            m2[j] = fmaxf(b - a * a * inv, 0.f);
+            const float squares = fmaf(-a * inv, a, b);
+            m2[j] = squares < 0.f ? 0.f : squares == squares ? squares : b;  // b: infinite where the squares overflow
             if (!WHOLE) scratch[row * L.p.channels + c + j] = make_float2(mean[j], m2[j]);
             shift += mean[j] - mean[0];
         }

@@ -230,3 +230,16 @@ def test_group_norm_into_a_transposed_map(cuda):
         nt.group_norm_backward(x, x, mean, rstd, 3, activation="silu", out=dx)
         assert float((y.float() - want.float()).abs().max()) <= 2.0 ** -10 * float(want.abs().max())
         assert float((dx.float() - wdx.float()).abs().max()) <= 2.0 ** -10 * float(wdx.abs().max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("period", [1, 3, 256, 512])
+def test_group_norm_of_values_whose_squares_overflow(cuda, dtype, period):
+    """+-10^20 in turn: the variance is past fp32, so rstd is 0 (and y beta) or a NaN, never that of a small variance."""
+    import neural_textures_b200 as nt
+    sign = 1 - 2.0 * ((torch.arange(64 * 64, device="cuda") // period) % 2)
+    x = (1e20 * sign)[:, None].repeat(1, 8).view(1, 64, 64, 8).to(dtype)
+    for images in (1, 150):
+        y, mean, rstd = nt.group_norm(x.expand(images, 64, 64, 8), 2)
+        assert not (rstd > 0).any(), rstd
+        assert not (y.abs() > 0).any()
