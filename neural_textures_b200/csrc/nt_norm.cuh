@@ -289,10 +289,10 @@ struct Threads {
         }
     };
 
-    // use(slot, i) for texels 0 .. count - 1, after before(i) for every fourth i at least.  Afterwards the last kDepth of
-    // them are still in the ring, texel i in slot (i - near) % kDepth.
-    template <class Use, class Before>
-    __device__ __forceinline__ void each_forth(int c, int count, int near, int slot0, Use use, Before before) const
+    // use(slot, i) for texels 0 .. count - 1.  In front of texel `stop`, a multiple of 4, stop = pause(stop).  Afterwards the
+    // last kDepth texels are still in the ring, texel i in slot (i - near) % kDepth.
+    template <class Use, class Pause>
+    __device__ __forceinline__ void each_forth(int c, int count, int near, int slot0, Use use, int stop, Pause pause) const
     {
         const uint32_t keep = kept + slot0 * kSlot, ring = kept + L.keep * kSlot;
         const Source src(*this, c);
@@ -305,19 +305,24 @@ struct Threads {
             fetch_commit();
         }
         fetch_wait<kDepth>();
+        int i = 0;
+        while (i < near) {  // runs between two stops: looking for one at every texel cost 17% of 200 x 64 x 64 x 32 fp16
+            const int end = min(near, stop);
 #pragma unroll 2
-        for (int i = 0; i < near; ++i) {
-            before(i);
-            use(keep + i * kSlot, i);
+            for (; i < end; ++i) use(keep + i * kSlot, i);
+            if (i == stop && i < count) stop = pause(i);
         }
+        while (i < count) {
+            const int end = min(count, stop);
 #pragma unroll 2
-        for (int i = near; i < count; ++i) {
-            const uint32_t slot = ring + ((i - near) & (kDepth - 1)) * kSlot;
-            before(i);
-            fetch_wait<kDepth - 1>();
-            use(slot, i);
-            if (i + kDepth < count) src.get(slot, i + kDepth, again);
-            fetch_commit();
+            for (; i < end; ++i) {
+                const uint32_t slot = ring + ((i - near) & (kDepth - 1)) * kSlot;
+                fetch_wait<kDepth - 1>();
+                use(slot, i);
+                if (i + kDepth < count) src.get(slot, i + kDepth, again);
+                fetch_commit();
+            }
+            if (i == stop && i < count) stop = pause(i);
         }
     }
 
@@ -348,10 +353,10 @@ struct Threads {
         for (int i = near - 1; i >= 0; --i) use(keep + i * kSlot, i);
     }
 
-    // use(slot, i) for every texel, nothing kept: texels 0 .. count - 1 (before(i) as above), or backwards.  The ring's slots are constants of an
+    // use(slot, i) for every texel, nothing kept: texels 0 .. count - 1 (with stops as above), or backwards.  The ring's slots are constants of an
     // unrolled loop.
-    template <bool REVERSED, class Use, class Before>
-    __device__ __forceinline__ void each_fresh(int c, int count, Use use, Before before) const
+    template <bool REVERSED, class Use, class Pause>
+    __device__ __forceinline__ void each_fresh(int c, int count, Use use, int stop, Pause pause) const
     {
         const Source src(*this, c);
         const uint64_t policy = REVERSED ? policy_once() : policy_again();
@@ -362,9 +367,9 @@ struct Threads {
             fetch_commit();
         }
         int i = 0;
-        static_assert(kDepth == 4, "before(i)");
+        static_assert(kDepth == 4, "a stop is a multiple of it");
         for (; i + 2 * kDepth <= count; i += kDepth) {
-            before(i);
+            if (i == stop) stop = pause(i);
 #pragma unroll
             for (int u = 0; u < kDepth; ++u) {
                 fetch_wait<kDepth - 1>();
@@ -375,7 +380,7 @@ struct Threads {
         }
 #pragma unroll 1
         for (; i < count; i += kDepth) {
-            before(i);
+            if (i == stop) stop = pause(i);
 #pragma unroll
             for (int u = 0; u < kDepth; ++u) {
                 fetch_wait<kDepth - 1>();
@@ -386,19 +391,16 @@ struct Threads {
         }
     }
 
-    struct Nothing {
-        __device__ __forceinline__ void operator()(int) const {}
-    };
-    template <class Use, class Before = Nothing>
-    __device__ __forceinline__ void every_forth(int c, int count, int near, int slot0, Use use, Before before = {}) const
+    template <class Use, class Pause>
+    __device__ __forceinline__ void every_forth(int c, int count, int near, int slot0, Use use, int stop, Pause pause) const
     {
-        if constexpr (PHASE == kSums) each_fresh<false>(c, count, use, before);
-        else each_forth(c, count, near, slot0, use, before);
+        if constexpr (PHASE == kSums) each_fresh<false>(c, count, use, stop, pause);
+        else each_forth(c, count, near, slot0, use, stop, pause);
     }
     template <class Use>
     __device__ __forceinline__ void every_back(int c, int count, int near, int slot0, bool fresh, Use use) const
     {
-        if constexpr (PHASE == kApply) each_fresh<true>(c, count, use, Nothing());
+        if constexpr (PHASE == kApply) each_fresh<true>(c, count, use, -1, [](int) { return -1; });
         else each_back(c, count, near, slot0, fresh, use);
     }
 
@@ -410,7 +412,6 @@ struct Threads {
         // texels cost 2.5% of the variance.  The squares of 64 texels are added to those before them at once: long
         // chains of equal terms round one way.
         float2 pivot[P] = {}, s1[P] = {}, s2[P] = {}, before[P] = {};  // pivot: its negative; before: squares
-        uint32_t next = 4;
         bool begun = false;
         auto add = [&](uint32_t slot, int) {
             float2 f[P];
@@ -427,9 +428,7 @@ struct Threads {
                 s2[j] = __ffma2_rn(d, d, s2[j]);
             }
         };
-        every_forth(c, count, near, slot0, add, [&](int i) {
-            if ((uint32_t)i != next) return;
-            next = next < 64 ? 4 * next : next + 64;
+        every_forth(c, count, near, slot0, add, 4, [&](int i) {
             const float inv = __fdividef(-1.f, (float)i);
 #pragma unroll
             for (int j = 0; j < P; ++j) {  // up by -d: s1' = s1 + i d, s2' = s2 + 2 d s1 + i d^2 = s2 + d (s1 + s1')
@@ -440,6 +439,7 @@ struct Threads {
                 s1[j] = t;
                 pivot[j] = to;
             }
+            return i < 64 ? 4 * i : i + 64;
         });
         // (mean, centred squares) of each channel, or of the vector about the mean of its channels
         const float inv = count > 0 ? __fdividef(1.f, (float)count) : 0.f;
@@ -509,11 +509,11 @@ struct Threads {
                 s1[j] = __fadd2_rn(s1[j], e);
                 s2[j] = __ffma2_rn(e, h, s2[j]);
             }
-        }, [&](int i) {
-            if (i % 256 || i == 0) return;
+        }, 256, [&](int i) {
             put_sums(i > 256);
 #pragma unroll
             for (int j = 0; j < P; ++j) s1[j] = s2[j] = f2(0.f);
+            return i + 256;
         });
         put_sums(count > 256);
     }
