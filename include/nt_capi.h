@@ -515,7 +515,7 @@ typedef enum NtActivation {
 
 /* A feature map: element (n, y, x, c) is data[n * image_stride + y * row_stride +
  * x * texel_stride + c], strides in elements.  Maps that are read may have any strides (0 repeats
- * a texel, a row or an image); maps that are written must not overlap themselves. */
+ * a texel, a row or an image); maps that are written must not overlap themselves, their axes in any order. */
 typedef struct NtFeatureMap {
     void *data;
     int64_t image_stride;
@@ -526,12 +526,12 @@ typedef struct NtFeatureMap {
 /* Group normalisation.  Per image n and group g of channels / groups consecutive channels, over
  * the group's values on all texels: mean, rstd = 1 / sqrt(variance + epsilon) (biased variance);
  *   h = (x - mean) rstd,  z = gamma[c] h + beta[c],  y = activation(z).
- * Statistics and sums are fp32 (centred, so a large common offset costs no digits); y is rounded
- * once.  A NaN or an infinity makes its own group NaN and no other.  Results do not depend on
+ * Statistics and sums are fp32 (about means of the data, so a large common offset costs no digits, in chains of
+ * at most a few hundred terms); y is rounded once.  A NaN or an infinity makes its own group NaN and no other.  Results do not depend on
  * the order in which thread blocks run. */
 #define NT_GROUP_NORM_MAX_CHANNELS 8192
 typedef struct NtGroupNorm {
-    int32_t images;   /* may be 0: nothing to do (backward: dgamma = dbeta = 0) */
+    int32_t images;   /* 0 .. 65535; 0: nothing to do (backward: dgamma = dbeta = 0) */
     int32_t height;
     int32_t width;    /* height * width < 2^31 */
     int32_t channels; /* 1 .. NT_GROUP_NORM_MAX_CHANNELS, a multiple of groups */

@@ -33,13 +33,13 @@ struct Plan {
 // A cluster costs about 1 us over a single block; two launches let every SM compute, but take the host 3 us more.  A
 // turn of a block (a vector for each of its threads, both passes) takes about 0.35 us forward and 0.6 us backward.
 // So an image is split until a block has four turns, and takes two launches where the largest cluster would
-// leave it more than kTurns.  On the device, fp16, forward: 64 x 64 x 64 (4 turns) 7.1 us in a cluster of 16 and 6.6 us in two
-// launches, 96 x 96 x 64 (9 turns) 9.2 and 6.6 us; backward: 64 x 64 x 64 (5.3 turns) 10.8 and 9.1 us.
+// leave it more than kTurns.  On the device, fp16, forward: 64 x 64 x 64 (4 turns) 7.4 us in a cluster of 16 and 6.8 us in two
+// launches, 96 x 96 x 64 (9 turns) 9.5 and 6.9 us; backward: 64 x 64 x 64 (5.3 turns) 10.8 and 9.3 us.
 constexpr int kForwardTurns = 8, kBackwardTurns = 4;
 constexpr int kApplyTurns = 16;  // of a block of the second launch: enough of them that fast SMs take more
 
 // Channels of a vector: up to 16 bytes of them, and up to 4 where vectors cross groups, whose per-channel values take
-// the registers of a second block on the SM otherwise (3x83x138x48 fp16 of 8 groups: 14.2 us in vectors of 8, 9.2 in 4).
+// the registers of a second block on the SM otherwise (3x83x138x48 fp16 of 8 groups: 14.2 us in vectors of 8, 9.4 in 4).
 int vector_width(const NtGroupNorm *p)
 {
     int v = 16 / layer_dtype_size(p->dtype);

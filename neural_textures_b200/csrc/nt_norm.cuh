@@ -20,7 +20,7 @@
 // All sums are joined in a fixed order.
 //
 // Bound by HBM (2 to 3 readings of a map in all) and, in the second pass, by issue slots and the special-function unit.
-// 1024 x 1024 x 64 fp16 with SiLU, one B200: 68 us forward (25 sums, 5.0 TB/s; 43 result), 115 us backward.
+// 1024 x 1024 x 64 fp16 with SiLU, one B200: 68.5 us forward (25 sums, 5.3 TB/s; 43 result), 117 us backward.
 #pragma once
 
 #include "nt_layer_common.cuh"

@@ -36,7 +36,7 @@ class LatentEncoder:
 
     @_on_device
     def encode(self, features, keep: bool = False):
-        """Latents of `features` [h][w][F] (fp16), written into the texture's grid."""
+        """Latents of `features` [h][w][F] (fp16), written into the texture's grid on torch's current stream."""
         self._check()
         x = features
         for layer in self.layers:
