@@ -353,8 +353,8 @@ struct Threads {
         for (int i = near - 1; i >= 0; --i) use(keep + i * kSlot, i);
     }
 
-    // use(slot, i) for every texel, nothing kept: texels 0 .. count - 1 (with stops as above), or backwards.  The ring's slots are constants of an
-    // unrolled loop.
+    // use(slot, i) for every texel, nothing kept: texels 0 .. count - 1 (with stops as above), or backwards.  The ring's slots
+    // are constants of an unrolled loop.
     template <bool REVERSED, class Use, class Pause>
     __device__ __forceinline__ void each_fresh(int c, int count, Use use, int stop, Pause pause) const
     {
@@ -485,7 +485,7 @@ struct Threads {
     {
         float2 s1[P] = {}, s2[P] = {}, shift[P], rstd[P], gamma[P], beta[P];
         // In chains of 256, added up in shared memory, as long chains of equal terms (a broadcast dy) round one way: 11,000
-        // of them cost 10^-4.  Chains of 64 made 1024 x 1024 x 64 fp16 2 us slower: the stores conflict in their banks.
+        // of them cost 10^-4.  Chains of 64 cost 1024 x 1024 x 64 fp16 another 0.5 us: the stores conflict in their banks.
         float2 *const sums = scratch + row * L.p.channels + c;
         auto put_sums = [&](bool add) {
 #pragma unroll

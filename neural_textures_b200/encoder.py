@@ -50,8 +50,8 @@ class LatentEncoder:
     @_on_device
     def train_step(self, features) -> None:
         """One step: latents from the features, the texture's training pass, gradients back through the layers,
-        Adam on them, on the texture's network and on its other grid.  The loss is added to tex.loss_accum.  Everything is queued on
-        torch's current stream."""
+        Adam on them, on the texture's network and on its other grid.  The loss is added to tex.loss_accum.
+        Everything is queued on torch's current stream."""
         import torch
         tex = self.tex
         stream = torch.cuda.current_stream(self.device).cuda_stream
